@@ -38,6 +38,8 @@ DEV_BAD_WEIGHTS = 0x40
 F16 = 0
 BF16 = 1
 MAX_EXPERTS = 1024
+GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
+ACT_NONE, ACT_SWIGLU = 0, 1
 
 
 class MoEB200Error(RuntimeError):
@@ -128,6 +130,22 @@ def lib() -> ctypes.CDLL:
     L.moe_b200_ep_epoch.argtypes = [vp]
     L.moe_b200_unpermute.restype = cint
     L.moe_b200_unpermute.argtypes = [vp, vp, vp, cint, cint, cint, cint, vp, vp]
+    i64, f32 = ctypes.c_int64, ctypes.c_float
+    L.moe_b200_block_norm.restype = cint
+    L.moe_b200_block_norm.argtypes = [vp, i64, vp, i64, cint, vp, vp, vp, cint, f32, f32, cint, cint, cint, vp, vp, vp]
+    L.moe_b200_block_norm_backward_workspace_bytes.restype = sz
+    L.moe_b200_block_norm_backward_workspace_bytes.argtypes = [cint, cint, cint]
+    L.moe_b200_block_norm_backward.restype = cint
+    L.moe_b200_block_norm_backward.argtypes = [vp, vp, vp, i64, cint, vp, i64, vp, vp, vp, cint, f32, f32, cint, cint,
+                                               cint, vp, vp, vp, vp, vp, vp, sz, vp]
+    for f in (L.moe_b200_grouped_mm, L.moe_b200_grouped_mm_dgrad):
+        f.restype = cint
+        f.argtypes = [vp, vp, vp, cint, cint, cint, cint, cint, vp, cint, vp, vp]
+    L.moe_b200_grouped_mm_wgrad.restype = cint
+    L.moe_b200_grouped_mm_wgrad.argtypes = [vp, vp, vp, cint, cint, cint, cint, cint, vp, vp]
+    L.moe_b200_expert_linear_w4.restype = cint
+    L.moe_b200_expert_linear_w4.argtypes = [vp, cint, vp, cint, cint, cint, cint, cint, vp, vp, vp, cint, cint, cint,
+                                            vp, vp]
     _lib = L
     return L
 
@@ -456,4 +474,311 @@ def ep_layout(all_counts, rank, expert_first, out=None, stream=None):
     first = (ctypes.c_int32 * (N + 1))(*expert_first)
     _check(lib().moe_b200_ep_layout(_ptr(all_counts), N, E, rank, first, _ptr(out[0]), _ptr(out[1]),
                                     _ptr(out[2]), _ptr(out[3]), _stream_handle(stream)), "ep_layout")
+    return out
+
+
+# --------------------------------------------------------------------------
+# Norms around the block, expert products and their gradients, 4-bit weights
+# --------------------------------------------------------------------------
+
+def _refuse(what: str, why: str):
+    raise MoEB200Error(ERR_INVALID_ARG, f"{what}: {why}")
+
+
+def _rows(what, name, t, shape, dtype, strided=False):
+    """Checks a tensor's shape, type and layout (strided: rows may lie apart)."""
+    if t.shape != shape or t.dtype != dtype:
+        _refuse(what, f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if not t.is_contiguous() and not (strided and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+        _refuse(what, f"{name} must be contiguous" + (" or have contiguous rows that do not overlap" if strided else ""))
+
+
+def _same_device(what, *tensors):
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        _refuse(what, f"tensors must be on a CUDA device, got {dev}")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            _refuse(what, f"tensors on {dev} and {t.device}")
+    return dev
+
+
+def _enqueue(what, fn, dev, stream, fresh, *args):
+    """Calls fn(*args, stream) with `dev` current.  `fresh`: tensors that this
+    call allocated, which the allocator must not hand out again before the
+    work on `stream` is done."""
+    import torch
+    if stream is None:
+        handle = torch.cuda.current_stream(dev).cuda_stream or None
+    else:
+        handle = _stream_handle(stream)
+        s = torch.cuda.ExternalStream(handle or 0, device=dev) if isinstance(stream, int) else stream
+        if s != torch.cuda.current_stream(dev):
+            for t in fresh:
+                if t is not None:
+                    t.record_stream(s)
+    if torch.cuda.current_device() == dev.index:
+        status = fn(*args, handle)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, handle)
+    if status != OK:
+        _check(status, what)
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _gate_form(what, gate, T, d, dtype):
+    if gate is None:
+        return GATE_NONE
+    if gate.dtype != dtype or not gate.is_contiguous():
+        _refuse(what, f"gate must be contiguous {dtype}")
+    shape = tuple(gate.shape)
+    if shape == (T, d):
+        return GATE_FULL
+    if shape == (T, 1):
+        return GATE_TOKEN
+    if shape in ((1, d), (d,)):
+        return GATE_CHANNEL
+    _refuse(what, f"gate must be ({T}, 1), (1, {d}), ({d},) or ({T}, {d}), got {shape}")
+
+
+class BlockNormResult(NamedTuple):
+    residual_out: object
+    normed: object
+
+
+class BlockNormGrads(NamedTuple):
+    d_residual: object
+    d_y: object
+    d_w_post: object
+    d_w_pre: object
+    d_gate: object
+
+
+def _check_block_norm(what, residual, y, w_post, w_pre, gate, dtype):
+    import torch
+    T, d = residual.shape
+    dtype_code(dtype)
+    if residual.dtype not in (dtype, torch.float32):
+        _refuse(what, f"residual must be {dtype} or float32, got {residual.dtype}")
+    _rows(what, "residual", residual, (T, d), residual.dtype, strided=True)
+    if y is None and (w_post is not None or gate is not None):
+        _refuse(what, "w_post and gate need y")
+    if y is not None:
+        _rows(what, "y", y, (T, d), dtype, strided=True)
+    for name, w in (("w_post", w_post), ("w_pre", w_pre)):
+        if w is not None:
+            _rows(what, name, w, (d,), dtype)
+    return T, d
+
+
+def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, eps=1e-6, out=None, stream=None):
+    """Norms behind and before a block, fused with its gate and residual scale:
+      z = rms(y) * w_post (w_post None: y);  residual_out = residual + scale * gate * z
+      normed = rms(residual_out) * w_pre (w_pre None: None)
+    residual [T, d] 16-bit or float32, y [T, d] 16-bit (None: residual_out is
+    the residual), gate [T, 1], [1, d] / [d] or [T, d].  residual and y may be
+    row-strided.  out: a BlockNormResult of contiguous tensors to write."""
+    import torch
+    if residual.dim() != 2:
+        _refuse("block_norm", "residual must be [T, d]")
+    some = y if y is not None else w_pre
+    if some is None:
+        _refuse("block_norm", "nothing to do without y and w_pre")
+    dtype = some.dtype
+    T, d = _check_block_norm("block_norm", residual, y, w_post, w_pre, gate, dtype)
+    form = _gate_form("block_norm", gate, T, d, dtype)
+    dev = _same_device("block_norm", residual, y, w_post, w_pre, gate)
+    fresh = ()
+    if out is None:
+        fresh = out = BlockNormResult(
+            residual_out=torch.empty((T, d), dtype=residual.dtype, device=dev) if y is not None else None,
+            normed=torch.empty((T, d), dtype=dtype, device=dev) if w_pre is not None else None)
+    else:
+        if (out.residual_out is None) != (y is None) or (out.normed is None) != (w_pre is None):
+            _refuse("block_norm", "out needs residual_out with y and normed with w_pre, and neither without")
+        _same_device("block_norm", residual, *out)
+        if y is not None:
+            _rows("block_norm", "out.residual_out", out.residual_out, (T, d), residual.dtype)
+        if w_pre is not None:
+            _rows("block_norm", "out.normed", out.normed, (T, d), dtype)
+    if T == 0:
+        return out if y is not None else BlockNormResult(residual, out.normed)
+    _enqueue("block_norm", lib().moe_b200_block_norm, dev, stream, fresh,
+             _ptr(y), _row_stride(y) if y is not None else 0, _ptr(residual), _row_stride(residual),
+             int(residual.dtype == torch.float32), _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d,
+             dtype_code(dtype), _ptr(out.residual_out), _ptr(out.normed))
+    return out if y is not None else BlockNormResult(residual, out.normed)
+
+
+def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=None, w_pre=None, gate=None, scale=1.0,
+                        eps=1e-6, stream=None):
+    """Gradients of block_norm from those of its results (d_residual_out None:
+    zero; d_normed None without w_pre) and its stored residual_out.  Returns
+    BlockNormGrads: d_residual in the residual's type, d_y 16-bit, d_w_post and
+    d_w_pre float32 [d], d_gate float32 [T, 1] or the gate's [1, d] / [d], or
+    16-bit [T, d]."""
+    import torch
+    what = "block_norm_backward"
+    if residual_out.dim() != 2:
+        _refuse(what, "residual_out must be [T, d]")
+    some = y if y is not None else w_pre
+    if some is None:
+        _refuse(what, "nothing to do without y and w_pre")
+    dtype = some.dtype
+    T, d = _check_block_norm(what, residual_out, y, w_post, w_pre, gate, dtype)
+    form = _gate_form(what, gate, T, d, dtype)
+    if (d_normed is None) != (w_pre is None):
+        _refuse(what, "d_normed and w_pre go together")
+    if d_residual_out is None and w_pre is None:
+        _refuse(what, "no gradient given")
+    if d_residual_out is not None:
+        _rows(what, "d_residual_out", d_residual_out, (T, d), residual_out.dtype)
+    if d_normed is not None:
+        _rows(what, "d_normed", d_normed, (T, d), dtype)
+    dev = _same_device(what, residual_out, d_residual_out, d_normed, y, w_post, w_pre, gate)
+    res32 = int(residual_out.dtype == torch.float32)
+    nbytes = int(lib().moe_b200_block_norm_backward_workspace_bytes(T, d, res32))
+
+    def empty(shape, dt):
+        return torch.empty(shape, dtype=dt, device=dev)
+
+    got = BlockNormGrads(
+        d_residual=empty((T, d), residual_out.dtype),
+        d_y=empty((T, d), dtype) if y is not None else None,
+        d_w_post=empty((d,), torch.float32) if w_post is not None else None,
+        d_w_pre=empty((d,), torch.float32) if w_pre is not None else None,
+        d_gate=empty(gate.shape, dtype if form == GATE_FULL else torch.float32) if gate is not None else None)
+    if T == 0:  # sums over no token
+        with torch.cuda.stream(stream if not isinstance(stream, int) else torch.cuda.ExternalStream(stream, device=dev)):
+            for t in got[2:]:
+                if t is not None:
+                    t.zero_()
+        return got
+    ws = empty((max(nbytes, 256),), torch.uint8)
+    _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream, (*got, ws),
+             _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), _row_stride(residual_out), res32, _ptr(y),
+             _row_stride(y) if y is not None else 0, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d,
+             dtype_code(dtype), _ptr(got.d_residual), _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre),
+             _ptr(got.d_gate), _ptr(ws), ws.numel())
+    return got
+
+
+def _grouped_mm(what, fn, rows_in, seg_start, w, seg_expert, out, stream, forward):
+    import torch
+    if rows_in.dim() != 2 or w.dim() != 3 or seg_start.dim() != 1 or seg_start.numel() < 2:
+        _refuse(what, "rows must be 2-D, w [E, N, K] and seg_start [nseg + 1]")
+    E, N, K = w.shape
+    rows = rows_in.shape[0]
+    width_in, width_out = (K, N) if forward else (N, K)
+    nseg = seg_start.numel() - 1
+    dtype = rows_in.dtype
+    code = dtype_code(dtype)
+    _rows(what, "rows", rows_in, (rows, width_in), dtype)
+    _rows(what, "w", w, (E, N, K), dtype)
+    _rows(what, "seg_start", seg_start, (nseg + 1,), torch.int32)
+    if seg_expert is not None:
+        _rows(what, "seg_expert", seg_expert, (nseg,), torch.int32)
+    elif nseg > E:
+        _refuse(what, f"{nseg} segments for {E} experts need seg_expert")
+    dev = _same_device(what, rows_in, seg_start, w, seg_expert, out)
+    fresh = ()
+    if out is None:
+        out = torch.empty((rows, width_out), dtype=dtype, device=dev)
+        fresh = (out,)
+    else:
+        _rows(what, "out", out, (rows, width_out), dtype)
+    _enqueue(what, fn, dev, stream, fresh, _ptr(rows_in), _ptr(seg_start), _ptr(seg_expert), nseg, rows, N, K, E,
+             _ptr(w), code, _ptr(out))
+    return out
+
+
+def grouped_mm(x, seg_start, w, seg_expert=None, out=None, stream=None):
+    """One product per expert: y[r] = w[e] . x[r] for the rows r of segment s
+    (rows seg_start[s] .. seg_start[s+1] - 1, e = seg_expert[s] or s).
+    x [rows, K], w [E, N, K] -> [rows, N]; rows outside every segment are not
+    written."""
+    return _grouped_mm("grouped_mm", lib().moe_b200_grouped_mm, x, seg_start, w, seg_expert, out, stream, True)
+
+
+def grouped_mm_dgrad(dy, seg_start, w, seg_expert=None, out=None, stream=None):
+    """Gradient of grouped_mm for its rows: dx[r] = w[e]^T . dy[r];
+    dy [rows, N], w [E, N, K] -> [rows, K]."""
+    return _grouped_mm("grouped_mm_dgrad", lib().moe_b200_grouped_mm_dgrad, dy, seg_start, w, seg_expert, out, stream,
+                       False)
+
+
+def grouped_mm_wgrad(dy, x, seg_start, out=None, stream=None):
+    """Gradient of grouped_mm for its weights: dw[s] = sum over the segment's
+    rows of dy[r] x[r]^T; dy [rows, N], x [rows, K] -> [nseg, N, K], zeros for
+    empty segments (segments that share an expert are to be added up by the
+    caller)."""
+    import torch
+    what = "grouped_mm_wgrad"
+    if dy.dim() != 2 or x.dim() != 2 or seg_start.dim() != 1 or seg_start.numel() < 2:
+        _refuse(what, "dy and x must be 2-D and seg_start [nseg + 1]")
+    rows, N = dy.shape
+    K = x.shape[1]
+    nseg = seg_start.numel() - 1
+    dtype = x.dtype
+    code = dtype_code(dtype)
+    _rows(what, "dy", dy, (rows, N), dtype)
+    _rows(what, "x", x, (rows, K), dtype)
+    _rows(what, "seg_start", seg_start, (nseg + 1,), torch.int32)
+    dev = _same_device(what, x, dy, seg_start, out)
+    fresh = ()
+    if out is None:
+        out = torch.empty((nseg, N, K), dtype=dtype, device=dev)
+        fresh = (out,)
+    else:
+        _rows(what, "out", out, (nseg, N, K), dtype)
+    _enqueue(what, lib().moe_b200_grouped_mm_wgrad, dev, stream, fresh, _ptr(dy), _ptr(x), _ptr(seg_start), nseg, rows,
+             N, K, code, _ptr(out))
+    return out
+
+
+def expert_linear_w4(x, asgn, w_q, w_scale, w_zero=None, act=None, out=None, stream=None):
+    """Products of few tokens with 4-bit expert weights, slot (t, k) with
+    expert asgn[t, k] (int32; -1: no expert, a row of zeros).
+      x       [T, d], or [T, K, d] with a row of its own for each slot
+      w_q     uint8 [E, N, d/2] (even column in the low half of a byte)
+      w_scale [E, N, d/group] of x's type, group 32, 64 or 128
+      w_zero  uint8 [E, N, d/group], None: 8
+      act     None, or "swiglu": silu(y[:, :N/2]) * y[:, N/2:]
+    Returns [T*K, N] (swiglu [T*K, N/2]); combine a down product's rows with
+    unpermute and slot_pos = arange(T*K)."""
+    import torch
+    what = "expert_linear_w4"
+    if act not in (None, "swiglu"):
+        _refuse(what, f"act must be None or 'swiglu', got {act!r}")
+    if asgn.dim() != 2 or w_q.dim() != 3 or w_scale.dim() != 3 or x.dim() not in (2, 3):
+        _refuse(what, "x must be [T, d] or [T, K, d], asgn [T, K], w_q and w_scale 3-D")
+    T, K = asgn.shape
+    E, N, half = w_q.shape
+    d = 2 * half
+    dtype = x.dtype
+    code = dtype_code(dtype)
+    _rows(what, "x", x, (T, d) if x.dim() == 2 else (T, K, d), dtype)
+    _rows(what, "asgn", asgn, (T, K), torch.int32)
+    _rows(what, "w_q", w_q, (E, N, half), torch.uint8)
+    groups = w_scale.shape[2]
+    if groups < 1 or d % groups != 0:
+        _refuse(what, f"w_scale has {groups} groups for d={d}")
+    _rows(what, "w_scale", w_scale, (E, N, groups), dtype)
+    if w_zero is not None:
+        _rows(what, "w_zero", w_zero, (E, N, groups), torch.uint8)
+    n_out = N // 2 if act else N
+    dev = _same_device(what, x, asgn, w_q, w_scale, w_zero, out)
+    fresh = ()
+    if out is None:
+        out = torch.empty((T * K, n_out), dtype=dtype, device=dev)
+        fresh = (out,)
+    else:
+        _rows(what, "out", out, (T * K, n_out), dtype)
+    _enqueue(what, lib().moe_b200_expert_linear_w4, dev, stream, fresh,
+             _ptr(x), int(x.dim() == 3), _ptr(asgn), T, K, E, d, N, _ptr(w_q), _ptr(w_scale), _ptr(w_zero), d // groups,
+             ACT_SWIGLU if act else ACT_NONE, code, _ptr(out))
     return out

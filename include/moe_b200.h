@@ -229,6 +229,33 @@ int moe_b200_grouped_ffn(const void* x, const int32_t* seg_start, const int32_t*
 int moe_b200_ffn_weights_from_reference(const void* w1, const void* w2, int E, int d, int F,
                                         void* w_up, void* w_down, void* stream);
 
+/* ------------------------------------------- expert products, gradients ---- */
+
+/* ONE product per expert over ragged row segments, and its two gradients, on
+ * the tcgen05 tensor cores; w [E, N, K], rows [seg_start[s], seg_start[s+1])
+ * of segment s belong to expert e = seg_expert[s] (NULL: e = s):
+ *   moe_b200_grouped_mm        y[r]  = w[e] . x[r]          x [rows, K] -> y [rows, N]
+ *   moe_b200_grouped_mm_dgrad  dx[r] = w[e]^T . dy[r]       dy [rows, N] -> dx [rows, K]
+ *   moe_b200_grouped_mm_wgrad  dw[s] = sum dy[r] x[r]^T over the segment's rows,
+ *                              [nseg, N, K]; zeros for an empty segment
+ * fp32 accumulation, each result rounded once to dtype.  With them the
+ * layer's products (moe_b200_grouped_ffn's up and down products are two of
+ * them) can be trained; the gradient of a packed row's token is
+ * moe_b200_unpermute with weights of 1.
+ * seg_start [nseg + 1] ascending within [0, rows] (held inside it otherwise);
+ * rows outside every segment are left as they were, and a segment whose
+ * expert is outside [0, E) gives zeros.  N and K multiples of 8; nseg <= 1024;
+ * pointers 16-byte aligned; no workspace.  Replaces the per-expert
+ * cublasHgemm calls of apps/bench_e2e.cu:274-301 as single products; the
+ * reference has no gradients.  Device-side conditions:
+ * moe_b200_device_status().                                                 */
+int moe_b200_grouped_mm(const void* x, const int32_t* seg_start, const int32_t* seg_expert, int nseg, int rows, int N,
+                        int K, int E, const void* w, int dtype, void* y, void* stream);
+int moe_b200_grouped_mm_dgrad(const void* dy, const int32_t* seg_start, const int32_t* seg_expert, int nseg, int rows,
+                              int N, int K, int E, const void* w, int dtype, void* dx, void* stream);
+int moe_b200_grouped_mm_wgrad(const void* dy, const void* x, const int32_t* seg_start, int nseg, int rows, int N,
+                              int K, int dtype, void* dw, void* stream);
+
 /* ----------------------------------------------------- expert parallel ---- */
 
 /* Exchange layout of rank `rank` among `nranks` expert-parallel ranks, on the
@@ -338,6 +365,85 @@ int moe_b200_ep_step(void* ctx, const void* emb, const int32_t* asgn, const floa
                      size_t workspace_bytes, void* out, void* stream);
 /* Largest epoch enqueued on this context so far (0 before the first step). */
 uint64_t moe_b200_ep_epoch(void* ctx);
+
+/* --------------------------------------------- norms around the block ---- */
+
+/* RMS norms behind and before a block of a residual network (the MoE layer is
+ * such a block), fused with the block's gate and residual scale, one pass:
+ *   rms(v) = v * rsqrt(mean(v^2) + eps)  per row of d columns
+ *   z            = rms(y) * w_post              (w_post NULL: z = y)
+ *   residual_out = residual + scale * gate * z  (y NULL: no block, residual_out unused)
+ *   normed       = rms(residual_out) * w_pre    (w_pre NULL: none)
+ *   y            [T, d]  block output, 16-bit (dtype), rows y_stride elements apart
+ *   residual     [T, d]  16-bit (dtype) or fp32 (residual_f32), rows
+ *                        residual_stride elements apart
+ *   w_post, w_pre [d]    16-bit (dtype)
+ *   gate                 16-bit (dtype): one value per token [T], per channel
+ *                        [d] or per element [T, d] (MOE_B200_GATE_*)
+ *   residual_out [T, d]  out, contiguous, the residual's type; may be the
+ *                        residual itself where that is contiguous
+ *   normed       [T, d]  out, contiguous, 16-bit; taken from the unrounded
+ *                        residual_out; may be y itself where that is contiguous
+ * Sums in fp32; d <= 16384, any alignment (rows whose d, strides and pointers
+ * are in 16-byte steps are read in 16-byte pieces).  No counterpart in the
+ * reference, whose layer has no norms.                                      */
+enum moe_b200_gate_form {
+    MOE_B200_GATE_NONE = 0,
+    MOE_B200_GATE_TOKEN = 1,
+    MOE_B200_GATE_CHANNEL = 2,
+    MOE_B200_GATE_FULL = 3
+};
+int moe_b200_block_norm(const void* y, int64_t y_stride, const void* residual, int64_t residual_stride,
+                        int residual_f32, const void* w_post, const void* w_pre, const void* gate, int gate_form,
+                        float scale, float eps, int T, int d, int dtype, void* residual_out, void* normed,
+                        void* stream);
+
+/* Gradients of moe_b200_block_norm, given those of its two results:
+ *   d_residual_out [T, d] contiguous, the residual's type (NULL: zero; needs w_pre)
+ *   d_normed       [T, d] contiguous, 16-bit (unused without w_pre)
+ *   residual_out   the forward's result (unused without w_pre); y, w_post,
+ *                  w_pre, gate, scale, eps as in the forward
+ * Results:
+ *   d_residual [T, d] the residual's type    d_y [T, d] 16-bit (with y)
+ *   d_w_post, d_w_pre [d] fp32               (with w_post / w_pre)
+ *   d_gate  fp32 [T] / fp32 [d] / 16-bit [T, d] by gate_form
+ * Sums over tokens are taken in a fixed order.  workspace:
+ * moe_b200_block_norm_backward_workspace_bytes(T, d, residual_f32) bytes,
+ * 256-byte aligned, needs no initial value; concurrent calls use distinct
+ * ones.                                                                     */
+size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d, int residual_f32);
+int moe_b200_block_norm_backward(const void* d_residual_out, const void* d_normed, const void* residual_out,
+                                 int64_t residual_stride, int residual_f32, const void* y, int64_t y_stride,
+                                 const void* w_post, const void* w_pre, const void* gate, int gate_form, float scale,
+                                 float eps, int T, int d, int dtype, void* d_residual, void* d_y, float* d_w_post,
+                                 float* d_w_pre, void* d_gate, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* ------------------------------------------------ 4-bit expert products ---- */
+
+/* Products with 4-bit expert weights for few tokens (decode batches), each
+ * slot (t, k) with its own expert and without a packing pass:
+ *   y[s, n] = sum_i x[row(s), i] * (q[e, n, i] - z[e, n, i / group]) * w_scale[e, n, i / group]
+ *   s = t*K + k, e = asgn[s], row(s) = t, or s when x_per_slot
+ *   x       [T, d] or [T*K, d]  16-bit (dtype)
+ *   asgn    [T, K]              expert of each slot; -1: no expert, the slot's
+ *                               output row is zeros (padded batches)
+ *   w_q     [E, N, d/2]         two weights a byte, even column in the low half
+ *   w_scale [E, N, d/group]     16-bit (dtype)
+ *   w_zero  [E, N, d/group]     bytes 0..15; NULL: 8 everywhere
+ *   out     [T*K, n_out]        16-bit; MOE_B200_ACT_NONE: n_out = N;
+ *                               MOE_B200_ACT_SWIGLU: n_out = N/2,
+ *                               silu(y[:, :N/2]) * y[:, N/2:]
+ * fp32 accumulation, out rounded once.  The outputs of a down product are
+ * combined by moe_b200_unpermute with slot_pos[s] = s.  group 32, 64 or 128
+ * and a divisor of d; N a multiple of 8 (SwiGLU: 16); T*K <= 4096; pointers
+ * 16-byte aligned.  An expert outside [0, E) other than -1 gives zeros too
+ * and MOE_B200_DEV_BAD_ASSIGNMENT in moe_b200_device_status().  No
+ * counterpart in the reference, whose expert weights are 16-bit.            */
+enum moe_b200_act { MOE_B200_ACT_NONE = 0, MOE_B200_ACT_SWIGLU = 1 };
+int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const int32_t* asgn, int T, int K, int E, int d, int N,
+                              const void* w_q, const void* w_scale, const void* w_zero, int group, int act, int dtype,
+                              void* out, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
