@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -30,7 +31,6 @@ int fail(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t err, const char* where);
 
 constexpr int kNormMaxD = 16384;
-constexpr int kNormMaxThreads = 1024;
 
 enum { kGateNone = MOE_B200_GATE_NONE, kGateToken = MOE_B200_GATE_TOKEN, kGateChannel = MOE_B200_GATE_CHANNEL,
        kGateFull = MOE_B200_GATE_FULL };
@@ -128,26 +128,26 @@ __device__ __forceinline__ void store8(void* row, const float (&x)[8], int chunk
     }
 }
 
-// Sums of N values over the `nt` threads of a row group (nt a multiple of 32),
-// the same bits in every thread.  `red` holds two buffers of N floats a warp;
+// Sums of N values over a row's threads: a warp (WARP) or the whole CTA, the
+// same bits in every thread.  `red` holds two buffers of 4 floats a warp;
 // `phase` alternates them, so one barrier a reduction is enough: a buffer is
 // written again only after the next reduction's barrier, which no thread
 // passes before it has read this one.
-template <int N>
-__device__ __forceinline__ void group_sum(float (&v)[N], float* red, int nt, int group, int warp_in_group, int& phase) {
+template <bool WARP, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if (nt == 32) return;
-    const int nw = nt >> 5;
+    if (WARP) return;
+    const int nw = blockDim.x >> 5;
     float* b = red + (phase & 1) * (nw * 4);
     ++phase;
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) b[warp_in_group * 4 + i] = v[i];
+        for (int i = 0; i < N; ++i) b[(threadIdx.x >> 5) * 4 + i] = v[i];
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(nt) : "memory");
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.f;
     for (int w = 0; w < nw; ++w) {
@@ -161,85 +161,96 @@ struct NormArgs {
     int64_t y_stride, res_stride;  // elements
     int gate_form;
     float scale, eps;
-    int T, d, row_threads;
+    int T, d;
     void *residual_out, *normed;
 };
 
-// A group of `row_threads` threads per row, V chunks of 8 columns a thread, a
-// CTA of at least 128 threads.  No loop over rows: the grid's many small CTAs
-// keep enough loads in flight.
-template <int DT, bool RES32, bool ALIGNED, int V>
-__global__ void __launch_bounds__(kNormMaxThreads)
+// A row belongs to one warp (WARP: CTAs of 4 rows) or to a CTA; each thread
+// holds V chunks of 8 columns.  The grid fits the card and walks the rows; the
+// weights stay packed in registers and the next row's loads are in flight
+// while a row is reduced and written.
+template <int DT, bool RES32, bool ALIGNED, bool WARP, int V, int MAXT>
+__global__ void __launch_bounds__(MAXT)
 block_norm_kernel(const NormArgs a) {
     __shared__ float s_red[2 * 4 * 32];
-    const int nt = a.row_threads, group = threadIdx.x / nt, t = threadIdx.x - group * nt, wig = t >> 5;
-    const int64_t row = int64_t(blockIdx.x) * (blockDim.x / nt) + group;
-    if (row >= a.T) return;  // whole groups leave together; barriers are per group
-    float* red = s_red + group * (nt >> 5) * 8;
+    const int nt = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
+    const int rows_per_cta = WARP ? blockDim.x >> 5 : 1;
+    const int64_t step = int64_t(gridDim.x) * rows_per_cta;
+    int64_t row = int64_t(blockIdx.x) * rows_per_cta + (WARP ? threadIdx.x >> 5 : 0);
+    if (row >= a.T) return;
     int phase = 0;
     const int d = a.d;
     const float inv_d = 1.0f / float(d);
-    const char* res_row = static_cast<const char*>(a.residual) + row * a.res_stride * (RES32 ? 4 : 2);
-    const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + row * a.y_stride;
+    Raw<false> wp[V], gc[V], wn[V], yr[V], gr[V];
     Raw<RES32> res[V];
-    Raw<false> yr[V], wp[V], gr[V], wn[V];
+    auto fetch = [&](int64_t r) {
+        const char* res_row = static_cast<const char*>(a.residual) + r * a.res_stride * (RES32 ? 4 : 2);
+        const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + r * a.y_stride;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            res[i] = load_raw<ALIGNED, RES32>(res_row, i, t, nt, d);
+            if (a.y) yr[i] = load_raw<ALIGNED, false>(y_row, i, t, nt, d);
+            if (a.gate_form == kGateFull)
+                gr[i] = load_raw<ALIGNED, false>(static_cast<const uint16_t*>(a.gate) + r * d, i, t, nt, d);
+        }
+    };
+    fetch(row);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        res[i] = load_raw<ALIGNED, RES32>(res_row, i, t, nt, d);
-        if (a.y) yr[i] = load_raw<ALIGNED, false>(y_row, i, t, nt, d);
-        if (a.gate_form == kGateFull)
-            gr[i] = load_raw<ALIGNED, false>(static_cast<const uint16_t*>(a.gate) + row * d, i, t, nt, d);
-        if (a.gate_form == kGateChannel) gr[i] = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
+        if (a.gate_form == kGateChannel) gc[i] = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
         if (a.w_post) wp[i] = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
         if (a.w_pre) wn[i] = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
     }
-    float r[V][8];
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[i][j] = raw_get<DT, RES32>(res[i], j);
-    if (a.y) {
-        float f = a.scale;
-        if (a.gate_form == kGateToken) f *= from16<DT>(static_cast<const uint16_t*>(a.gate)[row]);
-        if (a.w_post) {
-            float s[1] = {0.f};
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = raw_get<DT, false>(yr[i], j);
-                    s[0] += y * y;
-                }
-            group_sum(s, red, nt, group, wig, phase);
-            f *= rsqrtf(s[0] * inv_d + a.eps);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float z = raw_get<DT, false>(yr[i], j) * f;
-                if (a.w_post) z *= raw_get<DT, false>(wp[i], j);
-                if (a.gate_form >= kGateChannel) z *= raw_get<DT, false>(gr[i], j);
-                r[i][j] += z;
-            }
-        char* out = static_cast<char*>(a.residual_out) + row * d * (RES32 ? 4 : 2);
-#pragma unroll
-        for (int i = 0; i < V; ++i) store8<DT, ALIGNED, RES32>(out, r[i], i, t, nt, d);
-    }
-    if (a.w_pre) {
+    for (; row < a.T; row += step) {
+        float r[V][8], y[V][8];
         float s[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[0] += r[i][j] * r[i][j];
-        group_sum(s, red, nt, group, wig, phase);
-        const float c = rsqrtf(s[0] * inv_d + a.eps);
-        uint16_t* out = static_cast<uint16_t*>(a.normed) + row * d;
+            for (int j = 0; j < 8; ++j) {
+                r[i][j] = raw_get<DT, RES32>(res[i], j);
+                if (a.y) {
+                    y[i][j] = raw_get<DT, false>(yr[i], j);
+                    s[0] += y[i][j] * y[i][j];
+                    if (a.gate_form == kGateChannel) y[i][j] *= raw_get<DT, false>(gc[i], j);
+                    if (a.gate_form == kGateFull) y[i][j] *= raw_get<DT, false>(gr[i], j);
+                }
+            }
+        float f = a.scale;
+        if (a.gate_form == kGateToken) f *= from16<DT>(static_cast<const uint16_t*>(a.gate)[row]);
+        if (row + step < a.T) fetch(row + step);
+        if (a.y) {
+            if (a.w_post) {
+                row_sum<WARP>(s, s_red, phase);
+                f *= rsqrtf(s[0] * inv_d + a.eps);
+            }
+            char* out = static_cast<char*>(a.residual_out) + row * d * (RES32 ? 4 : 2);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < V; ++i) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[i][j] *= c * raw_get<DT, false>(wn[i], j);
-            store8<DT, ALIGNED, false>(out, r[i], i, t, nt, d);
+                for (int j = 0; j < 8; ++j) {
+                    float z = y[i][j] * f;
+                    if (a.w_post) z *= raw_get<DT, false>(wp[i], j);
+                    r[i][j] += z;
+                }
+                store8<DT, ALIGNED, RES32>(out, r[i], i, t, nt, d);
+            }
+        }
+        if (a.w_pre) {
+            s[0] = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[0] += r[i][j] * r[i][j];
+            row_sum<WARP>(s, s_red, phase);
+            const float c = rsqrtf(s[0] * inv_d + a.eps);
+            uint16_t* out = static_cast<uint16_t*>(a.normed) + row * d;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[i][j] *= c * raw_get<DT, false>(wn[i], j);
+                store8<DT, ALIGNED, false>(out, r[i], i, t, nt, d);
+            }
         }
     }
 }
@@ -249,112 +260,167 @@ struct NormGradArgs {
     int64_t y_stride, res_stride;
     int gate_form;
     float scale, eps;
-    int T, d, row_threads;
+    int T, d;
     void *d_res, *d_y, *d_gate;
     // Column sums of each CTA: up to three vectors of d floats, [vector][CTA][d].
     float* part;
     int sum_pre, sum_post, sum_gate;  // index of the vector, or -1
+    // Ring of rows in shared memory (RING): bytes of a staged row and where its
+    // parts lie in it (-1: absent).
+    int row_bytes, off_ds, off_rr, off_dn, off_y, off_gate;
+    uint32_t* status;
 };
 
-// Rows are dealt to the groups of a grid that fits the card, so that each
-// thread keeps its columns' sums over its rows in registers and the column
-// gradients cost one row of partial sums a CTA.  Row data stays packed as
-// loaded until it is used.
-template <int DT, bool RES32, bool ALIGNED, int V, int MAXT>
+constexpr int kNormStages = 3;
+
+// Rows are dealt to a grid that fits the card, so that each thread keeps its
+// columns' sums over its rows in registers and the column gradients cost one
+// row of partial sums a CTA.  RING: the rows come through a ring of shared-
+// memory stages filled by bulk copies kNormStages rows ahead, which costs no
+// registers; otherwise (rows not in 16-byte steps, or too wide for the ring)
+// they are read from global memory at each of the two uses.
+template <int DT, bool RES32, bool ALIGNED, bool RING, bool WARP, int V, int MAXT>
 __global__ void __launch_bounds__(MAXT)
 block_norm_backward_kernel(const NormGradArgs a) {
-    extern __shared__ float s_dyn[];  // [2 * 4 * 32] reduction words, then (several groups) [d] column sums
-    const int nt = a.row_threads, group = threadIdx.x / nt, t = threadIdx.x - group * nt, wig = t >> 5;
-    const int groups = blockDim.x / nt;
-    float* red = s_dyn + group * (nt >> 5) * 8;
+    extern __shared__ __align__(128) unsigned char s_dyn[];
+    __shared__ float s_red[2 * 4 * 32];
+    __shared__ uint64_t s_full[4 * kNormStages], s_empty[4 * kNormStages];
+    const int nt = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
+    const int groups = WARP ? blockDim.x >> 5 : 1, group = WARP ? threadIdx.x >> 5 : 0;
+    const int64_t step = int64_t(gridDim.x) * groups;
+    const int64_t row0 = int64_t(blockIdx.x) * groups + group;
     int phase = 0;
     const int d = a.d;
     const float inv_d = 1.0f / float(d);
+    constexpr int kRes = RES32 ? 4 : 2;
+    uint64_t *full = s_full + group * kNormStages, *empty = s_empty + group * kNormStages;
+    unsigned char* ring = s_dyn + size_t(group) * kNormStages * a.row_bytes;
+
+    auto ds_row = [&](int64_t r) { return static_cast<const char*>(a.d_res_out) + r * d * kRes; };
+    auto rr_row = [&](int64_t r) { return static_cast<const char*>(a.res_out) + r * a.res_stride * kRes; };
+    auto dn_row = [&](int64_t r) { return static_cast<const char*>(a.d_normed) + r * d * 2; };
+    auto y_row = [&](int64_t r) { return static_cast<const char*>(a.y) + r * a.y_stride * 2; };
+    auto g_row = [&](int64_t r) { return static_cast<const char*>(a.gate) + r * d * 2; };
+    auto fill = [&](int64_t r, int s) {  // one thread
+        unsigned char* p = ring + size_t(s) * a.row_bytes;
+        mbar_arrive_expect_tx(full + s, a.row_bytes);
+        if (a.off_ds >= 0) bulk_g2s(p + a.off_ds, ds_row(r), d * kRes, full + s);
+        if (a.off_rr >= 0) bulk_g2s(p + a.off_rr, rr_row(r), d * kRes, full + s);
+        if (a.off_dn >= 0) bulk_g2s(p + a.off_dn, dn_row(r), d * 2, full + s);
+        if (a.off_y >= 0) bulk_g2s(p + a.off_y, y_row(r), d * 2, full + s);
+        if (a.off_gate >= 0) bulk_g2s(p + a.off_gate, g_row(r), d * 2, full + s);
+    };
+    if (RING) {
+        if (t == 0) {
+            for (int s = 0; s < kNormStages; ++s) {
+                mbar_init(full + s, 1);
+                mbar_init(empty + s, nt >> 5);
+            }
+            mbar_fence_init();
+        }
+        __syncthreads();
+        if (t == 0)
+            for (int s = 0; s < kNormStages; ++s)
+                if (row0 + s * step < a.T) fill(row0 + s * step, s);
+    }
+
     float s_pre[V][8], s_post[V][8], s_gate[V][8];
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) s_pre[i][j] = s_post[i][j] = s_gate[i][j] = 0.f;
 
-    for (int64_t row = int64_t(blockIdx.x) * groups + group; row < a.T; row += int64_t(gridDim.x) * groups) {
-        Raw<RES32> ds[V], rr[V];
-        Raw<false> dn[V], yr[V], gr[V];
-        const char* ds_row = static_cast<const char*>(a.d_res_out) + row * d * (RES32 ? 4 : 2);
-        const char* rr_row = static_cast<const char*>(a.res_out) + row * a.res_stride * (RES32 ? 4 : 2);
-        const uint16_t* dn_row = static_cast<const uint16_t*>(a.d_normed) + row * d;
-        const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + row * a.y_stride;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (a.w_pre) {
-                rr[i] = load_raw<ALIGNED, RES32>(rr_row, i, t, nt, d);
-                dn[i] = load_raw<ALIGNED, false>(dn_row, i, t, nt, d);
+    uint32_t n = 0;
+    for (int64_t row = row0; row < a.T; row += step, ++n) {
+        const int st = int(n % kNormStages);
+        const unsigned char* p = ring + size_t(st) * a.row_bytes;
+        if (RING) {
+            // Refill the stage of the row before, once all its warps are through with it.
+            const int64_t ahead = row + (kNormStages - 1) * step;
+            if (t == 0 && n > 0 && ahead < a.T) {
+                const int prev = int((n - 1) % kNormStages);
+                if (!mbar_wait(empty + prev, ((n - 1) / kNormStages) & 1u)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
+                fill(ahead, prev);
             }
-            if (a.y) yr[i] = load_raw<ALIGNED, false>(y_row, i, t, nt, d);
-            if (a.d_res_out) ds[i] = load_raw<ALIGNED, RES32>(ds_row, i, t, nt, d);
-            if (a.gate_form == kGateFull)
-                gr[i] = load_raw<ALIGNED, false>(static_cast<const uint16_t*>(a.gate) + row * d, i, t, nt, d);
-            if (a.gate_form == kGateChannel) gr[i] = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
+            if (!mbar_wait(full + st, (n / kNormStages) & 1u)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
         }
+        auto get16 = [&](int off, const char* g, int i) {
+            return RING ? load_raw<ALIGNED, false>(p + off, i, t, nt, d) : load_raw<ALIGNED, false>(g, i, t, nt, d);
+        };
+        auto getres = [&](int off, const char* g, int i) {
+            return RING ? load_raw<ALIGNED, RES32>(p + off, i, t, nt, d) : load_raw<ALIGNED, RES32>(g, i, t, nt, d);
+        };
         float sums[3] = {0.f, 0.f, 0.f};  // sum r'^2, sum u r', sum y^2
-        float q[V][8];
         if (a.w_pre) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const Raw<false> wn = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
+                const Raw<false> dn = get16(a.off_dn, dn_row(row), i);
+                const Raw<RES32> rr = getres(a.off_rr, rr_row(row), i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float r = raw_get<DT, RES32>(rr[i], j);
-                    q[i][j] = raw_get<DT, false>(dn[i], j) * raw_get<DT, false>(wn, j);
+                    const float r = raw_get<DT, RES32>(rr, j);
                     sums[0] += r * r;
-                    sums[1] += q[i][j] * r;
+                    sums[1] += raw_get<DT, false>(dn, j) * raw_get<DT, false>(wn, j) * r;
                 }
             }
         }
         if (a.w_post) {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
+            for (int i = 0; i < V; ++i) {
+                const Raw<false> yr = get16(a.off_y, y_row(row), i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float y = raw_get<DT, false>(yr[i], j);
+                    const float y = raw_get<DT, false>(yr, j);
                     sums[2] += y * y;
                 }
+            }
         }
-        if (a.w_pre || a.w_post) group_sum(sums, red, nt, group, wig, phase);
+        if (a.w_pre || a.w_post) row_sum<WARP>(sums, s_red, phase);
         const float c = rsqrtf(sums[0] * inv_d + a.eps);
         const float k = sums[1] * inv_d * c * c;
         const float post = a.w_post ? rsqrtf(sums[2] * inv_d + a.eps) : 1.0f;
-        char* dres_out = static_cast<char*>(a.d_res) + row * d * (RES32 ? 4 : 2);
+        char* dres_out = static_cast<char*>(a.d_res) + row * d * kRes;
         float f = a.scale;
         if (a.gate_form == kGateToken) f *= from16<DT>(static_cast<const uint16_t*>(a.gate)[row]);
         float sums2[2] = {0.f, 0.f};  // sum v yh, sum ds z (gate per token)
+        float q[V][8];
+        Raw<false> yr[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+            Raw<RES32> ds, rr;
+            Raw<false> wn, dn, wp, gr;
+            if (a.d_res_out) ds = getres(a.off_ds, ds_row(row), i);
+            if (a.w_pre) {
+                wn = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
+                dn = get16(a.off_dn, dn_row(row), i);
+                rr = getres(a.off_rr, rr_row(row), i);
+            }
+            if (a.y) yr[i] = get16(a.off_y, y_row(row), i);
+            if (a.w_post) wp = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
+            if (a.gate_form == kGateFull) gr = get16(a.off_gate, g_row(row), i);
+            if (a.gate_form == kGateChannel) gr = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float g = a.d_res_out ? raw_get<DT, RES32>(ds[i], j) : 0.f;
+                float g = a.d_res_out ? raw_get<DT, RES32>(ds, j) : 0.f;
                 if (a.w_pre) {
-                    const float r = raw_get<DT, RES32>(rr[i], j);
-                    g += c * (q[i][j] - r * k);
-                    s_pre[i][j] += raw_get<DT, false>(dn[i], j) * (r * c);
+                    const float r = raw_get<DT, RES32>(rr, j), dnj = raw_get<DT, false>(dn, j);
+                    g += c * (dnj * raw_get<DT, false>(wn, j) - r * k);
+                    s_pre[i][j] += dnj * (r * c);
                 }
                 q[i][j] = g;
             }
             store8<DT, ALIGNED, RES32>(dres_out, q[i], i, t, nt, d);
-        }
-        if (a.y) {
-            float dg[8];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                Raw<false> wp;
-                if (a.w_post) wp = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
+            if (a.y) {
+                float dg[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float yh = raw_get<DT, false>(yr[i], j) * post;
                     const float w = a.w_post ? raw_get<DT, false>(wp, j) : 1.0f;
                     const float g = q[i][j];
-                    if (a.gate_form != kGateNone) dg[j] = a.scale * g * (yh * w);
+                    dg[j] = a.scale * g * (yh * w);
                     float v = g * f;
-                    if (a.gate_form >= kGateChannel) v *= raw_get<DT, false>(gr[i], j);
+                    if (a.gate_form >= kGateChannel) v *= raw_get<DT, false>(gr, j);
                     if (a.w_post) {
                         s_post[i][j] += v * yh;
                         v *= w;
@@ -367,7 +433,13 @@ block_norm_backward_kernel(const NormGradArgs a) {
                 if (a.gate_form == kGateFull)
                     store8<DT, ALIGNED, false>(static_cast<uint16_t*>(a.d_gate) + row * d, dg, i, t, nt, d);
             }
-            if (a.w_post || a.gate_form == kGateToken) group_sum(sums2, red, nt, group, wig, phase);
+        }
+        if (RING) {  // the stage is read
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(empty + st);
+        }
+        if (a.y) {
+            if (a.w_post || a.gate_form == kGateToken) row_sum<WARP>(sums2, s_red, phase);
             if (a.gate_form == kGateToken && t == 0) static_cast<float*>(a.d_gate)[row] = sums2[1];
             const float m = sums2[0] * inv_d;
             uint16_t* dy_out = static_cast<uint16_t*>(a.d_y) + row * d;
@@ -382,9 +454,10 @@ block_norm_backward_kernel(const NormGradArgs a) {
         }
     }
 
-    // Column sums: the groups of the CTA add up through shared memory in group
-    // order, then the CTA writes its row of partial sums.
-    float* s_col = s_dyn + 2 * 4 * 32;
+    // Column sums: the CTA's rows side by side add up through shared memory in
+    // warp order, then the CTA writes its row of partial sums.
+    __syncthreads();  // the ring is free
+    float* s_col = reinterpret_cast<float*>(s_dyn);
 #pragma unroll
     for (int which = 0; which < 3; ++which) {
         const int vec = which == 0 ? a.sum_pre : which == 1 ? a.sum_post : a.sum_gate;
@@ -419,25 +492,27 @@ block_norm_backward_kernel(const NormGradArgs a) {
     pdl_launch_dependents();
 }
 
-// Adds the CTAs' partial rows: a warp per 32 columns of one vector, 8 warps
-// split the rows; each output is a fixed-order sum.
-__global__ void __launch_bounds__(256)
+// Adds the CTAs' partial rows: a CTA per 32 columns of one vector, its 32
+// warps split the rows; each output is a fixed-order sum.
+__global__ void __launch_bounds__(1024)
 block_norm_columns_kernel(const float* __restrict__ part, int nparts, int d, float* out0, float* out1, float* out2) {
-    __shared__ float s[8][33];
+    __shared__ float s[32][33];
     pdl_wait_primary();
     float* out = blockIdx.y == 0 ? out0 : blockIdx.y == 1 ? out1 : out2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
     const float* p = part + int64_t(blockIdx.y) * nparts * d;
     float v = 0.f;
-    if (col < d)
-        for (int i = warp; i < nparts; i += 8) v += p[int64_t(i) * d + col];
+    if (col < d) {
+#pragma unroll 4
+        for (int i = warp; i < nparts; i += 32) v += p[int64_t(i) * d + col];
+    }
     s[warp][lane] = v;
     __syncthreads();
-    if (warp == 0 && col < d) {
+    v = s[lane][warp];  // column `warp` of the 32, part `lane`
 #pragma unroll
-        for (int w = 1; w < 8; ++w) v += s[w][lane];
-        out[col] = v;
-    }
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int mine = blockIdx.x * 32 + warp;
+    if (lane == 0 && mine < d) out[mine] = v;
 }
 
 // ----------------------------------------------------------------- host ----
@@ -470,14 +545,13 @@ static int column_vectors(bool pre, bool post, int gate_form) {
 struct NormGradPlan {
     int v, row_threads, cta_threads, grid;
 };
-static NormGradPlan plan_norm_backward(int T, int d, bool res32) {
+static NormGradPlan plan_norm_backward(int T, int d) {
     NormGradPlan p{};
-    // Two chunks a thread and up to 512 threads: 48 sums and the packed row
-    // fit 128 registers; fp32 residuals (twice the words) take one chunk while
-    // 512 threads cover the row; the widest rows take four.
-    p.v = (res32 && d <= 4096) ? 1 : d <= 8192 ? 2 : 4;
+    // Two chunks a thread and up to 512 threads: 48 column sums and the row in
+    // flight fit 128 registers; the widest rows take four.
+    p.v = d <= 8192 ? 2 : 4;
     p.row_threads = row_threads_for(d, p.v);
-    p.cta_threads = p.row_threads < 128 ? 128 : p.row_threads;
+    p.cta_threads = p.row_threads == 32 ? 128 : p.row_threads;
     const int groups = p.cta_threads / p.row_threads;
     const int64_t need = (int64_t(T) + groups - 1) / groups;
     const int64_t fit = int64_t(sm_count_norm()) * (512 / p.cta_threads);
@@ -502,30 +576,75 @@ static int check_norm(const char* who, int T, int d, int dtype, int gate_form, c
     return MOE_B200_OK;
 }
 
-template <int DT, bool RES32, bool AL>
-static cudaError_t launch_norm(const NormArgs& a0, cudaStream_t s) {
-    NormArgs a = a0;
-    a.row_threads = row_threads_for(a.d, 2);
-    const int cta = a.row_threads < 128 ? 128 : a.row_threads;
-    const int groups = cta / a.row_threads;
-    const unsigned grid = unsigned((int64_t(a.T) + groups - 1) / groups);
-    block_norm_kernel<DT, RES32, AL, 2><<<grid, cta, 0, s>>>(a);
+template <int DT, bool RES32, bool AL, bool WARP, int MAXT>
+static cudaError_t launch_norm_as(const NormArgs& a, int cta, cudaStream_t s) {
+    auto kern = block_norm_kernel<DT, RES32, AL, WARP, 2, MAXT>;
+    static std::atomic<int> per_sm[MAXT / 32 + 1];  // CTAs an SM holds, by warps a CTA
+    std::atomic<int>& fit = per_sm[cta / 32];
+    int n = fit.load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, cta, 0) != cudaSuccess || n < 1) n = 1;
+        fit.store(n, std::memory_order_relaxed);
+    }
+    const int rows = WARP ? cta / 32 : 1;
+    int64_t grid = (int64_t(a.T) + rows - 1) / rows;
+    const int64_t most = int64_t(sm_count_norm()) * n;
+    if (grid > most) grid = most;
+    kern<<<unsigned(grid), cta, 0, s>>>(a);
     return cudaGetLastError();
 }
 
-template <int DT, bool RES32, bool AL, int V, int MAXT>
-static cudaError_t launch_norm_backward_v(const NormGradArgs& a, const NormGradPlan& p, cudaStream_t s) {
+template <int DT, bool RES32, bool AL>
+static cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
+    const int nt = row_threads_for(a.d, 2);
+    if (nt == 32) return launch_norm_as<DT, RES32, AL, true, 128>(a, 128, s);
+    if (nt <= 256) return launch_norm_as<DT, RES32, AL, false, 256>(a, nt, s);
+    return launch_norm_as<DT, RES32, AL, false, 1024>(a, nt, s);
+}
+
+// Shared memory of the ring that lets two CTAs (or the one of a wide row) stay on an SM.
+constexpr size_t kNormRingLimit = 200 * 1024;
+
+template <int DT, bool RES32, bool AL, bool RING, bool WARP, int V>
+static cudaError_t launch_norm_backward_as(const NormGradArgs& a, const NormGradPlan& p, size_t smem, cudaStream_t s) {
+    constexpr int kMax = WARP ? 128 : 512;
+    auto kern = block_norm_backward_kernel<DT, RES32, AL, RING, WARP, V, kMax>;
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (err != cudaSuccess) return err;
+    kern<<<p.grid, p.cta_threads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <int DT, bool RES32, bool AL>
+static cudaError_t launch_norm_backward(const NormGradArgs& a0, const NormGradPlan& p, cudaStream_t s) {
+    NormGradArgs a = a0;
     const int groups = p.cta_threads / p.row_threads;
-    const size_t smem = sizeof(float) * (2 * 4 * 32 + (groups > 1 ? a.d : 0));
-    block_norm_backward_kernel<DT, RES32, AL, V, MAXT><<<p.grid, p.cta_threads, smem, s>>>(a);
-    return cudaGetLastError();
-}
-
-template <int DT, bool RES32, bool AL>
-static cudaError_t launch_norm_backward(const NormGradArgs& a, const NormGradPlan& p, cudaStream_t s) {
-    if (p.v == 1) return launch_norm_backward_v<DT, RES32, AL, 1, 512>(a, p, s);
-    if (p.v == 2) return launch_norm_backward_v<DT, RES32, AL, 2, 512>(a, p, s);
-    return launch_norm_backward_v<DT, RES32, AL, 4, 512>(a, p, s);
+    int off = 0;
+    auto part = [&](bool present, int bytes) {
+        const int at = present ? off : -1;
+        off += present ? bytes : 0;
+        return at;
+    };
+    a.off_ds = part(a.d_res_out != nullptr, a.d * (RES32 ? 4 : 2));
+    a.off_rr = part(a.w_pre != nullptr, a.d * (RES32 ? 4 : 2));
+    a.off_dn = part(a.w_pre != nullptr, a.d * 2);
+    a.off_y = part(a.y != nullptr, a.d * 2);
+    a.off_gate = part(a.gate_form == kGateFull, a.d * 2);
+    a.row_bytes = off;
+    const size_t cols = groups > 1 ? size_t(a.d) * 4 : 0;
+    const size_t ring = size_t(groups) * kNormStages * off;
+    const bool use_ring = AL && p.v == 2 && ring <= kNormRingLimit;
+    const size_t smem = use_ring && ring > cols ? ring : cols;
+    const bool warp = p.row_threads == 32;
+    if constexpr (AL) {
+        if (use_ring) {
+            if (warp) return launch_norm_backward_as<DT, RES32, AL, true, true, 2>(a, p, smem, s);
+            return launch_norm_backward_as<DT, RES32, AL, true, false, 2>(a, p, smem, s);
+        }
+    }
+    if (warp) return launch_norm_backward_as<DT, RES32, AL, false, true, 2>(a, p, smem, s);
+    if (p.v == 2) return launch_norm_backward_as<DT, RES32, AL, false, false, 2>(a, p, smem, s);
+    return launch_norm_backward_as<DT, RES32, AL, false, false, 4>(a, p, smem, s);
 }
 
 template <typename F>
@@ -560,7 +679,7 @@ extern "C" int moe_b200_block_norm(const void* y, int64_t y_stride, const void* 
         return fail(MOE_B200_ERR_INVALID_ARG, "block_norm: row strides below d=%d", d);
     if (T == 0) return MOE_B200_OK;
     const NormArgs a{y, residual, w_post, w_pre, gate, y ? y_stride : 0, residual_stride, gate_form, scale, eps, T, d,
-                     0, y ? residual_out : nullptr, w_pre ? normed : nullptr};
+                     y ? residual_out : nullptr, w_pre ? normed : nullptr};
     const bool al = d % 8 == 0 && (!y || y_stride % 8 == 0) && residual_stride % (residual_f32 ? 4 : 8) == 0 &&
                     aligned16({y, residual, w_post, w_pre, gate_form >= kGateChannel ? gate : nullptr, a.residual_out,
                                a.normed});
@@ -571,10 +690,10 @@ extern "C" int moe_b200_block_norm(const void* y, int64_t y_stride, const void* 
     return err == cudaSuccess ? MOE_B200_OK : cuda_fail(err, "block_norm launch");
 }
 
-extern "C" size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d, int residual_f32) {
+extern "C" size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d, int /*residual_f32*/) {
     using namespace moe_b200;
     if (T < 0 || d < 1 || d > kNormMaxD) return 0;
-    return align256(size_t(3) * size_t(plan_norm_backward(T, d, residual_f32 != 0).grid) * size_t(d) * 4);
+    return align256(size_t(3) * size_t(plan_norm_backward(T, d).grid) * size_t(d) * 4);
 }
 
 extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const void* d_normed,
@@ -592,7 +711,7 @@ extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const vo
     if ((w_pre && residual_stride < d) || (y && y_stride < d))
         return fail(MOE_B200_ERR_INVALID_ARG, "block_norm_backward: row strides below d=%d", d);
     const bool res32 = residual_f32 != 0;
-    const NormGradPlan p = plan_norm_backward(T, d, res32);
+    const NormGradPlan p = plan_norm_backward(T, d);
     const int vectors = column_vectors(w_pre != nullptr, w_post != nullptr, gate_form);
     if (vectors && (!workspace || workspace_bytes < align256(size_t(vectors) * p.grid * size_t(d) * 4)))
         return fail(MOE_B200_ERR_WORKSPACE, "block_norm_backward: workspace too small");
@@ -611,9 +730,11 @@ extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const vo
         }
         return MOE_B200_OK;
     }
+    uint32_t* status = device_status_word();
+    if (!status) return fail(MOE_B200_ERR_CUDA, "block_norm_backward: device status word unavailable");
     const NormGradArgs a{d_residual_out, d_normed, residual_out, y, w_post, w_pre, gate, y ? y_stride : 0,
-                         w_pre ? residual_stride : 0, gate_form, scale, eps, T, d, p.row_threads, d_residual, d_y,
-                         d_gate, static_cast<float*>(workspace), i_pre, i_post, i_gate};
+                         w_pre ? residual_stride : 0, gate_form, scale, eps, T, d, d_residual, d_y, d_gate,
+                         static_cast<float*>(workspace), i_pre, i_post, i_gate, 0, -1, -1, -1, -1, -1, status};
     const bool al = d % 8 == 0 && a.y_stride % 8 == 0 && a.res_stride % (res32 ? 4 : 8) == 0 &&
                     aligned16({d_residual_out, d_normed, residual_out, y, w_post, w_pre,
                                gate_form >= kGateChannel ? gate : nullptr, d_residual, d_y,
@@ -622,7 +743,7 @@ extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const vo
         return launch_norm_backward<decltype(dt)::value, decltype(r32)::value, decltype(ali)::value>(a, p, s);
     });
     if (err == cudaSuccess && n > 0) {
-        cudaLaunchConfig_t cfg = pdl_config(dim3((d + 31) / 32, n), dim3(256), 0, s);
+        cudaLaunchConfig_t cfg = pdl_config(dim3((d + 31) / 32, n), dim3(1024), 0, s);
         cudaLaunchAttribute attr[1] = {pdl_attr()};
         cfg.attrs = attr;
         cfg.numAttrs = 1;

@@ -8,9 +8,10 @@
 //
 // With a few rows per expert the time is that of reading the chosen experts'
 // weights once (half a byte per weight), so the kernel streams them:
-//  - A CTA belongs to one expert (found from asgn on the device, no packing
-//    pass) and to a range of its weight rows; it lists the expert's slots and
-//    serves up to NT * 8 of them for one read of the weights.
+//  - Every CTA sorts the slots by expert in shared memory (a few hundred
+//    words, no packing pass) and takes an even share of all (expert, weight
+//    rows) units, so that any routing is balanced; up to NT * 8 slots of an
+//    expert are served by one read of its weights.
 //  - Weights keep their natural layout.  Each warp streams 32 weight rows x
 //    128 k (2 KB) per step through its own cp.async ring of kStages steps, so
 //    no registers and no barriers are spent on loads in flight.
@@ -59,10 +60,10 @@ struct W4Args {
     int swiglu;          // 1: gate rows [0, N/2), up rows [N/2, N)
     int n_out;           // output columns
     int tiles;           // warp tiles per expert
-    int tiles_per_cta, wk;
-    int by_slot;         // 1: blockIdx.y is a slot, the first slot of an expert serves it
+    int wk;              // warps that share a tile's k blocks
+    int units;           // units (8 / wk neighbouring tiles) per expert and pass
     int x_pitch;         // bytes of a staged x row
-    int s_x, s_red, s_list;  // offsets of the staged x, the join buffer and the slot list
+    int s_x, s_red, s_tab;  // offsets of the staged x, the join buffer and the slot tables
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
@@ -135,17 +136,6 @@ template <int DT> __device__ __forceinline__ uint16_t w4_to16(float f) {
     return DT == MOE_B200_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
 }
 
-// Row `r` (0..31) of tile `tile`: its weight row, or -1 past the last one.
-// SwiGLU: rows 0..15 are gate rows, rows 16..31 the matching up rows.
-__device__ __forceinline__ int w4_row(const W4Args& a, int tile, int r) {
-    if (a.swiglu) {
-        const int n = tile * 16 + (r & 15);
-        return n < a.n_out ? n + (r >> 4) * a.n_out : -1;
-    }
-    const int n = tile * kW4TileRows + r;
-    return n < a.N ? n : -1;
-}
-
 // Bytes of one ring step: weights, then per row and group a 4-byte word
 // holding its scale and one holding its zero point.
 template <int G> constexpr int w4_step_bytes() { return kW4StageBytes + 32 * (kW4Block / G) * 8; }
@@ -153,233 +143,340 @@ template <int G> constexpr int w4_step_bytes() { return kW4StageBytes + 32 * (kW
 // XS: x is staged in shared memory; otherwise (rows too long for it) each lane
 // reads its pieces of x from global memory, where they stay in L1 / L2.
 template <int DT, int G, int NT, bool XS>
-__global__ void __launch_bounds__(kW4Threads)
+__global__ void __launch_bounds__(kW4Threads, 2)
 expert_linear_w4_kernel(const W4Args a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int kGroups = kW4Block / G;  // groups of a row per step
     constexpr int kStep = w4_step_bytes<G>();
-    uint16_t* s_list = reinterpret_cast<uint16_t*>(smem + a.s_list);
-    __shared__ int s_warp[kW4Warps];
+    int* s_cnt = reinterpret_cast<int*>(smem + a.s_tab);  // [E] slots of an expert
+    int* s_first = s_cnt + a.E;                           // [E] its first place in s_slots
+    int* s_unit = s_first + a.E;                          // [E + 1] units of the experts before
+    int* s_cur = s_unit + a.E + 1;                        // [8][E] next place, by warp
+    uint16_t* s_slots = reinterpret_cast<uint16_t*>(s_cur + kW4Warps * a.E);  // [slots] by expert, ascending
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
 
-    int e = int(blockIdx.y);
-    if (a.by_slot) e = a.asgn[blockIdx.y];
-    const bool e_ok = e >= 0 && e < a.E;
+    // Slots by expert, ascending within an expert (every CTA has to find the
+    // same order: CTAs share an expert's slots by their places in it).  Each
+    // warp counts and deals one stretch of the slots.
+    const int part = ((a.slots + kW4Threads - 1) / kW4Threads) * 32;
+    const int s_lo = warp * part, s_hi = min(s_lo + part, a.slots);
+    for (int i = threadIdx.x; i < kW4Warps * a.E; i += kW4Threads) s_cur[i] = 0;
+    __syncthreads();
+    for (int s = s_lo + lane; s < s_hi; s += 32) {
+        const int e = a.asgn[s];
+        if (e >= 0 && e < a.E) atomicAdd(&s_cur[warp * a.E + e], 1);
+        else if (e != -1 && blockIdx.x == 0) atomicOr(a.status, MOE_B200_DEV_BAD_ASSIGNMENT);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int rows = 0, units = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            const int e = e0 + lane;
+            int c = 0;
+            if (e < a.E)
+                for (int w = 0; w < kW4Warps; ++w) c += s_cur[w * a.E + e];
+            int r = c, u = (c + NT * 8 - 1) / (NT * 8) * a.units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int rv = __shfl_up_sync(0xffffffffu, r, o), uv = __shfl_up_sync(0xffffffffu, u, o);
+                if (lane >= o) r += rv, u += uv;
+            }
+            if (e < a.E) {
+                s_cnt[e] = c;
+                int at = rows + r - c;
+                s_first[e] = at;
+                for (int w = 0; w < kW4Warps; ++w) {
+                    const int n = s_cur[w * a.E + e];
+                    s_cur[w * a.E + e] = at;
+                    at += n;
+                }
+                s_unit[e + 1] = units + u;
+            }
+            rows += __shfl_sync(0xffffffffu, r, 31);
+            units += __shfl_sync(0xffffffffu, u, 31);
+        }
+        if (lane == 0) s_unit[0] = 0;
+    }
+    __syncthreads();
+    for (int s0 = s_lo; s0 < s_hi; s0 += 32) {
+        const int s = s0 + lane;
+        const int e = s < s_hi ? a.asgn[s] : -1;
+        const bool ok = e >= 0 && e < a.E;
+        const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
+        int base = 0;
+        if (ok) base = s_cur[warp * a.E + e];
+        __syncwarp();
+        if (ok) {
+            s_slots[base + __popc(same & lanemask_lt())] = uint16_t(s);
+            if ((same & lanemask_lt()) == 0) s_cur[warp * a.E + e] = base + __popc(same);
+        }
+        __syncwarp();
+    }
+    // Slots without an expert get rows of zeros, dealt over the grid.
+    for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
+        const int e = a.asgn[s];
+        if (e >= 0 && e < a.E) continue;
+        for (int c = threadIdx.x; c < a.n_out; c += kW4Threads)
+            static_cast<uint16_t*>(a.out)[int64_t(s) * a.n_out + c] = 0;
+    }
+    __syncthreads();
+
+    // This CTA's even share of all units.
+    const int64_t total = s_unit[a.E];
+    const int u_begin = int(total * blockIdx.x / gridDim.x), u_end = int(total * (blockIdx.x + 1) / gridDim.x);
+    if (u_begin >= u_end) return;
 
     const int wk = a.wk, wn_count = kW4Warps / wk, kw = warp % wk, wn = warp / wk;
-    const int tile0 = int(blockIdx.x) * a.tiles_per_cta;
-    const int tile_end = min(tile0 + a.tiles_per_cta, a.tiles);
-    const int steps = (a.tiles_per_cta + wn_count - 1) / wn_count;  // tiles a warp walks
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     const int my_blocks = blocks > kw ? (blocks - kw + wk - 1) / wk : 0;
-    const int iters = steps * my_blocks;  // of one pass over the weights
     const int ngroups = a.K / G;
-    const uint32_t ring = smem_u32(smem) + warp * (kW4Stages * kStep);
-    const int64_t row_bytes = a.K / 2;
+    const int row_bytes = a.K / 2;
 
-    // Step `i` of a pass: tile tile0 + (i / my_blocks) * wn_count + wn, k block kw + (i % my_blocks) * wk.
-    auto issue = [&](int i) {
-        if (i < iters && e_ok) {
-            const int tile = tile0 + (i / my_blocks) * wn_count + wn, b = kw + (i % my_blocks) * wk;
-            const uint32_t dst = ring + (i % kW4Stages) * kStep;
-            const bool tile_ok = tile < tile_end;
+    // A place in the walk over units: expert, unit of its current pass, pass.
+    struct Place {
+        int u, e, tg, pass;
+    };
+    auto expert_of = [&](int u) {  // last expert with s_unit[e] <= u
+        int lo = 0, hi = a.E - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_unit[mid] <= u) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    auto place_at = [&](int u) {
+        Place p;
+        p.u = u;
+        p.e = expert_of(u);
+        const int local = u - s_unit[p.e];
+        p.pass = local / a.units;
+        p.tg = local - p.pass * a.units;
+        return p;
+    };
+    auto advance = [&](Place& p) {
+        ++p.u;
+        if (++p.tg < a.units) return;
+        p.tg = 0;
+        ++p.pass;
+        if (p.u >= s_unit[p.e + 1] && p.u < u_end) {
+            p.e = expert_of(p.u);
+            p.pass = 0;
+        }
+    };
+
+    // ---- weights: a ring of steps per warp, filled ahead by the same walk ----
+    const uint32_t ring = smem_u32(smem) + warp * (kW4Stages * kStep);
+    Place pf = place_at(u_begin);
+    int pf_b = 0, pf_slot = 0;    // block of this warp, ring slot
+    const uint8_t* pf_w = nullptr;  // row g of the tile, this lane's 16 bytes of the block
+    int64_t pf_s = 0;               // index of the scale of row `lane`, this block
+    uint32_t pf_ok = 0;             // bit j: rows 8j .. 8j+7 of the tile exist
+    // Rows 8j + g, j = 0..3, of a tile lie at these distances from row g.
+    const int64_t off1 = 8 * int64_t(row_bytes);
+    const int64_t off2 = a.swiglu ? int64_t(a.n_out) * row_bytes : 16 * int64_t(row_bytes);
+    auto pf_tile = [&]() {
+        const int tile = pf.tg * wn_count + wn;
+        const int n0 = tile * (a.swiglu ? 16 : kW4TileRows);
+        pf_ok = 0;
+        if (tile < a.tiles) {
+            // N (SwiGLU: N/2) is a multiple of 8: eight rows exist together
+            if (a.swiglu) pf_ok = 5u | (n0 + 8 < a.n_out ? 10u : 0u);
+            else pf_ok = 1u | (n0 + 8 < a.N ? 2u : 0u) | (n0 + 16 < a.N ? 4u : 0u) | (n0 + 24 < a.N ? 8u : 0u);
+        }
+        const int64_t row = int64_t(pf.e) * a.N + n0;
+        pf_w = a.wq + (row + g) * row_bytes + kw * (kW4Block / 2) + t * 16;
+        const int lane_row = a.swiglu ? (lane & 15) + (lane >> 4) * a.n_out : lane;
+        pf_s = (row + lane_row) * ngroups + kw * kGroups;
+    };
+    auto issue = [&]() {
+        if (pf.u < u_end && my_blocks > 0) {
+            const uint32_t dst = ring + pf_slot * kStep;
+            const int b = kw + pf_b * wk;
+            const bool k_ok = b * kW4Block + t * 32 < a.K;
+            // 16-byte pieces of row r sit at piece ^ (r / 2 mod 4): word reads are free of bank conflicts
+            const uint32_t d = dst + g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int r = j * 8 + g;  // 8 rows x 64 bytes per instruction
-                const int n = tile_ok ? w4_row(a, tile, r) : -1;
-                const bool ok = n >= 0 && b * kW4Block + t * 32 < a.K;
-                const uint8_t* src = ok ? a.wq + (int64_t(e) * a.N + n) * row_bytes + b * (kW4Block / 2) + t * 16 : a.wq;
-                // 16-byte pieces of a row sit at piece ^ (row / 2 mod 4): word reads are free of bank conflicts
-                cp_async16(dst + r * 64 + ((t ^ ((r >> 1) & 3)) << 4), src, ok);
+                const bool ok = k_ok && ((pf_ok >> j) & 1);
+                cp_async16(d + j * 512, ok ? pf_w + (j & 1) * off1 + (j >> 1) * off2 : a.wq, ok);
             }
-            const int n = tile_ok ? w4_row(a, tile, lane) : -1;
+            const bool r_ok = (pf_ok >> (lane >> 3)) & 1;
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) {
-                const int grp = b * kGroups + q;
-                const bool ok = n >= 0 && grp < ngroups;
-                const int64_t at = ok ? (int64_t(e) * a.N + n) * ngroups + grp : 0;
-                const uint32_t d = dst + kW4StageBytes + (q * 32 + lane) * 8;
-                cp_async4(d, static_cast<const uint16_t*>(a.scale) + (at & ~int64_t(1)), ok);
-                if (a.zero) cp_async4(d + 4, a.zero + (at & ~int64_t(3)), ok);
+                const bool ok = r_ok && b * kGroups + q < ngroups;
+                const int64_t at = ok ? pf_s + q : 0;
+                const uint32_t ds = dst + kW4StageBytes + (q * 32 + lane) * 8;
+                cp_async4(ds, static_cast<const uint16_t*>(a.scale) + (at & ~int64_t(1)), ok);
+                if (a.zero) cp_async4(ds + 4, a.zero + (at & ~int64_t(3)), ok);
+            }
+            pf_slot = pf_slot + 1 == kW4Stages ? 0 : pf_slot + 1;
+            if (++pf_b < my_blocks) {
+                pf_w += wk * (kW4Block / 2);
+                pf_s += wk * kGroups;
+            } else {
+                pf_b = 0;
+                advance(pf);
+                if (pf.u < u_end) pf_tile();
             }
         }
         cp_commit();
     };
+    pf_tile();
 #pragma unroll
-    for (int i = 0; i < kW4Stages - 1; ++i) issue(i);
-
-    // The expert's slots in ascending order; slots without an expert (-1 or
-    // out of range) get rows of zeros from the first row of CTAs.
-    int count = 0;
-    bool earlier = false;
-    for (int s0 = 0; s0 < a.slots; s0 += kW4Threads) {
-        const int s = s0 + threadIdx.x;
-        const int v = s < a.slots ? a.asgn[s] : -1;
-        const bool mine = e_ok && s < a.slots && v == e;
-        if (mine && a.by_slot && s < int(blockIdx.y)) earlier = true;
-        const uint32_t m = __ballot_sync(0xffffffffu, mine);
-        if (lane == 0) s_warp[warp] = __popc(m);
-        __syncthreads();
-        int at = count;
-        for (int w = 0; w < kW4Warps; ++w) {
-            if (w < warp) at += s_warp[w];
-            count += s_warp[w];
-        }
-        if (mine) s_list[at + __popc(m & lanemask_lt())] = uint16_t(s);
-        if (blockIdx.y == 0 && s < a.slots && (v < 0 || v >= a.E)) {
-            if (v != -1 && blockIdx.x == 0) atomicOr(a.status, MOE_B200_DEV_BAD_ASSIGNMENT);
-            const int per = a.swiglu ? 16 : kW4TileRows;
-            for (int c = tile0 * per; c < min(tile_end * per, a.n_out); ++c)
-                static_cast<uint16_t*>(a.out)[int64_t(s) * a.n_out + c] = 0;
-        }
-        __syncthreads();
-    }
-    if (__syncthreads_or(earlier ? 1 : 0) || count == 0) {
-        cp_wait<0>();
-        return;
-    }
+    for (int i = 0; i < kW4Stages - 1; ++i) issue();
 
     const uint32_t sx = smem_u32(smem + a.s_x);
     float* s_red = reinterpret_cast<float*>(smem + a.s_red);
-    for (int r0 = 0; r0 < count; r0 += NT * 8) {
-        const int nrows = min(count - r0, NT * 8);
-        const int nt = (nrows + 7) >> 3;
-        if (r0 > 0) {  // the next rows read the weights again (from L2)
+    Place at = place_at(u_begin);
+    int staged_e = -1, staged_pass = 0, nrows = 0, nt = 0, list0 = 0, slot = 0;
+    const uint16_t* x_row[NT];
+    for (; at.u < u_end; advance(at)) {
+        if (at.e != staged_e || at.pass != staged_pass) {
+            staged_e = at.e, staged_pass = at.pass;
+            const int cnt = s_cnt[at.e];
+            list0 = s_first[at.e] + at.pass * NT * 8;
+            nrows = min(cnt - at.pass * NT * 8, NT * 8);
+            nt = (nrows + 7) >> 3;
+            if (XS) {  // zeros past K and past the last row
+                const int chunks = blocks * (kW4Block / 8);
+                for (int r = 0; r < nt * 8; ++r) {
+                    const uint16_t* row =
+                        r < nrows ? static_cast<const uint16_t*>(a.x) + int64_t(s_slots[list0 + r] / a.x_div) * a.K : nullptr;
+                    for (int c = threadIdx.x; c < chunks; c += kW4Threads) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (row && c * 8 < a.K) v = *reinterpret_cast<const uint4*>(row + c * 8);
+                        *reinterpret_cast<uint4*>(smem + a.s_x + r * a.x_pitch + c * 16) = x_pairs(v);
+                    }
+                }
+                __syncthreads();
+            } else {
 #pragma unroll
-            for (int i = 0; i < kW4Stages - 1; ++i) issue(i);
-        }
-        // Stage x, zeros past K and past the last row.
-        const uint16_t* x_row[NT];
-        if (XS) {
-            const int chunks = blocks * (kW4Block / 8);
-            for (int c = threadIdx.x; c < nt * 8 * chunks; c += kW4Threads) {
-                const int r = c / chunks, k8 = c - r * chunks;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < nrows && k8 * 8 < a.K)
-                    v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) +
-                                                        int64_t(s_list[r0 + r] / a.x_div) * a.K + k8 * 8);
-                *reinterpret_cast<uint4*>(smem + a.s_x + r * a.x_pitch + k8 * 16) = x_pairs(v);
+                for (int q = 0; q < NT; ++q)
+                    x_row[q] = q * 8 + g < nrows ? static_cast<const uint16_t*>(a.x) +
+                                                       int64_t(s_slots[list0 + q * 8 + g] / a.x_div) * a.K + t * 8
+                                                 : nullptr;
             }
-            __syncthreads();
-        } else {
+        }
+        const int tile = at.tg * wn_count + wn;
+        // Low bits of the scale index of this lane's four rows (group 0): which
+        // half of the 4-byte word holds the scale, which byte the zero point.
+        uint32_t low[2][2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t n = a.swiglu ? uint32_t(tile * 16 + h * 8 + g + m * a.n_out)
+                                            : uint32_t(tile * kW4TileRows + m * 16 + h * 8 + g);
+                low[m][h] = (uint32_t(at.e) * uint32_t(a.N) + n) * uint32_t(ngroups);
+            }
+        float acc[2][NT][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int q = 0; q < NT; ++q)
-                x_row[q] = q * 8 + g < nrows ? static_cast<const uint16_t*>(a.x) +
-                                                   int64_t(s_list[r0 + q * 8 + g] / a.x_div) * a.K + t * 8
-                                             : nullptr;
-        }
-
-        int i = 0;
-        for (int step = 0; step < steps; ++step) {
-            const int tile = tile0 + step * wn_count + wn;
-            float acc[2][NT][4];
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+                for (int j = 0; j < 4; ++j) acc[m][q][j] = 0.f;
+#pragma unroll 1
+        for (int jb = 0; jb < my_blocks; ++jb) {
+            cp_wait<kW4Stages - 2>();
+            __syncwarp();
+            issue();  // into the step read last time
+            const uint32_t st = ring + slot * kStep;
+            slot = slot + 1 == kW4Stages ? 0 : slot + 1;
+            const int b = kw + jb * wk;
+            const uint32_t xb = sx + b * (kW4Block * 2) + t * 16 + g * a.x_pitch;
+            const uint32_t swz = (g >> 1) & 3;
+            const uint32_t wb = st + g * 64 + t * 4;
 #pragma unroll
-                for (int q = 0; q < NT; ++q)
+            for (int q4 = 0; q4 < kGroups; ++q4) {
+                float sc[2][2];
+                uint32_t z2[2][2];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[m][q][j] = 0.f;
-            for (int jb = 0; jb < my_blocks; ++jb, ++i) {
-                cp_wait<kW4Stages - 2>();
-                __syncwarp();
-                issue(i + kW4Stages - 1);  // into the step read last time
-                const uint32_t st = ring + (i % kW4Stages) * kStep;
-                const int b = kw + jb * wk;
-                const uint32_t xb = sx + b * (kW4Block * 2) + t * 16;
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int q4 = 0; q4 < kGroups; ++q4) {
-                    // scales and zero points of this lane's four rows
-                    float sc[2][2];
-                    uint32_t z2[2][2];
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int r = m * 16 + h * 8 + g;
-                            const uint32_t d = st + kW4StageBytes + (q4 * 32 + r) * 8;
-                            const int n = w4_row(a, tile, r);
-                            const uint32_t at = uint32_t(e * a.N + n) * uint32_t(ngroups) + uint32_t(b * kGroups + q4);
-                            const uint32_t sw = lds32(d);
-                            sc[m][h] = w4_from16<DT>((at & 1) ? (sw >> 16) : (sw & 0xffffu));
-                            uint32_t z = 8;
-                            if (a.zero) z = (lds32(d + 4) >> (8 * (at & 3))) & 0xffu;
-                            z2[m][h] = z * 0x00010001u | magic<DT>();
-                        }
-                    float d4[2][NT][4];
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int q = 0; q < NT; ++q)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) d4[m][q][j] = 0.f;
-#pragma unroll
-                    for (int s4 = 0; s4 < G / 32; ++s4) {
-                        const int s = q4 * (G / 32) + s4;  // 32 k of the block
-                        uint4 xv[NT];
-#pragma unroll
-                        for (int q = 0; q < NT; ++q)
-                            if (XS) {
-                                if (q < nt) xv[q] = lds128(xb + (q * 8 + g) * a.x_pitch + s * 64);
-                            } else {
-                                const int k = b * kW4Block + s * 32;
-                                xv[q] = make_uint4(0, 0, 0, 0);
-                                if (x_row[q] && k < a.K) xv[q] = x_pairs(*reinterpret_cast<const uint4*>(x_row[q] + k));
-                            }
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            uint32_t lo[4], hi[4];
-                            const int ra = m * 16 + g, rb = ra + 8;
-                            unpack8<DT>(lds32(st + ra * 64 + ((s ^ ((ra >> 1) & 3)) << 4) + t * 4), z2[m][0], lo);
-                            unpack8<DT>(lds32(st + rb * 64 + ((s ^ ((rb >> 1) & 3)) << 4) + t * 4), z2[m][1], hi);
-#pragma unroll
-                            for (int q = 0; q < NT; ++q)
-                                if (q < nt) {
-                                    mma_16816<DT>(d4[m][q], lo[0], hi[0], lo[1], hi[1], xv[q].x, xv[q].y);
-                                    mma_16816<DT>(d4[m][q], lo[2], hi[2], lo[3], hi[3], xv[q].z, xv[q].w);
-                                }
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t d = st + kW4StageBytes + (q4 * 32 + m * 16 + h * 8 + g) * 8;
+                        const uint32_t i = low[m][h] + uint32_t(b * kGroups + q4);
+                        sc[m][h] = w4_from16<DT>((lds32(d) >> ((i & 1) * 16)) & 0xffffu);
+                        const uint32_t z = a.zero ? (lds32(d + 4) >> ((i & 3) * 8)) & 0xffu : 8u;
+                        z2[m][h] = z * 0x00010001u | magic<DT>();
                     }
+                float d4[2][NT][4];
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int q = 0; q < NT; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) d4[m][q][j] = 0.f;
+#pragma unroll
+                for (int s4 = 0; s4 < G / 32; ++s4) {
+                    const int s = q4 * (G / 32) + s4;  // 32 k of the block
+                    uint4 xv[NT];
+#pragma unroll
+                    for (int q = 0; q < NT; ++q)
+                        if (XS) {
+                            if (q < nt) xv[q] = lds128(xb + q * 8 * a.x_pitch + s * 64);
+                        } else {
+                            const int k = b * kW4Block + s * 32;
+                            xv[q] = make_uint4(0, 0, 0, 0);
+                            if (x_row[q] && k < a.K) xv[q] = x_pairs(*reinterpret_cast<const uint4*>(x_row[q] + k));
+                        }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        uint32_t lo[4], hi[4];
+                        const uint32_t wa = wb + m * 1024 + ((uint32_t(s) ^ swz) << 4);
+                        unpack8<DT>(lds32(wa), z2[m][0], lo);
+                        unpack8<DT>(lds32(wa + 512), z2[m][1], hi);
 #pragma unroll
                         for (int q = 0; q < NT; ++q)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) acc[m][q][j] += sc[m][j >> 1] * d4[m][q][j];
+                            if (q < nt) {
+                                mma_16816<DT>(d4[m][q], lo[0], hi[0], lo[1], hi[1], xv[q].x, xv[q].y);
+                                mma_16816<DT>(d4[m][q], lo[2], hi[2], lo[3], hi[3], xv[q].z, xv[q].w);
+                            }
+                    }
                 }
-                __syncwarp();  // the step is read before its refill
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int q = 0; q < NT; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[m][q][j] += sc[m][j >> 1] * d4[m][q][j];
             }
-            // Join the WK parts: [warp][m][q][lane][4] floats.
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int q = 0; q < NT; ++q)
-                    if (q < nt)
-                        *reinterpret_cast<float4*>(s_red + (((warp * 2 + m) * NT + q) * 32 + lane) * 4) =
-                            make_float4(acc[m][q][0], acc[m][q][1], acc[m][q][2], acc[m][q][3]);
-            __syncthreads();
-            // One output a thread and turn: value j of lane l of the fragment
-            // is row l/4 + 8*(j/2), column (l%4)*2 + j%2.
-            const int per = (a.swiglu ? 1 : 2) * nt * 128;
-            for (int o = threadIdx.x; o < wn_count * per; o += kW4Threads) {
-                const int w2 = o / per, rem = o - w2 * per, f = rem >> 7, l = (rem & 127) >> 2, j = rem & 3;
-                const int m = a.swiglu ? 0 : f / nt, q = a.swiglu ? f : f - m * nt;
-                float v0 = 0.f, v1 = 0.f;
-                for (int w = 0; w < wk; ++w) {
-                    const float* p = s_red + ((((w2 * wk + w) * 2 + m) * NT + q) * 32 + l) * 4 + j;
-                    v0 += p[0];
-                    if (a.swiglu) v1 += p[NT * 128];
-                }
-                const int tl = tile0 + step * wn_count + w2, col = q * 8 + (l & 3) * 2 + (j & 1);
-                const int rr = (l >> 2) + (j >> 1) * 8;
-                const int n = a.swiglu ? tl * 16 + rr : tl * kW4TileRows + m * 16 + rr;
-                if (tl < tile_end && n < a.n_out && col < nrows) {
-                    if (a.swiglu) v0 = v0 / (1.0f + __expf(-v0)) * v1;
-                    static_cast<uint16_t*>(a.out)[int64_t(s_list[r0 + col]) * a.n_out + n] = w4_to16<DT>(v0);
-                }
-            }
-            __syncthreads();
+            __syncwarp();  // the step is read before its refill
         }
+        // Join the WK parts: [warp][m][q][lane][4] floats.  Value j of lane l
+        // is row l/4 + 8*(j/2), column (l%4)*2 + j%2 of the 16 x 8 fragment.
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+                *reinterpret_cast<float4*>(s_red + (((warp * 2 + m) * NT + q) * 32 + lane) * 4) =
+                    make_float4(acc[m][q][0], acc[m][q][1], acc[m][q][2], acc[m][q][3]);
+        __syncthreads();
+        // A thread sums one value of (tile, q) for both m and writes them, or their SwiGLU.
+        for (int o = threadIdx.x; o < wn_count * NT * 128; o += kW4Threads) {
+            const int q = (o >> 7) % NT, w2 = (o >> 7) / NT, l = (o & 127) >> 2, j = o & 3;
+            const int tl = at.tg * wn_count + w2, col = q * 8 + (l & 3) * 2 + (j & 1), rr = (l >> 2) + (j >> 1) * 8;
+            if (col >= nrows || tl >= a.tiles) continue;
+            float v[2] = {0.f, 0.f};
+            const float* p = s_red + ((w2 * wk * 2 * NT + q) * 32 + l) * 4 + j;
+            for (int w = 0; w < wk; ++w) {
+                v[0] += p[w * (2 * NT * 128)];
+                v[1] += p[w * (2 * NT * 128) + NT * 128];
+            }
+            uint16_t* out = static_cast<uint16_t*>(a.out) + int64_t(s_slots[list0 + col]) * a.n_out;
+            if (a.swiglu) {
+                const int n = tl * 16 + rr;
+                if (n < a.n_out) out[n] = w4_to16<DT>(v[0] / (1.0f + __expf(-v[0])) * v[1]);
+            } else {
+                const int n = tl * kW4TileRows + rr;
+                if (n < a.N) out[n] = w4_to16<DT>(v[0]);
+                if (n + 16 < a.N) out[n + 16] = w4_to16<DT>(v[1]);
+            }
+        }
+        __syncthreads();
     }
     cp_wait<0>();
 }
@@ -402,8 +499,8 @@ static size_t w4_layout(W4Args& a, int nt, bool xs) {
     off += xs ? size_t(nt) * 8 * a.x_pitch : 0;
     a.s_red = int(off);
     off += size_t(kW4Warps) * 2 * nt * 128 * 4;
-    a.s_list = int(off);
-    off += (size_t(a.slots) * 2 + 15) & ~size_t(15);
+    a.s_tab = int(off);
+    off += size_t((3 + kW4Warps) * a.E + 1) * 4 + ((size_t(a.slots) * 2 + 15) & ~size_t(15));
     return off;
 }
 
@@ -419,19 +516,22 @@ static cudaError_t launch_w4(W4Args a, dim3 grid, cudaStream_t s) {
 
 template <int DT, int G>
 static cudaError_t run_w4(W4Args a, cudaStream_t s) {
-    a.by_slot = a.slots < a.E;
-    const int served = a.by_slot ? a.slots : a.E;  // experts that may have work
-    // Rows served per read of the weights: 8, or 16 when some expert may have more and they fit.
-    const bool two = a.slots > 8 && w4_layout<G>(a, 2, true) <= kW4SmemLimit;
+    const int served = a.slots < a.E ? a.slots : a.E;  // experts that may have work
+    // Warps that share a tile's k: as many as lose less than an eighth of their
+    // steps to an uneven split.
+    const int blocks = (a.K + kW4Block - 1) / kW4Block;
+    a.wk = kW4Warps;
+    while (a.wk > 1 && 8 * blocks < 7 * a.wk * ((blocks + a.wk - 1) / a.wk)) a.wk /= 2;
+    a.units = (a.tiles + kW4Warps / a.wk - 1) / (kW4Warps / a.wk);
+    // Rows served per read of the weights: 8, or 16 when experts have more than that on average.
+    const bool two = a.slots > 8 * served && w4_layout<G>(a, 2, true) <= kW4SmemLimit;
     const bool staged = two || w4_layout<G>(a, 1, true) <= kW4SmemLimit;
-    a.wk = 8;
-    const int64_t units = int64_t(a.tiles) * served;
-    a.tiles_per_cta = int(units / (int64_t(sm_count_w4()) * 8));
-    if (a.tiles_per_cta < 1) a.tiles_per_cta = 1;
-    if (a.tiles_per_cta > 8) a.tiles_per_cta = 8;
-    const dim3 grid((a.tiles + a.tiles_per_cta - 1) / a.tiles_per_cta, served);
-    if (two) return launch_w4<DT, G, 2, true>(a, grid, s);
-    return staged ? launch_w4<DT, G, 1, true>(a, grid, s) : launch_w4<DT, G, 1, false>(a, grid, s);
+    const int64_t most = int64_t(a.units) * (a.slots < a.E ? a.slots : a.E + a.slots / 8);
+    int64_t grid = 2 * sm_count_w4();
+    if (grid > most) grid = most;
+    if (two) return launch_w4<DT, G, 2, true>(a, dim3(unsigned(grid)), s);
+    return staged ? launch_w4<DT, G, 1, true>(a, dim3(unsigned(grid)), s)
+                  : launch_w4<DT, G, 1, false>(a, dim3(unsigned(grid)), s);
 }
 
 }  // namespace moe_b200

@@ -487,9 +487,11 @@ def _refuse(what: str, why: str):
 
 def _rows(what, name, t, shape, dtype, strided=False):
     """Checks a tensor's shape, type and layout (strided: rows may lie apart)."""
+    if t.shape == shape and t.dtype == dtype and t.is_contiguous():
+        return
     if t.shape != shape or t.dtype != dtype:
         _refuse(what, f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if not t.is_contiguous() and not (strided and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+    if not (strided and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
         _refuse(what, f"{name} must be contiguous" + (" or have contiguous rows that do not overlap" if strided else ""))
 
 
@@ -508,16 +510,16 @@ def _enqueue(what, fn, dev, stream, fresh, *args):
     call allocated, which the allocator must not hand out again before the
     work on `stream` is done."""
     import torch
-    if stream is None:
-        handle = torch.cuda.current_stream(dev).cuda_stream or None
-    else:
-        handle = _stream_handle(stream)
-        s = torch.cuda.ExternalStream(handle or 0, device=dev) if isinstance(stream, int) else stream
-        if s != torch.cuda.current_stream(dev):
+    index = dev.index
+    handle = torch._C._cuda_getCurrentRawStream(index) or None
+    if stream is not None:
+        current, handle = handle, _stream_handle(stream)
+        if handle != current:
+            s = torch.cuda.ExternalStream(handle or 0, device=dev)
             for t in fresh:
                 if t is not None:
                     t.record_stream(s)
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == index:
         status = fn(*args, handle)
     else:
         with torch.cuda.device(dev):
@@ -595,8 +597,9 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
     fresh = ()
     if out is None:
         fresh = out = BlockNormResult(
-            residual_out=torch.empty((T, d), dtype=residual.dtype, device=dev) if y is not None else None,
-            normed=torch.empty((T, d), dtype=dtype, device=dev) if w_pre is not None else None)
+            residual_out=torch.empty_like(residual, memory_format=torch.contiguous_format) if y is not None else None,
+            normed=torch.empty_like(some if some is y else residual, dtype=dtype, memory_format=torch.contiguous_format)
+            if w_pre is not None else None)
     else:
         if (out.residual_out is None) != (y is None) or (out.normed is None) != (w_pre is None):
             _refuse("block_norm", "out needs residual_out with y and normed with w_pre, and neither without")
