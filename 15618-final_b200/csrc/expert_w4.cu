@@ -13,8 +13,9 @@
 //    rows) units, so that any routing is balanced; up to NT * 8 slots of an
 //    expert are served by one read of its weights.
 //  - Weights keep their natural layout.  Each warp streams 32 weight rows x
-//    128 k (2 KB) per step through its own cp.async ring of kStages steps, so
-//    no registers and no barriers are spent on loads in flight.
+//    256 k (4 KB) per step through its own ring: two TMA boxes of 16 rows x
+//    128 bytes, whose 128-byte swizzle makes the word reads free of bank
+//    conflicts; no registers and no barriers are spent on loads in flight.
 //  - mma.sync m16n8k16 with the weights as the 16-row operand and 8 slots as
 //    the columns.  A 32-bit word holds 8 consecutive k of one row; the order
 //    of k inside a product does not matter as long as both operands agree, so
@@ -26,11 +27,13 @@
 //    by its scale.
 //  - The k blocks are split over the CTA's warps (WK ways) and joined in
 //    shared memory in warp order: results do not depend on timing.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace moe_b200 {
 
@@ -39,8 +42,8 @@ int cuda_fail(cudaError_t err, const char* where);
 
 constexpr int kW4Warps = 8;
 constexpr int kW4Threads = kW4Warps * 32;
-constexpr int kW4Stages = 4;
-constexpr int kW4Block = 128;       // k per step
+constexpr int kW4Stages = 2;
+constexpr int kW4Block = 256;       // k per step
 constexpr int kW4TileRows = 32;     // weight rows per warp step: two 16-row operands
 constexpr int kW4StageBytes = kW4TileRows * kW4Block / 2;
 constexpr int kW4MaxSlots = 4096;
@@ -50,7 +53,6 @@ constexpr size_t kW4SmemLimit = 227 * 1024 - 1024;
 struct W4Args {
     const void* x;
     const int32_t* asgn;
-    const uint8_t* wq;
     const void* scale;
     const uint8_t* zero;
     void* out;
@@ -66,27 +68,13 @@ struct W4Args {
     int s_x, s_red, s_tab;  // offsets of the staged x, the join buffer and the slot tables
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-    return v;
-}
-
 // 16-bit integers 0..15 as floats with an offset: 0x6400 | q is 1024 + q in
 // fp16, 0x4300 | q is 128 + q in bf16, both exact.
 template <int DT> __device__ __forceinline__ constexpr uint32_t magic() {
@@ -100,10 +88,16 @@ template <int DT> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t 
     __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&r);
 }
-// (nibble i, nibble i+4) - z for i = 0..3 of a word
+// (w & mask) | bits in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+// (nibble i, nibble i+4) - z for i = 0..3 of a word, z2 = the magic number + z twice
 template <int DT> __device__ __forceinline__ void unpack8(uint32_t w, uint32_t z2, uint32_t (&o)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = sub2<DT>(((w >> (4 * i)) & 0x000f000fu) | magic<DT>(), z2);
+    for (int i = 0; i < 4; ++i) o[i] = sub2<DT>(and_or(i ? w >> (4 * i) : w, 0x000f000fu, magic<DT>()), z2);
 }
 
 // Eight consecutive x in the order of a weight word's nibbles: (0,4) (1,5) (2,6) (3,7).
@@ -112,21 +106,21 @@ __device__ __forceinline__ uint4 x_pairs(const uint4& v) {
                       __byte_perm(v.y, v.w, 0x7632));
 }
 
-template <int DT>
+// c = A . B (FIRST) or c += A . B
+template <int DT, bool FIRST>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
+    const float i0 = FIRST ? 0.f : c[0], i1 = FIRST ? 0.f : c[1], i2 = FIRST ? 0.f : c[2], i3 = FIRST ? 0.f : c[3];
     if (DT == MOE_B200_BF16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %11, %12, %13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(i0), "f"(i1), "f"(i2), "f"(i3));
     else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %11, %12, %13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(i0), "f"(i1), "f"(i2), "f"(i3));
 }
 
 template <int DT> __device__ __forceinline__ float w4_from16(uint32_t b) {
@@ -136,18 +130,14 @@ template <int DT> __device__ __forceinline__ uint16_t w4_to16(float f) {
     return DT == MOE_B200_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
 }
 
-// Bytes of one ring step: weights, then per row and group a 4-byte word
-// holding its scale and one holding its zero point.
-template <int G> constexpr int w4_step_bytes() { return kW4StageBytes + 32 * (kW4Block / G) * 8; }
-
 // XS: x is staged in shared memory; otherwise (rows too long for it) each lane
 // reads its pieces of x from global memory, where they stay in L1 / L2.
 template <int DT, int G, int NT, bool XS>
 __global__ void __launch_bounds__(kW4Threads, 2)
-expert_linear_w4_kernel(const W4Args a) {
-    extern __shared__ __align__(128) unsigned char smem[];
+expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ uint64_t s_full[kW4Warps][kW4Stages];
     constexpr int kGroups = kW4Block / G;  // groups of a row per step
-    constexpr int kStep = w4_step_bytes<G>();
     int* s_cnt = reinterpret_cast<int*>(smem + a.s_tab);  // [E] slots of an expert
     int* s_first = s_cnt + a.E;                           // [E] its first place in s_slots
     int* s_unit = s_first + a.E;                          // [E + 1] units of the experts before
@@ -163,12 +153,14 @@ expert_linear_w4_kernel(const W4Args a) {
     const int s_lo = warp * part, s_hi = min(s_lo + part, a.slots);
     for (int i = threadIdx.x; i < kW4Warps * a.E; i += kW4Threads) s_cur[i] = 0;
     __syncthreads();
+    bool none = false;
     for (int s = s_lo + lane; s < s_hi; s += 32) {
         const int e = a.asgn[s];
         if (e >= 0 && e < a.E) atomicAdd(&s_cur[warp * a.E + e], 1);
         else if (e != -1 && blockIdx.x == 0) atomicOr(a.status, MOE_B200_DEV_BAD_ASSIGNMENT);
+        none |= e < 0 || e >= a.E;
     }
-    __syncthreads();
+    none = __syncthreads_or(none);
     if (warp == 0) {
         int rows = 0, units = 0;
         for (int e0 = 0; e0 < a.E; e0 += 32) {
@@ -214,7 +206,7 @@ expert_linear_w4_kernel(const W4Args a) {
         __syncwarp();
     }
     // Slots without an expert get rows of zeros, dealt over the grid.
-    for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
+    for (int s = blockIdx.x; none && s < a.slots; s += gridDim.x) {
         const int e = a.asgn[s];
         if (e >= 0 && e < a.E) continue;
         for (int c = threadIdx.x; c < a.n_out; c += kW4Threads)
@@ -223,15 +215,15 @@ expert_linear_w4_kernel(const W4Args a) {
     __syncthreads();
 
     // This CTA's even share of all units.
-    const int64_t total = s_unit[a.E];
-    const int u_begin = int(total * blockIdx.x / gridDim.x), u_end = int(total * (blockIdx.x + 1) / gridDim.x);
+    const int total = s_unit[a.E], share = total / int(gridDim.x), more = total - share * int(gridDim.x);
+    const int u_begin = share * int(blockIdx.x) + min(int(blockIdx.x), more);
+    const int u_end = u_begin + share + (int(blockIdx.x) < more ? 1 : 0);
     if (u_begin >= u_end) return;
 
     const int wk = a.wk, wn_count = kW4Warps / wk, kw = warp % wk, wn = warp / wk;
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     const int my_blocks = blocks > kw ? (blocks - kw + wk - 1) / wk : 0;
     const int ngroups = a.K / G;
-    const int row_bytes = a.K / 2;
 
     // A place in the walk over units: expert, unit of its current pass, pass.
     struct Place {
@@ -266,89 +258,75 @@ expert_linear_w4_kernel(const W4Args a) {
         }
     };
 
-    // ---- weights: a ring of steps per warp, filled ahead by the same walk ----
-    const uint32_t ring = smem_u32(smem) + warp * (kW4Stages * kStep);
-    Place pf = place_at(u_begin);
-    int pf_b = 0, pf_slot = 0;    // block of this warp, ring slot
-    const uint8_t* pf_w = nullptr;  // row g of the tile, this lane's 16 bytes of the block
-    int64_t pf_s = 0;               // index of the scale of row `lane`, this block
-    uint32_t pf_ok = 0;             // bit j: rows 8j .. 8j+7 of the tile exist
-    // Rows 8j + g, j = 0..3, of a tile lie at these distances from row g.
-    const int64_t off1 = 8 * int64_t(row_bytes);
-    const int64_t off2 = a.swiglu ? int64_t(a.n_out) * row_bytes : 16 * int64_t(row_bytes);
-    auto pf_tile = [&]() {
-        const int tile = pf.tg * wn_count + wn;
-        const int n0 = tile * (a.swiglu ? 16 : kW4TileRows);
-        pf_ok = 0;
-        if (tile < a.tiles) {
-            // N (SwiGLU: N/2) is a multiple of 8: eight rows exist together
-            if (a.swiglu) pf_ok = 5u | (n0 + 8 < a.n_out ? 10u : 0u);
-            else pf_ok = 1u | (n0 + 8 < a.N ? 2u : 0u) | (n0 + 16 < a.N ? 4u : 0u) | (n0 + 24 < a.N ? 8u : 0u);
+    // The next step of a warp, fetched while it works on one: its weights by
+    // TMA into the other half of its ring, and the scales and zero points of
+    // tile row `lane` into registers (handed out by shuffles).
+    unsigned char* ring = smem + warp * (kW4Stages * kW4StageBytes);
+    uint32_t sc_raw[kGroups], z_raw[kGroups];
+    auto fetch = [&](const Place& p, int b, int slot) {
+        const int n = (p.tg * wn_count + wn) * (a.swiglu ? 16 : kW4TileRows);
+        if (lane == 0) {  // rows past N and columns past K read as zeros
+            unsigned char* dst = ring + slot * kW4StageBytes;
+            uint64_t* bar = &s_full[warp][slot];
+            mbar_arrive_expect_tx(bar, kW4StageBytes);
+            tma_load_rows(dst, &tmap, b * (kW4Block / 2), n, p.e, bar);
+            tma_load_rows(dst + kW4StageBytes / 2, &tmap, b * (kW4Block / 2), n + (a.swiglu ? a.n_out : 16), p.e, bar);
         }
-        const int64_t row = int64_t(pf.e) * a.N + n0;
-        pf_w = a.wq + (row + g) * row_bytes + kw * (kW4Block / 2) + t * 16;
-        const int lane_row = a.swiglu ? (lane & 15) + (lane >> 4) * a.n_out : lane;
-        pf_s = (row + lane_row) * ngroups + kw * kGroups;
-    };
-    auto issue = [&]() {
-        if (pf.u < u_end && my_blocks > 0) {
-            const uint32_t dst = ring + pf_slot * kStep;
-            const int b = kw + pf_b * wk;
-            const bool k_ok = b * kW4Block + t * 32 < a.K;
-            // 16-byte pieces of row r sit at piece ^ (r / 2 mod 4): word reads are free of bank conflicts
-            const uint32_t d = dst + g * 64 + ((t ^ ((g >> 1) & 3)) << 4);
+        const int r = n + (a.swiglu ? lane & 15 : lane);
+        const bool row_ok = r < a.n_out;
+        const int64_t base = (int64_t(p.e) * a.N + r + (a.swiglu ? (lane >> 4) * a.n_out : 0)) * ngroups + b * kGroups;
+        const uint16_t* sp = static_cast<const uint16_t*>(a.scale) + base;
+        const uint8_t* zp = a.zero + base;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool ok = k_ok && ((pf_ok >> j) & 1);
-                cp_async16(d + j * 512, ok ? pf_w + (j & 1) * off1 + (j >> 1) * off2 : a.wq, ok);
-            }
-            const bool r_ok = (pf_ok >> (lane >> 3)) & 1;
-#pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                const bool ok = r_ok && b * kGroups + q < ngroups;
-                const int64_t at = ok ? pf_s + q : 0;
-                const uint32_t ds = dst + kW4StageBytes + (q * 32 + lane) * 8;
-                cp_async4(ds, static_cast<const uint16_t*>(a.scale) + (at & ~int64_t(1)), ok);
-                if (a.zero) cp_async4(ds + 4, a.zero + (at & ~int64_t(3)), ok);
-            }
-            pf_slot = pf_slot + 1 == kW4Stages ? 0 : pf_slot + 1;
-            if (++pf_b < my_blocks) {
-                pf_w += wk * (kW4Block / 2);
-                pf_s += wk * kGroups;
-            } else {
-                pf_b = 0;
-                advance(pf);
-                if (pf.u < u_end) pf_tile();
-            }
+        for (int q = 0; q < kGroups; ++q) {
+            const bool ok = row_ok && b * kGroups + q < ngroups;
+            sc_raw[q] = ok ? sp[q] : 0u;
+            z_raw[q] = 0u;
+            if (a.zero) z_raw[q] = ok ? zp[q] : 0u;
         }
-        cp_commit();
     };
-    pf_tile();
-#pragma unroll
-    for (int i = 0; i < kW4Stages - 1; ++i) issue();
-
-    const uint32_t sx = smem_u32(smem + a.s_x);
-    float* s_red = reinterpret_cast<float*>(smem + a.s_red);
+    if (lane == 0) {
+        for (int i = 0; i < kW4Stages; ++i) mbar_init(&s_full[warp][i], 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
     Place at = place_at(u_begin);
+    if (my_blocks > 0) fetch(at, kw, 0);
+
+    float* s_red = reinterpret_cast<float*>(smem + a.s_red);
+    int piece[kW4Block / 32];  // where the 16-byte pieces of this lane's rows sit
+#pragma unroll
+    for (int s = 0; s < kW4Block / 32; ++s) piece[s] = (s ^ g) << 4;
     int staged_e = -1, staged_pass = 0, nrows = 0, nt = 0, list0 = 0, slot = 0;
+    uint32_t parity = 0;
     const uint16_t* x_row[NT];
-    for (; at.u < u_end; advance(at)) {
+    while (at.u < u_end) {
+        Place next = at;
+        advance(next);
         if (at.e != staged_e || at.pass != staged_pass) {
             staged_e = at.e, staged_pass = at.pass;
             const int cnt = s_cnt[at.e];
             list0 = s_first[at.e] + at.pass * NT * 8;
             nrows = min(cnt - at.pass * NT * 8, NT * 8);
             nt = (nrows + 7) >> 3;
-            if (XS) {  // zeros past K and past the last row
-                const int chunks = blocks * (kW4Block / 8);
-                for (int r = 0; r < nt * 8; ++r) {
-                    const uint16_t* row =
-                        r < nrows ? static_cast<const uint16_t*>(a.x) + int64_t(s_slots[list0 + r] / a.x_div) * a.K : nullptr;
-                    for (int c = threadIdx.x; c < chunks; c += kW4Threads) {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (row && c * 8 < a.K) v = *reinterpret_cast<const uint4*>(row + c * 8);
-                        *reinterpret_cast<uint4*>(smem + a.s_x + r * a.x_pitch + c * 16) = x_pairs(v);
+            if (XS) {  // zeros past K; columns of the product past the last row are not written
+                const int chunks = blocks * (kW4Block / 8), all = nrows * chunks;
+                for (int c0 = threadIdx.x; c0 < all; c0 += 4 * kW4Threads) {
+                    uint4 v[4];
+                    int r[4], k8[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {  // four loads in flight
+                        const int c = c0 + i * kW4Threads;
+                        r[i] = c / chunks, k8[i] = c - r[i] * chunks;
+                        v[i] = make_uint4(0, 0, 0, 0);
+                        if (c < all && k8[i] * 8 < a.K)
+                            v[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) +
+                                                                   int64_t(s_slots[list0 + r[i]] / a.x_div) * a.K + k8[i] * 8);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c0 + i * kW4Threads < all)
+                            *reinterpret_cast<uint4*>(smem + a.s_x + r[i] * a.x_pitch + k8[i] * 16) = x_pairs(v[i]);
                 }
                 __syncthreads();
             } else {
@@ -359,18 +337,6 @@ expert_linear_w4_kernel(const W4Args a) {
                                                  : nullptr;
             }
         }
-        const int tile = at.tg * wn_count + wn;
-        // Low bits of the scale index of this lane's four rows (group 0): which
-        // half of the 4-byte word holds the scale, which byte the zero point.
-        uint32_t low[2][2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t n = a.swiglu ? uint32_t(tile * 16 + h * 8 + g + m * a.n_out)
-                                            : uint32_t(tile * kW4TileRows + m * 16 + h * 8 + g);
-                low[m][h] = (uint32_t(at.e) * uint32_t(a.N) + n) * uint32_t(ngroups);
-            }
         float acc[2][NT][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -380,15 +346,18 @@ expert_linear_w4_kernel(const W4Args a) {
                 for (int j = 0; j < 4; ++j) acc[m][q][j] = 0.f;
 #pragma unroll 1
         for (int jb = 0; jb < my_blocks; ++jb) {
-            cp_wait<kW4Stages - 2>();
-            __syncwarp();
-            issue();  // into the step read last time
-            const uint32_t st = ring + slot * kStep;
-            slot = slot + 1 == kW4Stages ? 0 : slot + 1;
             const int b = kw + jb * wk;
-            const uint32_t xb = sx + b * (kW4Block * 2) + t * 16 + g * a.x_pitch;
-            const uint32_t swz = (g >> 1) & 3;
-            const uint32_t wb = st + g * 64 + t * 4;
+            // scale in the upper half, zero point in the lower
+            uint32_t sz[kGroups];
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) sz[q] = sc_raw[q] << 16 | z_raw[q];
+            if (jb + 1 < my_blocks) fetch(at, b + wk, slot ^ 1);
+            else if (next.u < u_end) fetch(next, kw, slot ^ 1);
+            if (!mbar_wait(&s_full[warp][slot], parity)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
+            const unsigned char* wb = ring + slot * kW4StageBytes + g * 128 + t * 4;
+            parity ^= uint32_t(slot);
+            slot ^= 1;
+            const unsigned char* xb = smem + a.s_x + b * (kW4Block * 2) + t * 16 + g * a.x_pitch;
 #pragma unroll
             for (int q4 = 0; q4 < kGroups; ++q4) {
                 float sc[2][2];
@@ -397,27 +366,20 @@ expert_linear_w4_kernel(const W4Args a) {
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t d = st + kW4StageBytes + (q4 * 32 + m * 16 + h * 8 + g) * 8;
-                        const uint32_t i = low[m][h] + uint32_t(b * kGroups + q4);
-                        sc[m][h] = w4_from16<DT>((lds32(d) >> ((i & 1) * 16)) & 0xffffu);
-                        const uint32_t z = a.zero ? (lds32(d + 4) >> ((i & 3) * 8)) & 0xffu : 8u;
-                        z2[m][h] = z * 0x00010001u | magic<DT>();
+                        const uint32_t v = __shfl_sync(0xffffffffu, sz[q4], m * 16 + h * 8 + g);
+                        sc[m][h] = DT == MOE_B200_BF16 ? __uint_as_float(v & 0xffff0000u) : w4_from16<DT>(v >> 16);
+                        z2[m][h] = magic<DT>() + 8 * 0x00010001u;
+                        if (a.zero) z2[m][h] = (v & 0xffu) * 0x00010001u + magic<DT>();
                     }
                 float d4[2][NT][4];
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int q = 0; q < NT; ++q)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) d4[m][q][j] = 0.f;
-#pragma unroll
                 for (int s4 = 0; s4 < G / 32; ++s4) {
-                    const int s = q4 * (G / 32) + s4;  // 32 k of the block
+                    const int s = q4 * (G / 32) + s4;  // 32 k of the step
                     uint4 xv[NT];
 #pragma unroll
                     for (int q = 0; q < NT; ++q)
                         if (XS) {
-                            if (q < nt) xv[q] = lds128(xb + q * 8 * a.x_pitch + s * 64);
+                            if (q == 0 || q < nt) xv[q] = *reinterpret_cast<const uint4*>(xb + q * 8 * a.x_pitch + s * 64);
                         } else {
                             const int k = b * kW4Block + s * 32;
                             xv[q] = make_uint4(0, 0, 0, 0);
@@ -426,14 +388,16 @@ expert_linear_w4_kernel(const W4Args a) {
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         uint32_t lo[4], hi[4];
-                        const uint32_t wa = wb + m * 1024 + ((uint32_t(s) ^ swz) << 4);
-                        unpack8<DT>(lds32(wa), z2[m][0], lo);
-                        unpack8<DT>(lds32(wa + 512), z2[m][1], hi);
+                        // 16-byte piece s of row r sits at piece s ^ (r mod 8); r mod 8 = g
+                        const unsigned char* wa = wb + (m * 2048 + piece[s]);
+                        unpack8<DT>(*reinterpret_cast<const uint32_t*>(wa), z2[m][0], lo);
+                        unpack8<DT>(*reinterpret_cast<const uint32_t*>(wa + 1024), z2[m][1], hi);
 #pragma unroll
                         for (int q = 0; q < NT; ++q)
-                            if (q < nt) {
-                                mma_16816<DT>(d4[m][q], lo[0], hi[0], lo[1], hi[1], xv[q].x, xv[q].y);
-                                mma_16816<DT>(d4[m][q], lo[2], hi[2], lo[3], hi[3], xv[q].z, xv[q].w);
+                            if (q == 0 || q < nt) {
+                                if (s4 == 0) mma_16816<DT, true>(d4[m][q], lo[0], hi[0], lo[1], hi[1], xv[q].x, xv[q].y);
+                                else mma_16816<DT, false>(d4[m][q], lo[0], hi[0], lo[1], hi[1], xv[q].x, xv[q].y);
+                                mma_16816<DT, false>(d4[m][q], lo[2], hi[2], lo[3], hi[3], xv[q].z, xv[q].w);
                             }
                     }
                 }
@@ -441,8 +405,10 @@ expert_linear_w4_kernel(const W4Args a) {
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int q = 0; q < NT; ++q)
+                        if (q == 0 || q < nt) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[m][q][j] += sc[m][j >> 1] * d4[m][q][j];
+                            for (int j = 0; j < 4; ++j) acc[m][q][j] += sc[m][j >> 1] * d4[m][q][j];
+                        }
             }
             __syncwarp();  // the step is read before its refill
         }
@@ -469,7 +435,7 @@ expert_linear_w4_kernel(const W4Args a) {
             uint16_t* out = static_cast<uint16_t*>(a.out) + int64_t(s_slots[list0 + col]) * a.n_out;
             if (a.swiglu) {
                 const int n = tl * 16 + rr;
-                if (n < a.n_out) out[n] = w4_to16<DT>(v[0] / (1.0f + __expf(-v[0])) * v[1]);
+                if (n < a.n_out) out[n] = w4_to16<DT>(__fdividef(v[0], 1.0f + __expf(-v[0])) * v[1]);
             } else {
                 const int n = tl * kW4TileRows + rr;
                 if (n < a.N) out[n] = w4_to16<DT>(v[0]);
@@ -477,8 +443,8 @@ expert_linear_w4_kernel(const W4Args a) {
             }
         }
         __syncthreads();
+        at = next;
     }
-    cp_wait<0>();
 }
 
 // ----------------------------------------------------------------- host ----
@@ -490,11 +456,10 @@ static int sm_count_w4() {
 }
 
 // Shared memory of a CTA and its layout; xs: with x staged.
-template <int G>
 static size_t w4_layout(W4Args& a, int nt, bool xs) {
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     a.x_pitch = blocks * kW4Block * 2 + 64;  // 64 bytes off a multiple of 128: rows of a fragment on other banks
-    size_t off = size_t(kW4Warps) * kW4Stages * w4_step_bytes<G>();
+    size_t off = size_t(kW4Warps) * kW4Stages * kW4StageBytes;
     a.s_x = int(off);
     off += xs ? size_t(nt) * 8 * a.x_pitch : 0;
     a.s_red = int(off);
@@ -505,33 +470,49 @@ static size_t w4_layout(W4Args& a, int nt, bool xs) {
 }
 
 template <int DT, int G, int NT, bool XS>
-static cudaError_t launch_w4(W4Args a, dim3 grid, cudaStream_t s) {
-    const size_t smem = w4_layout<G>(a, NT, XS);
+static cudaError_t launch_w4(const CUtensorMap& map, W4Args a, dim3 grid, cudaStream_t s) {
+    const size_t smem = w4_layout(a, NT, XS);
     auto kern = expert_linear_w4_kernel<DT, G, NT, XS>;
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (err != cudaSuccess) return err;
-    kern<<<grid, kW4Threads, smem, s>>>(a);
+    kern<<<grid, kW4Threads, smem, s>>>(map, a);
     return cudaGetLastError();
 }
 
 template <int DT, int G>
-static cudaError_t run_w4(W4Args a, cudaStream_t s) {
+static cudaError_t run_w4(const CUtensorMap& map, W4Args a, cudaStream_t s) {
     const int served = a.slots < a.E ? a.slots : a.E;  // experts that may have work
-    // Warps that share a tile's k: as many as lose less than an eighth of their
-    // steps to an uneven split.
+    int64_t grid = 2 * sm_count_w4();
+    // Warps that share a tile's k: few, as each joint costs about as much as a
+    // step, but so that every CTA gets several units, and none that loses more
+    // than an eighth of its steps to an uneven split.
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     a.wk = kW4Warps;
-    while (a.wk > 1 && 8 * blocks < 7 * a.wk * ((blocks + a.wk - 1) / a.wk)) a.wk /= 2;
+    while (a.wk > 1 && (8 * blocks < 7 * a.wk * ((blocks + a.wk - 1) / a.wk) ||
+                        int64_t(a.tiles) * served * a.wk > 2 * kW4Warps * 8 * grid))
+        a.wk /= 2;
     a.units = (a.tiles + kW4Warps / a.wk - 1) / (kW4Warps / a.wk);
     // Rows served per read of the weights: 8, or 16 when experts have more than that on average.
-    const bool two = a.slots > 8 * served && w4_layout<G>(a, 2, true) <= kW4SmemLimit;
-    const bool staged = two || w4_layout<G>(a, 1, true) <= kW4SmemLimit;
+    const bool two = a.slots > 8 * served && w4_layout(a, 2, true) <= kW4SmemLimit;
+    const bool staged = two || w4_layout(a, 1, true) <= kW4SmemLimit;
     const int64_t most = int64_t(a.units) * (a.slots < a.E ? a.slots : a.E + a.slots / 8);
-    int64_t grid = 2 * sm_count_w4();
     if (grid > most) grid = most;
-    if (two) return launch_w4<DT, G, 2, true>(a, dim3(unsigned(grid)), s);
-    return staged ? launch_w4<DT, G, 1, true>(a, dim3(unsigned(grid)), s)
-                  : launch_w4<DT, G, 1, false>(a, dim3(unsigned(grid)), s);
+    if (two) return launch_w4<DT, G, 2, true>(map, a, dim3(unsigned(grid)), s);
+    return staged ? launch_w4<DT, G, 1, true>(map, a, dim3(unsigned(grid)), s)
+                  : launch_w4<DT, G, 1, false>(map, a, dim3(unsigned(grid)), s);
+}
+
+// 3-D map over w_q [E, N, d/2] bytes; box = 128 bytes x 16 rows of one expert, 128B swizzle.
+static bool make_map_w4(CUtensorMap* map, const void* base, int E, int N, int K) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {cuuint64_t(K / 2), cuuint64_t(N), cuuint64_t(E)};
+    cuuint64_t strides[2] = {cuuint64_t(K / 2), cuuint64_t(K / 2) * cuuint64_t(N)};
+    cuuint32_t box[3] = {128u, 16u, 1u};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace moe_b200
@@ -567,7 +548,6 @@ extern "C" int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const in
     W4Args a{};
     a.x = x;
     a.asgn = asgn;
-    a.wq = static_cast<const uint8_t*>(w_q);
     a.scale = w_scale;
     a.zero = static_cast<const uint8_t*>(w_zero);
     a.out = out;
@@ -581,10 +561,12 @@ extern "C" int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const in
     a.n_out = a.swiglu ? N / 2 : N;
     a.tiles = a.swiglu ? (a.n_out + 15) / 16 : (N + kW4TileRows - 1) / kW4TileRows;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    CUtensorMap map;
+    if (!make_map_w4(&map, w_q, E, N, d)) return fail(MOE_B200_ERR_CUDA, "expert_linear_w4: cuTensorMapEncodeTiled failed");
     const bool bf = dtype == MOE_B200_BF16;
     cudaError_t err;
-    if (group == 32) err = bf ? run_w4<MOE_B200_BF16, 32>(a, s) : run_w4<MOE_B200_F16, 32>(a, s);
-    else if (group == 64) err = bf ? run_w4<MOE_B200_BF16, 64>(a, s) : run_w4<MOE_B200_F16, 64>(a, s);
-    else err = bf ? run_w4<MOE_B200_BF16, 128>(a, s) : run_w4<MOE_B200_F16, 128>(a, s);
+    if (group == 32) err = bf ? run_w4<MOE_B200_BF16, 32>(map, a, s) : run_w4<MOE_B200_F16, 32>(map, a, s);
+    else if (group == 64) err = bf ? run_w4<MOE_B200_BF16, 64>(map, a, s) : run_w4<MOE_B200_F16, 64>(map, a, s);
+    else err = bf ? run_w4<MOE_B200_BF16, 128>(map, a, s) : run_w4<MOE_B200_F16, 128>(map, a, s);
     return err == cudaSuccess ? MOE_B200_OK : cuda_fail(err, "expert_linear_w4 launch");
 }
