@@ -43,6 +43,16 @@ template <int DT> __device__ __forceinline__ uint16_t to16(float f) {
     return DT == MOE_B200_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
 }
 
+// Two fp32 values to a word of two 16-bit ones.
+template <int DT> __device__ __forceinline__ uint32_t pack16(float a, float b) {
+    if (DT == MOE_B200_BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // A row's columns as a thread holds them: V chunks of 8.  Aligned rows
 // (ALIGNED: d, strides and pointers in 16-byte steps) give a thread 8
 // consecutive columns per chunk, one 16-byte access (two for fp32); other rows
@@ -53,8 +63,12 @@ __device__ __forceinline__ int col_of(int chunk, int j, int t, int nt) {
 }
 
 // Eight columns of a chunk as raw words: 16-bit rows use w[0..3] (two columns
-// a word), fp32 rows w[0..7].  Columns past d read as zero, which adds nothing
-// to any sum.
+// a word), fp32 rows w[0..7].  Aligned rows end with a chunk, and the caller
+// asks chunk_in() once per chunk; of other rows, columns past d read as zero,
+// which adds nothing to any sum.
+template <bool ALIGNED> __device__ __forceinline__ bool chunk_in(int chunk, int t, int nt, int d) {
+    return !ALIGNED || (chunk * nt + t) * 8 < d;
+}
 template <bool F32> struct Raw {
     uint32_t w[F32 ? 8 : 4];
 };
@@ -63,17 +77,12 @@ template <bool ALIGNED, bool F32>
 __device__ __forceinline__ Raw<F32> load_raw(const void* row, int chunk, int t, int nt, int d) {
     Raw<F32> r;
     if (ALIGNED) {
-        const int c = col_of<true>(chunk, 0, t, nt);
-        if (c < d) {
-            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + size_t(c) * (F32 ? 4 : 2));
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) +
+                                                        col_of<true>(chunk, 0, t, nt) * (F32 ? 4 : 2));
 #pragma unroll
-            for (int h = 0; h < (F32 ? 2 : 1); ++h) {
-                const uint4 v = p[h];
-                r.w[4 * h] = v.x, r.w[4 * h + 1] = v.y, r.w[4 * h + 2] = v.z, r.w[4 * h + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < (F32 ? 8 : 4); ++j) r.w[j] = 0;
+        for (int h = 0; h < (F32 ? 2 : 1); ++h) {
+            const uint4 v = p[h];
+            r.w[4 * h] = v.x, r.w[4 * h + 1] = v.y, r.w[4 * h + 2] = v.z, r.w[4 * h + 3] = v.w;
         }
     } else {
 #pragma unroll
@@ -101,9 +110,7 @@ __device__ __forceinline__ float raw_get(const Raw<F32>& r, int j) {
 template <int DT, bool ALIGNED, bool F32>
 __device__ __forceinline__ void store8(void* row, const float (&x)[8], int chunk, int t, int nt, int d) {
     if (ALIGNED) {
-        const int c = col_of<true>(chunk, 0, t, nt);
-        if (c >= d) return;
-        uint4* p = reinterpret_cast<uint4*>(static_cast<char*>(row) + size_t(c) * (F32 ? 4 : 2));
+        uint4* p = reinterpret_cast<uint4*>(static_cast<char*>(row) + col_of<true>(chunk, 0, t, nt) * (F32 ? 4 : 2));
         if (F32) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -112,8 +119,7 @@ __device__ __forceinline__ void store8(void* row, const float (&x)[8], int chunk
         } else {
             uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                o[j] = uint32_t(to16<DT>(x[2 * j])) | (uint32_t(to16<DT>(x[2 * j + 1])) << 16);
+            for (int j = 0; j < 4; ++j) o[j] = pack16<DT>(x[2 * j], x[2 * j + 1]);
             st_v4(p, make_uint4(o[0], o[1], o[2], o[3]));
         }
     } else {
@@ -128,11 +134,13 @@ __device__ __forceinline__ void store8(void* row, const float (&x)[8], int chunk
     }
 }
 
-// Sums of N values over a row's threads: a warp (WARP) or the whole CTA, the
-// same bits in every thread.  `red` holds two buffers of 4 floats a warp;
-// `phase` alternates them, so one barrier a reduction is enough: a buffer is
-// written again only after the next reduction's barrier, which no thread
-// passes before it has read this one.
+// Sums of N <= 4 values over a row's threads: a warp (WARP) or the whole CTA,
+// the same bits in every thread.  `red` holds two buffers of [N][warps] floats
+// (the number of warps rounded up to 4, the rest zeros); `phase` alternates
+// them, so one barrier a reduction is enough: a buffer is written again only
+// after the next reduction's barrier, which no thread passes before it has
+// read this one.
+constexpr int kRedFloats = 2 * 4 * 32;
 template <bool WARP, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
 #pragma unroll
@@ -140,20 +148,29 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     if (WARP) return;
-    const int nw = blockDim.x >> 5;
-    float* b = red + (phase & 1) * (nw * 4);
-    ++phase;
+    const int nw = ((blockDim.x >> 5) + 3) & ~3;
+    float* b = red + phase * (4 * 32);
+    phase ^= 1;
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) b[(threadIdx.x >> 5) * 4 + i] = v[i];
+        for (int i = 0; i < N; ++i) b[i * 32 + (threadIdx.x >> 5)] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
-    for (int w = 0; w < nw; ++w) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += b[w * 4 + i];
+    for (int i = 0; i < N; ++i) {
+        float4 s = *reinterpret_cast<const float4*>(b + i * 32);
+        for (int w = 4; w < nw; w += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(b + i * 32 + w);
+            s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+        }
+        v[i] = (s.x + s.y) + (s.z + s.w);
     }
+}
+// Zeros for the places of warps that do not exist; before the first row_sum.
+template <bool WARP> __device__ __forceinline__ void row_sum_init(float* red) {
+    if (WARP) return;
+    for (int i = threadIdx.x; i < kRedFloats; i += blockDim.x) red[i] = 0.f;
+    __syncthreads();
 }
 
 struct NormArgs {
@@ -165,92 +182,124 @@ struct NormArgs {
     void *residual_out, *normed;
 };
 
+// What a call consists of, where it is known when compiling (the forms that
+// models run all the time); kFormAny asks the arguments.  A column gate is one
+// per channel or per element: its rows lie 0 or d apart.
+enum { kFormAny = 0, kFormFull = 1, kFormFullColGate = 2, kFormAddNorm = 3, kFormNorm = 4 };
+template <int FORM> struct Form {
+    static constexpr bool any = FORM == kFormAny;
+    static constexpr bool y = FORM != kFormNorm, post = FORM == kFormFull || FORM == kFormFullColGate;
+    static constexpr bool col = FORM == kFormFullColGate;
+};
+
 // A row belongs to one warp (WARP: CTAs of 4 rows) or to a CTA; each thread
 // holds V chunks of 8 columns.  The grid fits the card and walks the rows; the
 // weights stay packed in registers and the next row's loads are in flight
 // while a row is reduced and written.
-template <int DT, bool RES32, bool ALIGNED, bool WARP, int V, int MAXT>
-__global__ void __launch_bounds__(MAXT)
+template <int DT, bool RES32, bool ALIGNED, bool WARP, int V, int MAXT, int FORM>
+__global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 768 / MAXT : 1)  // 80 registers: 24 warps an SM
 block_norm_kernel(const NormArgs a) {
-    __shared__ float s_red[2 * 4 * 32];
+    using F = Form<FORM>;
+    __shared__ __align__(16) float s_red[kRedFloats];
+    const bool has_y = F::any ? a.y != nullptr : F::y, has_post = F::any ? a.w_post != nullptr : F::post;
+    const bool has_col = F::any ? a.gate_form >= kGateChannel : F::col, has_pre = F::any ? a.w_pre != nullptr : true;
     const int nt = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
     const int rows_per_cta = WARP ? blockDim.x >> 5 : 1;
     const int64_t step = int64_t(gridDim.x) * rows_per_cta;
     int64_t row = int64_t(blockIdx.x) * rows_per_cta + (WARP ? threadIdx.x >> 5 : 0);
     if (row >= a.T) return;
+    row_sum_init<WARP>(s_red);
     int phase = 0;
     const int d = a.d;
     const float inv_d = 1.0f / float(d);
-    Raw<false> wp[V], gc[V], wn[V], yr[V], gr[V];
+    constexpr int kRes = RES32 ? 4 : 2;
+    const int64_t gate_stride = a.gate_form == kGateFull ? d : 0;
+    Raw<false> wp[V], wn[V], yr[V], gr[V];
     Raw<RES32> res[V];
-    auto fetch = [&](int64_t r) {
-        const char* res_row = static_cast<const char*>(a.residual) + r * a.res_stride * (RES32 ? 4 : 2);
-        const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + r * a.y_stride;
+    // Next row to load, and this row's results.
+    const char* res_row = static_cast<const char*>(a.residual) + row * a.res_stride * kRes;
+    const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + row * a.y_stride;
+    const uint16_t* g_row = static_cast<const uint16_t*>(a.gate) + row * gate_stride;
+    char* res_out = static_cast<char*>(a.residual_out) + row * d * kRes;
+    uint16_t* norm_out = static_cast<uint16_t*>(a.normed) + row * d;
+    auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+            if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
             res[i] = load_raw<ALIGNED, RES32>(res_row, i, t, nt, d);
-            if (a.y) yr[i] = load_raw<ALIGNED, false>(y_row, i, t, nt, d);
-            if (a.gate_form == kGateFull)
-                gr[i] = load_raw<ALIGNED, false>(static_cast<const uint16_t*>(a.gate) + r * d, i, t, nt, d);
+            if (has_y) yr[i] = load_raw<ALIGNED, false>(y_row, i, t, nt, d);
+            if (has_col) gr[i] = load_raw<ALIGNED, false>(g_row, i, t, nt, d);
         }
+        res_row += step * a.res_stride * kRes;
+        if (has_y) y_row += step * a.y_stride;
+        if (has_col) g_row += step * gate_stride;
     };
-    fetch(row);
+    fetch();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (a.gate_form == kGateChannel) gc[i] = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
-        if (a.w_post) wp[i] = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
-        if (a.w_pre) wn[i] = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
+        if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
+        if (has_post) wp[i] = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
+        if (has_pre) wn[i] = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
     }
     for (; row < a.T; row += step) {
-        float r[V][8], y[V][8];
+        float r[V][8], z[V][8];
         float s[1] = {0.f};
+        float f = a.scale;
+        if (has_y && !has_col && a.gate_form == kGateToken) f *= from16<DT>(static_cast<const uint16_t*>(a.gate)[row]);
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+        for (int i = 0; i < V; ++i) {
+            if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                r[i][j] = raw_get<DT, RES32>(res[i], j);
-                if (a.y) {
-                    y[i][j] = raw_get<DT, false>(yr[i], j);
-                    s[0] += y[i][j] * y[i][j];
-                    if (a.gate_form == kGateChannel) y[i][j] *= raw_get<DT, false>(gc[i], j);
-                    if (a.gate_form == kGateFull) y[i][j] *= raw_get<DT, false>(gr[i], j);
+            for (int j = 0; j < 8; ++j) r[i][j] = raw_get<DT, RES32>(res[i], j);
+            if (has_y) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[i][j] = raw_get<DT, false>(yr[i], j);
+                if (has_post) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        s[0] += z[i][j] * z[i][j];
+                        z[i][j] *= raw_get<DT, false>(wp[i], j);
+                    }
+                }
+                if (has_col) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[i][j] *= raw_get<DT, false>(gr[i], j);
                 }
             }
-        float f = a.scale;
-        if (a.gate_form == kGateToken) f *= from16<DT>(static_cast<const uint16_t*>(a.gate)[row]);
-        if (row + step < a.T) fetch(row + step);
-        if (a.y) {
-            if (a.w_post) {
+        }
+        if (row + step < a.T) fetch();
+        if (has_y) {
+            if (has_post) {
                 row_sum<WARP>(s, s_red, phase);
                 f *= rsqrtf(s[0] * inv_d + a.eps);
             }
-            char* out = static_cast<char*>(a.residual_out) + row * d * (RES32 ? 4 : 2);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float z = y[i][j] * f;
-                    if (a.w_post) z *= raw_get<DT, false>(wp[i], j);
-                    r[i][j] += z;
-                }
-                store8<DT, ALIGNED, RES32>(out, r[i], i, t, nt, d);
+                for (int j = 0; j < 8; ++j) r[i][j] += z[i][j] * f;
+                store8<DT, ALIGNED, RES32>(res_out, r[i], i, t, nt, d);
             }
+            res_out += step * d * kRes;
         }
-        if (a.w_pre) {
+        if (has_pre) {
             s[0] = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
+            for (int i = 0; i < V; ++i) {
+                if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s[0] += r[i][j] * r[i][j];
+            }
             row_sum<WARP>(s, s_red, phase);
             const float c = rsqrtf(s[0] * inv_d + a.eps);
-            uint16_t* out = static_cast<uint16_t*>(a.normed) + row * d;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[i][j] *= c * raw_get<DT, false>(wn[i], j);
-                store8<DT, ALIGNED, false>(out, r[i], i, t, nt, d);
+                store8<DT, ALIGNED, false>(norm_out, r[i], i, t, nt, d);
             }
+            norm_out += step * d;
         }
     }
 }
@@ -268,23 +317,31 @@ struct NormGradArgs {
     // Ring of rows in shared memory (RING): bytes of a staged row and where its
     // parts lie in it (-1: absent).
     int row_bytes, off_ds, off_rr, off_dn, off_y, off_gate;
+    int stages, off_w;  // rows in flight; the weights' copies (w_pre, w_post, channel gate) behind the ring
     uint32_t* status;
 };
 
-constexpr int kNormStages = 3;
+constexpr int kNormStages = 4;  // at most
 
 // Rows are dealt to a grid that fits the card, so that each thread keeps its
 // columns' sums over its rows in registers and the column gradients cost one
 // row of partial sums a CTA.  RING: the rows come through a ring of shared-
-// memory stages filled by bulk copies kNormStages rows ahead, which costs no
-// registers; otherwise (rows not in 16-byte steps, or too wide for the ring)
+// memory stages filled by bulk copies some rows ahead, which costs no registers,
+// and the weights are copied there once; otherwise (rows not in 16-byte steps, or too wide for the ring)
 // they are read from global memory at each of the two uses.
-template <int DT, bool RES32, bool ALIGNED, bool RING, bool WARP, int V, int MAXT>
+// GATE: the gate's form, or -1 where the call is of a rarer kind (a norm or
+// the residual's gradient missing) and the arguments are asked.
+template <int DT, bool RES32, bool ALIGNED, bool RING, bool WARP, int V, int MAXT, int GATE>
 __global__ void __launch_bounds__(MAXT)
 block_norm_backward_kernel(const NormGradArgs a) {
     extern __shared__ __align__(128) unsigned char s_dyn[];
-    __shared__ float s_red[2 * 4 * 32];
+    __shared__ __align__(16) float s_red[kRedFloats];
     __shared__ uint64_t s_full[4 * kNormStages], s_empty[4 * kNormStages];
+    constexpr bool kAny = GATE < 0;
+    const bool has_y = kAny ? a.y != nullptr : true, has_post = kAny ? a.w_post != nullptr : true;
+    const bool has_pre = kAny ? a.w_pre != nullptr : true, has_ds = kAny ? a.d_res_out != nullptr : true;
+    const int gate_form = kAny ? a.gate_form : GATE;
+    const bool has_col = gate_form >= kGateChannel;
     const int nt = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
     const int groups = WARP ? blockDim.x >> 5 : 1, group = WARP ? threadIdx.x >> 5 : 0;
     const int64_t step = int64_t(gridDim.x) * groups;
@@ -294,7 +351,8 @@ block_norm_backward_kernel(const NormGradArgs a) {
     const float inv_d = 1.0f / float(d);
     constexpr int kRes = RES32 ? 4 : 2;
     uint64_t *full = s_full + group * kNormStages, *empty = s_empty + group * kNormStages;
-    unsigned char* ring = s_dyn + size_t(group) * kNormStages * a.row_bytes;
+    unsigned char* ring = s_dyn + size_t(group) * a.stages * a.row_bytes;
+    unsigned char *s_wpre = s_dyn + a.off_w, *s_wpost = s_wpre + (has_pre ? d * 2 : 0), *s_wgate = s_wpost + (has_post ? d * 2 : 0);
 
     auto ds_row = [&](int64_t r) { return static_cast<const char*>(a.d_res_out) + r * d * kRes; };
     auto rr_row = [&](int64_t r) { return static_cast<const char*>(a.res_out) + r * a.res_stride * kRes; };
@@ -304,45 +362,57 @@ block_norm_backward_kernel(const NormGradArgs a) {
     auto fill = [&](int64_t r, int s) {  // one thread
         unsigned char* p = ring + size_t(s) * a.row_bytes;
         mbar_arrive_expect_tx(full + s, a.row_bytes);
-        if (a.off_ds >= 0) bulk_g2s(p + a.off_ds, ds_row(r), d * kRes, full + s);
-        if (a.off_rr >= 0) bulk_g2s(p + a.off_rr, rr_row(r), d * kRes, full + s);
-        if (a.off_dn >= 0) bulk_g2s(p + a.off_dn, dn_row(r), d * 2, full + s);
-        if (a.off_y >= 0) bulk_g2s(p + a.off_y, y_row(r), d * 2, full + s);
-        if (a.off_gate >= 0) bulk_g2s(p + a.off_gate, g_row(r), d * 2, full + s);
+        if (has_ds) bulk_g2s(p + a.off_ds, ds_row(r), d * kRes, full + s);
+        if (has_pre) bulk_g2s(p + a.off_rr, rr_row(r), d * kRes, full + s);
+        if (has_pre) bulk_g2s(p + a.off_dn, dn_row(r), d * 2, full + s);
+        if (has_y) bulk_g2s(p + a.off_y, y_row(r), d * 2, full + s);
+        if (gate_form == kGateFull) bulk_g2s(p + a.off_gate, g_row(r), d * 2, full + s);
     };
+    row_sum_init<WARP>(s_red);
     if (RING) {
         if (t == 0) {
-            for (int s = 0; s < kNormStages; ++s) {
+            for (int s = 0; s < a.stages; ++s) {
                 mbar_init(full + s, 1);
                 mbar_init(empty + s, nt >> 5);
             }
             mbar_fence_init();
         }
+        for (int c = threadIdx.x * 8; c < d; c += blockDim.x * 8) {
+            if (has_pre) *reinterpret_cast<uint4*>(s_wpre + c * 2) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.w_pre) + c);
+            if (has_post) *reinterpret_cast<uint4*>(s_wpost + c * 2) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.w_post) + c);
+            if (gate_form == kGateChannel) *reinterpret_cast<uint4*>(s_wgate + c * 2) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.gate) + c);
+        }
         __syncthreads();
         if (t == 0)
-            for (int s = 0; s < kNormStages; ++s)
+            for (int s = 0; s < a.stages; ++s)
                 if (row0 + s * step < a.T) fill(row0 + s * step, s);
     }
 
-    float s_pre[V][8], s_post[V][8], s_gate[V][8];
+    // Column sums.  A channel gate and w_post share one: with A = sum ds yh,
+    // d_w_post = scale * gate * A and d_gate = scale * w_post * A.
+    float s_pre[V][8], s_post[V][8];
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s_pre[i][j] = s_post[i][j] = s_gate[i][j] = 0.f;
+        for (int j = 0; j < 8; ++j) s_pre[i][j] = s_post[i][j] = 0.f;
 
     uint32_t n = 0;
+    int st = 0;         // ring stage and its phase
+    uint32_t ph = 0;
+    char* dres_out = static_cast<char*>(a.d_res) + row0 * d * kRes;
+    uint16_t* dy_out = static_cast<uint16_t*>(a.d_y) + row0 * d;
+    uint16_t* dg_out = static_cast<uint16_t*>(a.d_gate) + row0 * d;
     for (int64_t row = row0; row < a.T; row += step, ++n) {
-        const int st = int(n % kNormStages);
-        const unsigned char* p = ring + size_t(st) * a.row_bytes;
+        const unsigned char* p = ring + st * a.row_bytes;
         if (RING) {
             // Refill the stage of the row before, once all its warps are through with it.
-            const int64_t ahead = row + (kNormStages - 1) * step;
+            const int64_t ahead = row + (a.stages - 1) * step;
             if (t == 0 && n > 0 && ahead < a.T) {
-                const int prev = int((n - 1) % kNormStages);
-                if (!mbar_wait(empty + prev, ((n - 1) / kNormStages) & 1u)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
+                const int prev = st == 0 ? a.stages - 1 : st - 1;
+                if (!mbar_wait(empty + prev, st == 0 ? ph ^ 1u : ph)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
                 fill(ahead, prev);
             }
-            if (!mbar_wait(full + st, (n / kNormStages) & 1u)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
+            if (!mbar_wait(full + st, ph)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
         }
         auto get16 = [&](int off, const char* g, int i) {
             return RING ? load_raw<ALIGNED, false>(p + off, i, t, nt, d) : load_raw<ALIGNED, false>(g, i, t, nt, d);
@@ -350,11 +420,15 @@ block_norm_backward_kernel(const NormGradArgs a) {
         auto getres = [&](int off, const char* g, int i) {
             return RING ? load_raw<ALIGNED, RES32>(p + off, i, t, nt, d) : load_raw<ALIGNED, RES32>(g, i, t, nt, d);
         };
+        auto getw = [&](const unsigned char* s, const void* g, int i) {
+            return RING ? load_raw<ALIGNED, false>(s, i, t, nt, d) : load_raw<ALIGNED, false>(g, i, t, nt, d);
+        };
         float sums[3] = {0.f, 0.f, 0.f};  // sum r'^2, sum u r', sum y^2
-        if (a.w_pre) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const Raw<false> wn = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
+        for (int i = 0; i < V; ++i) {
+            if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
+            if (has_pre) {
+                const Raw<false> wn = getw(s_wpre, a.w_pre, i);
                 const Raw<false> dn = get16(a.off_dn, dn_row(row), i);
                 const Raw<RES32> rr = getres(a.off_rr, rr_row(row), i);
 #pragma unroll
@@ -364,10 +438,7 @@ block_norm_backward_kernel(const NormGradArgs a) {
                     sums[1] += raw_get<DT, false>(dn, j) * raw_get<DT, false>(wn, j) * r;
                 }
             }
-        }
-        if (a.w_post) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
+            if (has_post) {
                 const Raw<false> yr = get16(a.off_y, y_row(row), i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -376,94 +447,112 @@ block_norm_backward_kernel(const NormGradArgs a) {
                 }
             }
         }
-        if (a.w_pre || a.w_post) row_sum<WARP>(sums, s_red, phase);
+        if (has_pre || has_post) row_sum<WARP>(sums, s_red, phase);
         const float c = rsqrtf(sums[0] * inv_d + a.eps);
-        const float k = sums[1] * inv_d * c * c;
-        const float post = a.w_post ? rsqrtf(sums[2] * inv_d + a.eps) : 1.0f;
-        char* dres_out = static_cast<char*>(a.d_res) + row * d * kRes;
-        float f = a.scale;
-        if (a.gate_form == kGateToken) f *= from16<DT>(static_cast<const uint16_t*>(a.gate)[row]);
-        float sums2[2] = {0.f, 0.f};  // sum v yh, sum ds z (gate per token)
+        const float k = sums[1] * inv_d * c * c;  // ds = dr' + c dn w_pre - (c r') k
+        const float post = has_post ? rsqrtf(sums[2] * inv_d + a.eps) : 1.0f;
+        const float gate_t =
+            gate_form == kGateToken ? from16<DT>(static_cast<const uint16_t*>(a.gate)[row]) : 1.0f;
+        // q is first ds, then ds * (column gate) * w_post, without the row's scale f
+        const float f = a.scale * gate_t;
+        float sum2[1] = {0.f};  // sum q yh
         float q[V][8];
         Raw<false> yr[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            Raw<RES32> ds, rr;
-            Raw<false> wn, dn, wp, gr;
-            if (a.d_res_out) ds = getres(a.off_ds, ds_row(row), i);
-            if (a.w_pre) {
-                wn = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
-                dn = get16(a.off_dn, dn_row(row), i);
-                rr = getres(a.off_rr, rr_row(row), i);
-            }
-            if (a.y) yr[i] = get16(a.off_y, y_row(row), i);
-            if (a.w_post) wp = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
-            if (a.gate_form == kGateFull) gr = get16(a.off_gate, g_row(row), i);
-            if (a.gate_form == kGateChannel) gr = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
+            if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
+            if (has_ds) {
+                const Raw<RES32> ds = getres(a.off_ds, ds_row(row), i);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float g = a.d_res_out ? raw_get<DT, RES32>(ds, j) : 0.f;
-                if (a.w_pre) {
-                    const float r = raw_get<DT, RES32>(rr, j), dnj = raw_get<DT, false>(dn, j);
-                    g += c * (dnj * raw_get<DT, false>(wn, j) - r * k);
-                    s_pre[i][j] += dnj * (r * c);
-                }
-                q[i][j] = g;
+                for (int j = 0; j < 8; ++j) q[i][j] = raw_get<DT, RES32>(ds, j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[i][j] = 0.f;
             }
-            store8<DT, ALIGNED, RES32>(dres_out, q[i], i, t, nt, d);
-            if (a.y) {
-                float dg[8];
+            if (has_pre) {
+                const Raw<false> wn = getw(s_wpre, a.w_pre, i);
+                const Raw<false> dn = get16(a.off_dn, dn_row(row), i);
+                const Raw<RES32> rr = getres(a.off_rr, rr_row(row), i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float yh = raw_get<DT, false>(yr[i], j) * post;
-                    const float w = a.w_post ? raw_get<DT, false>(wp, j) : 1.0f;
-                    const float g = q[i][j];
-                    dg[j] = a.scale * g * (yh * w);
-                    float v = g * f;
-                    if (a.gate_form >= kGateChannel) v *= raw_get<DT, false>(gr, j);
-                    if (a.w_post) {
-                        s_post[i][j] += v * yh;
-                        v *= w;
-                        sums2[0] += v * yh;
-                    }
-                    q[i][j] = v;
-                    if (a.gate_form == kGateToken) sums2[1] += dg[j];
-                    if (a.gate_form == kGateChannel) s_gate[i][j] += dg[j];
+                    const float rc = raw_get<DT, RES32>(rr, j) * c, dnj = raw_get<DT, false>(dn, j);
+                    s_pre[i][j] += dnj * rc;
+                    q[i][j] += c * (dnj * raw_get<DT, false>(wn, j)) - rc * k;
                 }
-                if (a.gate_form == kGateFull)
-                    store8<DT, ALIGNED, false>(static_cast<uint16_t*>(a.d_gate) + row * d, dg, i, t, nt, d);
+            }
+            store8<DT, ALIGNED, RES32>(dres_out, q[i], i, t, nt, d);
+            if (has_y) {
+                yr[i] = get16(a.off_y, y_row(row), i);
+                Raw<false> wp, gr;
+                if (has_post) wp = getw(s_wpost, a.w_post, i);
+                if (gate_form == kGateChannel) gr = getw(s_wgate, a.gate, i);
+                if (gate_form == kGateFull) {
+                    gr = get16(a.off_gate, g_row(row), i);
+                    float dg[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dg[j] = a.scale * post * q[i][j] * raw_get<DT, false>(yr[i], j);
+                    if (has_post) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) dg[j] *= raw_get<DT, false>(wp, j);
+                    }
+                    store8<DT, ALIGNED, false>(dg_out, dg, i, t, nt, d);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[i][j] *= raw_get<DT, false>(gr, j);
+                }
+                if (has_post || gate_form == kGateChannel) {
+                    const float fp = gate_form == kGateChannel ? post : f * post;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s_post[i][j] += q[i][j] * (fp * raw_get<DT, false>(yr[i], j));
+                }
+                if (gate_form == kGateChannel) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[i][j] *= raw_get<DT, false>(gr, j);
+                }
+                if (has_post) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[i][j] *= raw_get<DT, false>(wp, j);
+                }
+                if (has_post || gate_form == kGateToken) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum2[0] += q[i][j] * raw_get<DT, false>(yr[i], j);
+                }
             }
         }
         if (RING) {  // the stage is read
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(empty + st);
+            if (++st == a.stages) st = 0, ph ^= 1;
         }
-        if (a.y) {
-            if (a.w_post || a.gate_form == kGateToken) row_sum<WARP>(sums2, s_red, phase);
-            if (a.gate_form == kGateToken && t == 0) static_cast<float*>(a.d_gate)[row] = sums2[1];
-            const float m = sums2[0] * inv_d;
-            uint16_t* dy_out = static_cast<uint16_t*>(a.d_y) + row * d;
+        if (has_y) {
+            if (has_post || gate_form == kGateToken) row_sum<WARP>(sum2, s_red, phase);
+            if (gate_form == kGateToken && t == 0) static_cast<float*>(a.d_gate)[row] = a.scale * post * sum2[0];
+            const float fp = f * post, m = sum2[0] * inv_d * post * post;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (a.w_post) {
+                if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
+                if (has_post) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) q[i][j] = post * (q[i][j] - raw_get<DT, false>(yr[i], j) * post * m);
+                    for (int j = 0; j < 8; ++j) q[i][j] = fp * (q[i][j] - raw_get<DT, false>(yr[i], j) * m);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[i][j] *= f;
                 }
                 store8<DT, ALIGNED, false>(dy_out, q[i], i, t, nt, d);
             }
         }
+        dres_out += step * d * kRes;
+        dy_out += step * d;
+        dg_out += step * d;
     }
 
     // Column sums: the CTA's rows side by side add up through shared memory in
-    // warp order, then the CTA writes its row of partial sums.
+    // warp order, then the CTA writes its rows of partial sums.
     __syncthreads();  // the ring is free
     float* s_col = reinterpret_cast<float*>(s_dyn);
 #pragma unroll
-    for (int which = 0; which < 3; ++which) {
-        const int vec = which == 0 ? a.sum_pre : which == 1 ? a.sum_post : a.sum_gate;
-        if (vec < 0) continue;
-        float* part = a.part + (int64_t(vec) * gridDim.x + blockIdx.x) * d;
-        float(&s)[V][8] = which == 0 ? s_pre : which == 1 ? s_post : s_gate;
+    for (int which = 0; which < 2; ++which) {
+        if (which == 0 ? a.sum_pre < 0 : a.sum_post < 0 && a.sum_gate < 0) continue;
+        float(&s)[V][8] = which == 0 ? s_pre : s_post;
         for (int g = 0; g < groups - 1; ++g) {
             if (group == g) {
 #pragma unroll
@@ -479,12 +568,32 @@ block_norm_backward_kernel(const NormGradArgs a) {
         if (group == groups - 1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int col = col_of<ALIGNED>(i, j, t, nt);
                     if (groups > 1 && col < d) s[i][j] += s_col[col];
                 }
-                store8<DT, ALIGNED, true>(part, s[i], i, t, nt, d);
+                auto row_of = [&](int vec) { return a.part + (int64_t(vec) * gridDim.x + blockIdx.x) * d; };
+                if (which == 0) {
+                    store8<DT, ALIGNED, true>(row_of(a.sum_pre), s[i], i, t, nt, d);
+                } else if (a.sum_gate < 0) {
+                    store8<DT, ALIGNED, true>(row_of(a.sum_post), s[i], i, t, nt, d);
+                } else {
+                    const Raw<false> gr = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
+                    float v[8];
+                    if (has_post) {
+                        const Raw<false> wp = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = a.scale * raw_get<DT, false>(gr, j) * s[i][j];
+                        store8<DT, ALIGNED, true>(row_of(a.sum_post), v, i, t, nt, d);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) s[i][j] *= raw_get<DT, false>(wp, j);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = a.scale * s[i][j];
+                    store8<DT, ALIGNED, true>(row_of(a.sum_gate), v, i, t, nt, d);
+                }
             }
         }
         __syncthreads();
@@ -576,9 +685,9 @@ static int check_norm(const char* who, int T, int d, int dtype, int gate_form, c
     return MOE_B200_OK;
 }
 
-template <int DT, bool RES32, bool AL, bool WARP, int MAXT>
+template <int DT, bool RES32, bool AL, bool WARP, int MAXT, int FORM>
 static cudaError_t launch_norm_as(const NormArgs& a, int cta, cudaStream_t s) {
-    auto kern = block_norm_kernel<DT, RES32, AL, WARP, 2, MAXT>;
+    auto kern = block_norm_kernel<DT, RES32, AL, WARP, 2, MAXT, FORM>;
     static std::atomic<int> per_sm[MAXT / 32 + 1];  // CTAs an SM holds, by warps a CTA
     std::atomic<int>& fit = per_sm[cta / 32];
     int n = fit.load(std::memory_order_relaxed);
@@ -594,25 +703,49 @@ static cudaError_t launch_norm_as(const NormArgs& a, int cta, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-template <int DT, bool RES32, bool AL>
-static cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
+template <int DT, bool RES32, bool AL, int FORM>
+static cudaError_t launch_norm_form(const NormArgs& a, cudaStream_t s) {
     const int nt = row_threads_for(a.d, 2);
-    if (nt == 32) return launch_norm_as<DT, RES32, AL, true, 128>(a, 128, s);
-    if (nt <= 256) return launch_norm_as<DT, RES32, AL, false, 256>(a, nt, s);
-    return launch_norm_as<DT, RES32, AL, false, 1024>(a, nt, s);
+    if (nt == 32) return launch_norm_as<DT, RES32, AL, true, 128, FORM>(a, 128, s);
+    if (nt <= 128) return launch_norm_as<DT, RES32, AL, false, 128, FORM>(a, nt, s);
+    if (nt <= 256) return launch_norm_as<DT, RES32, AL, false, 256, FORM>(a, nt, s);
+    return launch_norm_as<DT, RES32, AL, false, 1024, FORM>(a, nt, s);
 }
 
-// Shared memory of the ring that lets two CTAs (or the one of a wide row) stay on an SM.
-constexpr size_t kNormRingLimit = 200 * 1024;
+template <int DT, bool RES32, bool AL>
+static cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
+    if constexpr (AL) {
+        if (a.w_pre) {
+            if (!a.y) return launch_norm_form<DT, RES32, AL, kFormNorm>(a, s);
+            if (a.w_post)
+                return a.gate_form >= kGateChannel ? launch_norm_form<DT, RES32, AL, kFormFullColGate>(a, s)
+                                                   : launch_norm_form<DT, RES32, AL, kFormFull>(a, s);
+            if (a.gate_form < kGateChannel) return launch_norm_form<DT, RES32, AL, kFormAddNorm>(a, s);
+        }
+    }
+    return launch_norm_form<DT, RES32, AL, kFormAny>(a, s);
+}
 
-template <int DT, bool RES32, bool AL, bool RING, bool WARP, int V>
+template <int DT, bool RES32, bool AL, bool RING, bool WARP, int V, int GATE = -1>
 static cudaError_t launch_norm_backward_as(const NormGradArgs& a, const NormGradPlan& p, size_t smem, cudaStream_t s) {
     constexpr int kMax = WARP ? 128 : 512;
-    auto kern = block_norm_backward_kernel<DT, RES32, AL, RING, WARP, V, kMax>;
+    auto kern = block_norm_backward_kernel<DT, RES32, AL, RING, WARP, V, kMax, GATE>;
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (err != cudaSuccess) return err;
     kern<<<p.grid, p.cta_threads, smem, s>>>(a);
     return cudaGetLastError();
+}
+
+template <int DT, bool RES32, bool WARP>
+static cudaError_t launch_norm_backward_ring(const NormGradArgs& a, const NormGradPlan& p, size_t smem, cudaStream_t s) {
+    if (a.w_pre && a.w_post && a.d_res_out) {
+        if (a.gate_form == kGateNone) return launch_norm_backward_as<DT, RES32, true, true, WARP, 2, kGateNone>(a, p, smem, s);
+        if (a.gate_form == kGateToken) return launch_norm_backward_as<DT, RES32, true, true, WARP, 2, kGateToken>(a, p, smem, s);
+        if (a.gate_form == kGateChannel)
+            return launch_norm_backward_as<DT, RES32, true, true, WARP, 2, kGateChannel>(a, p, smem, s);
+        return launch_norm_backward_as<DT, RES32, true, true, WARP, 2, kGateFull>(a, p, smem, s);
+    }
+    return launch_norm_backward_as<DT, RES32, true, true, WARP, 2>(a, p, smem, s);
 }
 
 template <int DT, bool RES32, bool AL>
@@ -632,14 +765,21 @@ static cudaError_t launch_norm_backward(const NormGradArgs& a0, const NormGradPl
     a.off_gate = part(a.gate_form == kGateFull, a.d * 2);
     a.row_bytes = off;
     const size_t cols = groups > 1 ? size_t(a.d) * 4 : 0;
-    const size_t ring = size_t(groups) * kNormStages * off;
-    const bool use_ring = AL && p.v == 2 && ring <= kNormRingLimit;
+    // Ring: as many rows as fit the share of an SM's shared memory that each
+    // of the CTAs it holds may take, two at least.
+    const size_t weights = size_t(column_vectors(a.w_pre != nullptr, a.w_post != nullptr, a.gate_form)) * a.d * 2;
+    const size_t share = 227 * 1024 / (512 / p.cta_threads) - 3 * 1024;
+    a.stages = kNormStages;
+    while (a.stages > 1 && size_t(groups) * a.stages * off + weights > share) --a.stages;
+    a.off_w = groups * a.stages * off;
+    const size_t ring = size_t(a.off_w) + weights;
+    const bool use_ring = AL && p.v == 2 && a.stages > 1;
     const size_t smem = use_ring && ring > cols ? ring : cols;
     const bool warp = p.row_threads == 32;
     if constexpr (AL) {
         if (use_ring) {
-            if (warp) return launch_norm_backward_as<DT, RES32, AL, true, true, 2>(a, p, smem, s);
-            return launch_norm_backward_as<DT, RES32, AL, true, false, 2>(a, p, smem, s);
+            if (warp) return launch_norm_backward_ring<DT, RES32, true>(a, p, smem, s);
+            return launch_norm_backward_ring<DT, RES32, false>(a, p, smem, s);
         }
     }
     if (warp) return launch_norm_backward_as<DT, RES32, AL, false, true, 2>(a, p, smem, s);
@@ -734,7 +874,7 @@ extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const vo
     if (!status) return fail(MOE_B200_ERR_CUDA, "block_norm_backward: device status word unavailable");
     const NormGradArgs a{d_residual_out, d_normed, residual_out, y, w_post, w_pre, gate, y ? y_stride : 0,
                          w_pre ? residual_stride : 0, gate_form, scale, eps, T, d, d_residual, d_y, d_gate,
-                         static_cast<float*>(workspace), i_pre, i_post, i_gate, 0, -1, -1, -1, -1, -1, status};
+                         static_cast<float*>(workspace), i_pre, i_post, i_gate, 0, -1, -1, -1, -1, -1, 0, 0, status};
     const bool al = d % 8 == 0 && a.y_stride % 8 == 0 && a.res_stride % (res32 ? 4 : 8) == 0 &&
                     aligned16({d_residual_out, d_normed, residual_out, y, w_post, w_pre,
                                gate_form >= kGateChannel ? gate : nullptr, d_residual, d_y,
