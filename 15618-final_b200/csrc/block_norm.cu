@@ -19,7 +19,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -168,9 +167,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
 }
 // Zeros for the places of warps that do not exist; before the first row_sum.
 template <bool WARP> __device__ __forceinline__ void row_sum_init(float* red) {
-    if (WARP) return;
-    for (int i = threadIdx.x; i < kRedFloats; i += blockDim.x) red[i] = 0.f;
-    __syncthreads();
+    if (!WARP) {
+        for (int i = threadIdx.x; i < kRedFloats; i += blockDim.x) red[i] = 0.f;
+        __syncthreads();
+    }
 }
 
 struct NormArgs {
@@ -180,7 +180,13 @@ struct NormArgs {
     float scale, eps;
     int T, d;
     void *residual_out, *normed;
+    // Ring of rows in shared memory (RING): rows in flight, bytes of a staged
+    // row and where y and a full gate lie in it (the residual comes first).
+    int stages, row_bytes, off_y, off_gate;
+    uint32_t* status;
 };
+
+constexpr int kNormStages = 4;  // rows in flight, at most
 
 // What a call consists of, where it is known when compiling (the forms that
 // models run all the time); kFormAny asks the arguments.  A column gate is one
@@ -194,54 +200,86 @@ template <int FORM> struct Form {
 
 // A row belongs to one warp (WARP: CTAs of 4 rows) or to a CTA; each thread
 // holds V chunks of 8 columns.  The grid fits the card and walks the rows; the
-// weights stay packed in registers and the next row's loads are in flight
-// while a row is reduced and written.
-template <int DT, bool RES32, bool ALIGNED, bool WARP, int V, int MAXT, int FORM>
+// weights stay packed in registers.  RING: rows come through a ring of shared-
+// memory stages filled by bulk copies some rows ahead; otherwise (rows not in
+// 16-byte steps, too wide, or at most one row a CTA) by plain loads.
+template <int DT, bool RES32, bool ALIGNED, bool RING, bool WARP, int V, int MAXT, int FORM>
 __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 768 / MAXT : 1)  // 80 registers: 24 warps an SM
 block_norm_kernel(const NormArgs a) {
     using F = Form<FORM>;
+    extern __shared__ __align__(128) unsigned char s_dyn[];
     __shared__ __align__(16) float s_red[kRedFloats];
+    __shared__ uint64_t s_full[4 * kNormStages], s_empty[4 * kNormStages];
     const bool has_y = F::any ? a.y != nullptr : F::y, has_post = F::any ? a.w_post != nullptr : F::post;
     const bool has_col = F::any ? a.gate_form >= kGateChannel : F::col, has_pre = F::any ? a.w_pre != nullptr : true;
     const int nt = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
-    const int rows_per_cta = WARP ? blockDim.x >> 5 : 1;
-    const int64_t step = int64_t(gridDim.x) * rows_per_cta;
-    int64_t row = int64_t(blockIdx.x) * rows_per_cta + (WARP ? threadIdx.x >> 5 : 0);
-    if (row >= a.T) return;
+    const int groups = WARP ? blockDim.x >> 5 : 1, group = WARP ? threadIdx.x >> 5 : 0;
+    const int64_t step = int64_t(gridDim.x) * groups;
+    const int64_t row0 = int64_t(blockIdx.x) * groups + group;
     row_sum_init<WARP>(s_red);
+    if (row0 >= a.T) return;
     int phase = 0;
     const int d = a.d;
     const float inv_d = 1.0f / float(d);
     constexpr int kRes = RES32 ? 4 : 2;
-    const int64_t gate_stride = a.gate_form == kGateFull ? d : 0;
-    Raw<false> wp[V], wn[V], yr[V], gr[V];
-    Raw<RES32> res[V];
-    // Next row to load, and this row's results.
-    const char* res_row = static_cast<const char*>(a.residual) + row * a.res_stride * kRes;
-    const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + row * a.y_stride;
-    const uint16_t* g_row = static_cast<const uint16_t*>(a.gate) + row * gate_stride;
-    char* res_out = static_cast<char*>(a.residual_out) + row * d * kRes;
-    uint16_t* norm_out = static_cast<uint16_t*>(a.normed) + row * d;
-    auto fetch = [&]() {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
-            res[i] = load_raw<ALIGNED, RES32>(res_row, i, t, nt, d);
-            if (has_y) yr[i] = load_raw<ALIGNED, false>(y_row, i, t, nt, d);
-            if (has_col) gr[i] = load_raw<ALIGNED, false>(g_row, i, t, nt, d);
-        }
+    const bool gate_rows = has_col && a.gate_form == kGateFull;
+    uint64_t *full = s_full + group * kNormStages, *empty = s_empty + group * kNormStages;
+    unsigned char* ring = s_dyn + group * a.stages * a.row_bytes;
+
+    // Rows of the operands: of the next one to fetch.
+    const char* res_row = static_cast<const char*>(a.residual) + row0 * a.res_stride * kRes;
+    const uint16_t* y_row = static_cast<const uint16_t*>(a.y) + row0 * a.y_stride;
+    const uint16_t* g_row = static_cast<const uint16_t*>(a.gate) + (gate_rows ? row0 * d : 0);
+    auto next_rows = [&]() {
         res_row += step * a.res_stride * kRes;
         if (has_y) y_row += step * a.y_stride;
-        if (has_col) g_row += step * gate_stride;
+        if (gate_rows) g_row += step * d;
     };
-    fetch();
+    auto fill = [&](int s) {  // one thread
+        unsigned char* p = ring + s * a.row_bytes;
+        mbar_arrive_expect_tx(full + s, a.row_bytes);
+        bulk_g2s(p, res_row, d * kRes, full + s);
+        if (has_y) bulk_g2s(p + a.off_y, y_row, d * 2, full + s);
+        if (gate_rows) bulk_g2s(p + a.off_gate, g_row, d * 2, full + s);
+        next_rows();
+    };
+    if (RING) {
+        if (t == 0) {
+            for (int s = 0; s < a.stages; ++s) {
+                mbar_init(full + s, 1);
+                mbar_init(empty + s, nt >> 5);
+            }
+            mbar_fence_init();
+        }
+        if (WARP) __syncwarp();
+        else __syncthreads();
+        if (t == 0)
+            for (int s = 0; s < a.stages; ++s)
+                if (row0 + s * step < a.T) fill(s);
+    }
+    Raw<false> wp[V], wn[V], gc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
         if (has_post) wp[i] = load_raw<ALIGNED, false>(a.w_post, i, t, nt, d);
         if (has_pre) wn[i] = load_raw<ALIGNED, false>(a.w_pre, i, t, nt, d);
+        if (has_col && !gate_rows) gc[i] = load_raw<ALIGNED, false>(a.gate, i, t, nt, d);
     }
-    for (; row < a.T; row += step) {
+    int st = 0;
+    uint32_t ph = 0;
+    char* res_out = static_cast<char*>(a.residual_out) + row0 * d * kRes;
+    uint16_t* norm_out = static_cast<uint16_t*>(a.normed) + row0 * d;
+    for (int64_t row = row0; row < a.T; row += step) {
+        const unsigned char* p = ring + st * a.row_bytes;
+        if (RING) {
+            // Refill the stage of the row before, once all its warps have read it.
+            if (t == 0 && row > row0 && row + (a.stages - 1) * step < a.T) {
+                const int prev = st == 0 ? a.stages - 1 : st - 1;
+                if (!mbar_wait(empty + prev, st == 0 ? ph ^ 1u : ph)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
+                fill(prev);
+            }
+            if (!mbar_wait(full + st, ph)) atomicOr(a.status, MOE_B200_DEV_WAIT_TIMEOUT);
+        }
         float r[V][8], z[V][8];
         float s[1] = {0.f};
         float f = a.scale;
@@ -249,11 +287,19 @@ block_norm_kernel(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
+            const Raw<RES32> res = RING ? load_raw<ALIGNED, RES32>(p, i, t, nt, d) : load_raw<ALIGNED, RES32>(res_row, i, t, nt, d);
+            Raw<false> yr, gr;
+            if (has_y) yr = RING ? load_raw<ALIGNED, false>(p + a.off_y, i, t, nt, d) : load_raw<ALIGNED, false>(y_row, i, t, nt, d);
+            if (has_col) {
+                gr = gc[i];
+                if (gate_rows)
+                    gr = RING ? load_raw<ALIGNED, false>(p + a.off_gate, i, t, nt, d) : load_raw<ALIGNED, false>(g_row, i, t, nt, d);
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[i][j] = raw_get<DT, RES32>(res[i], j);
+            for (int j = 0; j < 8; ++j) r[i][j] = raw_get<DT, RES32>(res, j);
             if (has_y) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) z[i][j] = raw_get<DT, false>(yr[i], j);
+                for (int j = 0; j < 8; ++j) z[i][j] = raw_get<DT, false>(yr, j);
                 if (has_post) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -263,11 +309,17 @@ block_norm_kernel(const NormArgs a) {
                 }
                 if (has_col) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[i][j] *= raw_get<DT, false>(gr[i], j);
+                    for (int j = 0; j < 8; ++j) z[i][j] *= raw_get<DT, false>(gr, j);
                 }
             }
         }
-        if (row + step < a.T) fetch();
+        if (RING) {  // the stage is read
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(empty + st);
+            if (++st == a.stages) st = 0, ph ^= 1;
+        } else {
+            next_rows();
+        }
         if (has_y) {
             if (has_post) {
                 row_sum<WARP>(s, s_red, phase);
@@ -321,8 +373,6 @@ struct NormGradArgs {
     uint32_t* status;
 };
 
-constexpr int kNormStages = 4;  // at most
-
 // Rows are dealt to a grid that fits the card, so that each thread keeps its
 // columns' sums over its rows in registers and the column gradients cost one
 // row of partial sums a CTA.  RING: the rows come through a ring of shared-
@@ -341,7 +391,6 @@ block_norm_backward_kernel(const NormGradArgs a) {
     const bool has_y = kAny ? a.y != nullptr : true, has_post = kAny ? a.w_post != nullptr : true;
     const bool has_pre = kAny ? a.w_pre != nullptr : true, has_ds = kAny ? a.d_res_out != nullptr : true;
     const int gate_form = kAny ? a.gate_form : GATE;
-    const bool has_col = gate_form >= kGateChannel;
     const int nt = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
     const int groups = WARP ? blockDim.x >> 5 : 1, group = WARP ? threadIdx.x >> 5 : 0;
     const int64_t step = int64_t(gridDim.x) * groups;
@@ -685,45 +734,51 @@ static int check_norm(const char* who, int T, int d, int dtype, int gate_form, c
     return MOE_B200_OK;
 }
 
-template <int DT, bool RES32, bool AL, bool WARP, int MAXT, int FORM>
-static cudaError_t launch_norm_as(const NormArgs& a, int cta, cudaStream_t s) {
-    auto kern = block_norm_kernel<DT, RES32, AL, WARP, 2, MAXT, FORM>;
-    static std::atomic<int> per_sm[MAXT / 32 + 1];  // CTAs an SM holds, by warps a CTA
-    std::atomic<int>& fit = per_sm[cta / 32];
-    int n = fit.load(std::memory_order_relaxed);
-    if (n == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, cta, 0) != cudaSuccess || n < 1) n = 1;
-        fit.store(n, std::memory_order_relaxed);
-    }
-    const int rows = WARP ? cta / 32 : 1;
-    int64_t grid = (int64_t(a.T) + rows - 1) / rows;
-    const int64_t most = int64_t(sm_count_norm()) * n;
-    if (grid > most) grid = most;
-    kern<<<unsigned(grid), cta, 0, s>>>(a);
+template <int DT, bool RES32, bool AL, bool RING, bool WARP, int MAXT, int FORM>
+static cudaError_t launch_norm_as(NormArgs a, int cta, int64_t grid, size_t smem, cudaStream_t s) {
+    auto kern = block_norm_kernel<DT, RES32, AL, RING, WARP, 2, MAXT, FORM>;
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (err != cudaSuccess) return err;
+    kern<<<unsigned(grid), cta, smem, s>>>(a);
     return cudaGetLastError();
 }
 
-template <int DT, bool RES32, bool AL, int FORM>
-static cudaError_t launch_norm_form(const NormArgs& a, cudaStream_t s) {
-    const int nt = row_threads_for(a.d, 2);
-    if (nt == 32) return launch_norm_as<DT, RES32, AL, true, 128, FORM>(a, 128, s);
-    if (nt <= 128) return launch_norm_as<DT, RES32, AL, false, 128, FORM>(a, nt, s);
-    if (nt <= 256) return launch_norm_as<DT, RES32, AL, false, 256, FORM>(a, nt, s);
-    return launch_norm_as<DT, RES32, AL, false, 1024, FORM>(a, nt, s);
+template <int DT, bool RES32, bool AL, bool RING, int FORM>
+static cudaError_t launch_norm_form(const NormArgs& a, int nt, int64_t grid, size_t smem, cudaStream_t s) {
+    if (nt == 32) return launch_norm_as<DT, RES32, AL, RING, true, 128, FORM>(a, 128, grid, smem, s);
+    if (nt <= 128) return launch_norm_as<DT, RES32, AL, RING, false, 128, FORM>(a, nt, grid, smem, s);
+    if (nt <= 256) return launch_norm_as<DT, RES32, AL, RING, false, 256, FORM>(a, nt, grid, smem, s);
+    return launch_norm_as<DT, RES32, AL, RING, false, 1024, FORM>(a, nt, grid, smem, s);
 }
 
 template <int DT, bool RES32, bool AL>
-static cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
+static cudaError_t launch_norm(const NormArgs& a0, cudaStream_t s) {
+    NormArgs a = a0;
+    const int nt = row_threads_for(a.d, 2), cta = nt == 32 ? 128 : nt, groups = cta / nt;
+    const int per_sm = cta <= 256 ? 768 / cta : 1024 / cta;  // what the registers allow
+    const int64_t need = (int64_t(a.T) + groups - 1) / groups, most = int64_t(sm_count_norm()) * per_sm;
     if constexpr (AL) {
-        if (a.w_pre) {
-            if (!a.y) return launch_norm_form<DT, RES32, AL, kFormNorm>(a, s);
-            if (a.w_post)
-                return a.gate_form >= kGateChannel ? launch_norm_form<DT, RES32, AL, kFormFullColGate>(a, s)
-                                                   : launch_norm_form<DT, RES32, AL, kFormFull>(a, s);
-            if (a.gate_form < kGateChannel) return launch_norm_form<DT, RES32, AL, kFormAddNorm>(a, s);
+        a.off_y = a.d * (RES32 ? 4 : 2);
+        a.off_gate = a.off_y + (a.y ? a.d * 2 : 0);
+        a.row_bytes = a.off_gate + (a.gate_form == kGateFull ? a.d * 2 : 0);
+        const size_t share = 227 * 1024 / per_sm - 3 * 1024;
+        a.stages = kNormStages;
+        while (a.stages > 1 && size_t(groups) * a.stages * a.row_bytes > share) --a.stages;
+        if (need > most && a.stages > 1) {
+            const size_t smem = size_t(groups) * a.stages * a.row_bytes;
+            if (a.w_pre) {
+                if (!a.y) return launch_norm_form<DT, RES32, true, true, kFormNorm>(a, nt, most, smem, s);
+                if (a.w_post)
+                    return a.gate_form >= kGateChannel
+                               ? launch_norm_form<DT, RES32, true, true, kFormFullColGate>(a, nt, most, smem, s)
+                               : launch_norm_form<DT, RES32, true, true, kFormFull>(a, nt, most, smem, s);
+                if (a.gate_form < kGateChannel)
+                    return launch_norm_form<DT, RES32, true, true, kFormAddNorm>(a, nt, most, smem, s);
+            }
+            return launch_norm_form<DT, RES32, true, true, kFormAny>(a, nt, most, smem, s);
         }
     }
-    return launch_norm_form<DT, RES32, AL, kFormAny>(a, s);
+    return launch_norm_form<DT, RES32, AL, false, kFormAny>(a, nt, need < most ? need : most, 0, s);
 }
 
 template <int DT, bool RES32, bool AL, bool RING, bool WARP, int V, int GATE = -1>
@@ -818,8 +873,10 @@ extern "C" int moe_b200_block_norm(const void* y, int64_t y_stride, const void* 
     if (residual_stride < d || (y && y_stride < d))
         return fail(MOE_B200_ERR_INVALID_ARG, "block_norm: row strides below d=%d", d);
     if (T == 0) return MOE_B200_OK;
+    uint32_t* status = device_status_word();
+    if (!status) return fail(MOE_B200_ERR_CUDA, "block_norm: device status word unavailable");
     const NormArgs a{y, residual, w_post, w_pre, gate, y ? y_stride : 0, residual_stride, gate_form, scale, eps, T, d,
-                     y ? residual_out : nullptr, w_pre ? normed : nullptr};
+                     y ? residual_out : nullptr, w_pre ? normed : nullptr, 0, 0, 0, 0, status};
     const bool al = d % 8 == 0 && (!y || y_stride % 8 == 0) && residual_stride % (residual_f32 ? 4 : 8) == 0 &&
                     aligned16({y, residual, w_post, w_pre, gate_form >= kGateChannel ? gate : nullptr, a.residual_out,
                                a.normed});
