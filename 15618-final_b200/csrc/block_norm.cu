@@ -52,6 +52,31 @@ template <int DT> __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Pairs of fp32 values in one 64-bit register: sm_100a multiplies and adds two
+// at a time (each half rounded as the single operation).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float sum2(f32x2 v) {
+    float lo, hi;
+    split(v, lo, hi);
+    return lo + hi;
+}
+
 // A row's columns as a thread holds them: V chunks of 8.  Aligned rows
 // (ALIGNED: d, strides and pointers in 16-byte steps) give a thread 8
 // consecutive columns per chunk, one 16-byte access (two for fp32); other rows
@@ -103,6 +128,12 @@ __device__ __forceinline__ float raw_get(const Raw<F32>& r, int j) {
     const uint32_t w = r.w[(j >> 1) % 4];
     if (DT == MOE_B200_BF16) return __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));
     return from16<DT>(uint16_t((j & 1) ? (w >> 16) : w));
+}
+
+// Columns 2j and 2j + 1 of a chunk as a pair.
+template <int DT, bool F32>
+__device__ __forceinline__ f32x2 raw_pair(const Raw<F32>& r, int j) {
+    return pair(raw_get<DT, F32>(r, 2 * j), raw_get<DT, F32>(r, 2 * j + 1));
 }
 
 // Eight fp32 values to a row of 16-bit or fp32 columns.
@@ -171,6 +202,14 @@ template <bool WARP> __device__ __forceinline__ void row_sum_init(float* red) {
         for (int i = threadIdx.x; i < kRedFloats; i += blockDim.x) red[i] = 0.f;
         __syncthreads();
     }
+}
+
+template <int DT, bool ALIGNED, bool F32>
+__device__ __forceinline__ void store8(void* row, const f32x2 (&x)[4], int chunk, int t, int nt, int d) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split(x[j], v[2 * j], v[2 * j + 1]);
+    store8<DT, ALIGNED, F32>(row, v, chunk, t, nt, d);
 }
 
 struct NormArgs {
@@ -439,11 +478,11 @@ block_norm_backward_kernel(const NormGradArgs a) {
 
     // Column sums.  A channel gate and w_post share one: with A = sum ds yh,
     // d_w_post = scale * gate * A and d_gate = scale * w_post * A.
-    float s_pre[V][8], s_post[V][8];
+    f32x2 s_pre[V][4], s_post[V][4];
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s_pre[i][j] = s_post[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) s_pre[i][j] = s_post[i][j] = 0;
 
     uint32_t n = 0;
     int st = 0;         // ring stage and its phase
@@ -472,7 +511,7 @@ block_norm_backward_kernel(const NormGradArgs a) {
         auto getw = [&](const unsigned char* s, const void* g, int i) {
             return RING ? load_raw<ALIGNED, false>(s, i, t, nt, d) : load_raw<ALIGNED, false>(g, i, t, nt, d);
         };
-        float sums[3] = {0.f, 0.f, 0.f};  // sum r'^2, sum u r', sum y^2
+        f32x2 p_rr = 0, p_ur = 0, p_yy = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
@@ -481,21 +520,22 @@ block_norm_backward_kernel(const NormGradArgs a) {
                 const Raw<false> dn = get16(a.off_dn, dn_row(row), i);
                 const Raw<RES32> rr = getres(a.off_rr, rr_row(row), i);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float r = raw_get<DT, RES32>(rr, j);
-                    sums[0] += r * r;
-                    sums[1] += raw_get<DT, false>(dn, j) * raw_get<DT, false>(wn, j) * r;
+                for (int j = 0; j < 4; ++j) {
+                    const f32x2 r = raw_pair<DT, RES32>(rr, j);
+                    p_rr = fma2(r, r, p_rr);
+                    p_ur = fma2(mul2(raw_pair<DT, false>(dn, j), raw_pair<DT, false>(wn, j)), r, p_ur);
                 }
             }
             if (has_post) {
                 const Raw<false> yr = get16(a.off_y, y_row(row), i);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = raw_get<DT, false>(yr, j);
-                    sums[2] += y * y;
+                for (int j = 0; j < 4; ++j) {
+                    const f32x2 y = raw_pair<DT, false>(yr, j);
+                    p_yy = fma2(y, y, p_yy);
                 }
             }
         }
+        float sums[3] = {sum2(p_rr), sum2(p_ur), sum2(p_yy)};  // sum r'^2, sum u r', sum y^2
         if (has_pre || has_post) row_sum<WARP>(sums, s_red, phase);
         const float c = rsqrtf(sums[0] * inv_d + a.eps);
         const float k = sums[1] * inv_d * c * c;  // ds = dr' + c dn w_pre - (c r') k
@@ -504,8 +544,10 @@ block_norm_backward_kernel(const NormGradArgs a) {
             gate_form == kGateToken ? from16<DT>(static_cast<const uint16_t*>(a.gate)[row]) : 1.0f;
         // q is first ds, then ds * (column gate) * w_post, without the row's scale f
         const float f = a.scale * gate_t;
-        float sum2[1] = {0.f};  // sum q yh
-        float q[V][8];
+        const float fa = gate_form == kGateChannel ? post : f * post;  // of the sum behind w_post
+        const f32x2 c2 = pair(c, c), k2 = pair(-k, -k), fa2 = pair(fa, fa), dg2 = pair(a.scale * post, a.scale * post);
+        f32x2 p_qy = 0;
+        f32x2 q[V][4];
         Raw<false> yr[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -513,20 +555,20 @@ block_norm_backward_kernel(const NormGradArgs a) {
             if (has_ds) {
                 const Raw<RES32> ds = getres(a.off_ds, ds_row(row), i);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) q[i][j] = raw_get<DT, RES32>(ds, j);
+                for (int j = 0; j < 4; ++j) q[i][j] = raw_pair<DT, RES32>(ds, j);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) q[i][j] = 0.f;
+                for (int j = 0; j < 4; ++j) q[i][j] = 0;
             }
             if (has_pre) {
                 const Raw<false> wn = getw(s_wpre, a.w_pre, i);
                 const Raw<false> dn = get16(a.off_dn, dn_row(row), i);
                 const Raw<RES32> rr = getres(a.off_rr, rr_row(row), i);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float rc = raw_get<DT, RES32>(rr, j) * c, dnj = raw_get<DT, false>(dn, j);
-                    s_pre[i][j] += dnj * rc;
-                    q[i][j] += c * (dnj * raw_get<DT, false>(wn, j)) - rc * k;
+                for (int j = 0; j < 4; ++j) {
+                    const f32x2 rc = mul2(raw_pair<DT, RES32>(rr, j), c2), dnj = raw_pair<DT, false>(dn, j);
+                    s_pre[i][j] = fma2(dnj, rc, s_pre[i][j]);
+                    q[i][j] = fma2(c2, mul2(dnj, raw_pair<DT, false>(wn, j)), fma2(rc, k2, q[i][j]));
                 }
             }
             store8<DT, ALIGNED, RES32>(dres_out, q[i], i, t, nt, d);
@@ -537,33 +579,31 @@ block_norm_backward_kernel(const NormGradArgs a) {
                 if (gate_form == kGateChannel) gr = getw(s_wgate, a.gate, i);
                 if (gate_form == kGateFull) {
                     gr = get16(a.off_gate, g_row(row), i);
-                    float dg[8];
+                    f32x2 dg[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) dg[j] = a.scale * post * q[i][j] * raw_get<DT, false>(yr[i], j);
-                    if (has_post) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) dg[j] *= raw_get<DT, false>(wp, j);
+                    for (int j = 0; j < 4; ++j) {
+                        dg[j] = mul2(mul2(q[i][j], dg2), raw_pair<DT, false>(yr[i], j));
+                        if (has_post) dg[j] = mul2(dg[j], raw_pair<DT, false>(wp, j));
+                        q[i][j] = mul2(q[i][j], raw_pair<DT, false>(gr, j));
                     }
                     store8<DT, ALIGNED, false>(dg_out, dg, i, t, nt, d);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q[i][j] *= raw_get<DT, false>(gr, j);
                 }
                 if (has_post || gate_form == kGateChannel) {
-                    const float fp = gate_form == kGateChannel ? post : f * post;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) s_post[i][j] += q[i][j] * (fp * raw_get<DT, false>(yr[i], j));
+                    for (int j = 0; j < 4; ++j)
+                        s_post[i][j] = fma2(q[i][j], mul2(fa2, raw_pair<DT, false>(yr[i], j)), s_post[i][j]);
                 }
                 if (gate_form == kGateChannel) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) q[i][j] *= raw_get<DT, false>(gr, j);
+                    for (int j = 0; j < 4; ++j) q[i][j] = mul2(q[i][j], raw_pair<DT, false>(gr, j));
                 }
                 if (has_post) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) q[i][j] *= raw_get<DT, false>(wp, j);
+                    for (int j = 0; j < 4; ++j) q[i][j] = mul2(q[i][j], raw_pair<DT, false>(wp, j));
                 }
                 if (has_post || gate_form == kGateToken) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum2[0] += q[i][j] * raw_get<DT, false>(yr[i], j);
+                    for (int j = 0; j < 4; ++j) p_qy = fma2(q[i][j], raw_pair<DT, false>(yr[i], j), p_qy);
                 }
             }
         }
@@ -573,19 +613,17 @@ block_norm_backward_kernel(const NormGradArgs a) {
             if (++st == a.stages) st = 0, ph ^= 1;
         }
         if (has_y) {
-            if (has_post || gate_form == kGateToken) row_sum<WARP>(sum2, s_red, phase);
-            if (gate_form == kGateToken && t == 0) static_cast<float*>(a.d_gate)[row] = a.scale * post * sum2[0];
-            const float fp = f * post, m = sum2[0] * inv_d * post * post;
+            float qy[1] = {sum2(p_qy)};  // sum q y
+            if (has_post || gate_form == kGateToken) row_sum<WARP>(qy, s_red, phase);
+            if (gate_form == kGateToken && t == 0) static_cast<float*>(a.d_gate)[row] = a.scale * post * qy[0];
+            const float fp = f * post, m = -qy[0] * inv_d * post * post * fp;
+            const f32x2 fp2 = pair(fp, fp), m2 = pair(m, m), f2 = pair(f, f);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if (!chunk_in<ALIGNED>(i, t, nt, d)) continue;
-                if (has_post) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) q[i][j] = fp * (q[i][j] - raw_get<DT, false>(yr[i], j) * m);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q[i][j] *= f;
-                }
+                for (int j = 0; j < 4; ++j)
+                    q[i][j] = has_post ? fma2(fp2, q[i][j], mul2(raw_pair<DT, false>(yr[i], j), m2)) : mul2(q[i][j], f2);
                 store8<DT, ALIGNED, false>(dy_out, q[i], i, t, nt, d);
             }
         }
@@ -601,7 +639,11 @@ block_norm_backward_kernel(const NormGradArgs a) {
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         if (which == 0 ? a.sum_pre < 0 : a.sum_post < 0 && a.sum_gate < 0) continue;
-        float(&s)[V][8] = which == 0 ? s_pre : s_post;
+        float s[V][8];
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split(which == 0 ? s_pre[i][j] : s_post[i][j], s[i][2 * j], s[i][2 * j + 1]);
         for (int g = 0; g < groups - 1; ++g) {
             if (group == g) {
 #pragma unroll
