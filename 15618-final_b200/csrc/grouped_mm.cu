@@ -16,19 +16,33 @@
 //
 // One CTA per SM, 7 warps: TMA producer, MMA issuer, 4 epilogue warps (TMEM
 // accumulator double-buffered, so the epilogue of one tile runs under the MMAs
-// of the next), tile scheduler.  Forward and dgrad tiles cost the same, and a
-// persistent grid deals them round-robin.  A wgrad tile costs as much as its
-// segment has rows; there the grid is one CTA per tile and running CTAs take
-// over waiting ones (cluster launch control), which balances any routing.
+// of the next), tile scheduler.  Two forms share the code:
+//   CG=1  one SM per 128 x 256 tile, 48 KB a K step, 4 stages: for short
+//         segments, where a taller tile would be half empty
+//   CG=2  an SM pair (cluster of 2) per 256 x 256 tile: each CTA stages its 128
+//         rows of A and half of B, 32 KB a K step, 6 stages.  One SM cannot
+//         feed its tensor core at full rate (48 KB are written to and read from
+//         shared memory per 512 cycles); a pair can.
+// Forward and dgrad tiles cost the same, and a persistent grid deals them
+// round-robin.  A wgrad tile costs as much as its segment has rows; there the
+// grid is one CTA (pair) per tile and running ones take over waiting ones
+// (cluster launch control), which balances any routing.
 //
-// wgrad's last K step of a segment holds rows of the next segment: the MMA
-// warp clears those rows of both operands in shared memory (so that no
-// infinity or NaN there meets a zero) and issues only the 16-row MMAs that
-// hold rows.  Every wait is bounded, as in the expert FFN.
+// wgrad runs on single SMs (a pair would have to exchange the cleared ends of
+// segments).  Its last K step of a segment holds rows of the next segment: the
+// MMA warp clears them in shared memory in both operands (so that no infinity
+// or NaN there meets a zero) and issues only the 16-row MMAs that hold rows.
+//
+// The tensor core's queue holds about one K step: the loop of the issuing
+// thread has to come around within one MMA (128 cycles), so it does nothing
+// but wait, add to descriptors, issue and commit.  Every wait is bounded, as
+// in the expert FFN.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "gemm_epilogue.cuh"
@@ -41,26 +55,33 @@ int cuda_fail(cudaError_t err, const char* where);
 
 enum { kMmForward = 0, kMmDgrad = 1, kMmWgrad = 2 };
 
-constexpr int kMmTileM = 128;
+constexpr int kMmTileM = 128;  // rows of A per CTA
 constexpr int kMmTileN = 256;
 constexpr int kMmTileK = 64;
 constexpr int kMmThreads = 7 * 32;
-constexpr int kMmStages = 4;
 constexpr uint32_t kMmABytes = kMmTileM * kMmTileK * 2;  // 16 KB
-constexpr uint32_t kMmBBytes = kMmTileN * kMmTileK * 2;  // 32 KB
 constexpr uint32_t kMmBoxBytes = 64 * 64 * 2;            // one MN-major box: 64 columns x 64 reduced rows
 constexpr uint32_t kMmTmemCols = 512;
 constexpr int kMmMaxSegments = 1024;
 constexpr int kSchedSlots = 2;
+template <int CG> struct MmGeo {
+    static constexpr int kBlockRows = kMmTileM * CG;          // rows per tile
+    static constexpr int kBCols = kMmTileN / CG;              // columns of B a CTA holds
+    static constexpr uint32_t kBBytes = kBCols * kMmTileK * 2;
+    static constexpr int kStages = CG == 1 ? 4 : 6;           // 192 KB either way
+};
+constexpr int kMmMaxStages = 6;
 
 struct MmSmem {
-    uint64_t full[kMmStages];
-    uint64_t empty[kMmStages];
+    uint64_t full[kMmMaxStages];
+    uint64_t empty[kMmMaxStages];
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint64_t sched_full[kSchedSlots];
     uint64_t sched_empty[kSchedSlots];
-    uint4 sched[kSchedSlots];  // cluster launch control responses
+    uint64_t clc_full;  // answers of cluster launch control
+    uint4 clc;
+    int next[kSchedSlots];  // tiles handed to the warps
     uint32_t tmem_base;
     int abort_flag;
     int total_blocks;
@@ -127,17 +148,49 @@ __device__ __forceinline__ int clc_result(const uint4* response) {
     return ok ? int(x) : -1;
 }
 
-template <int MODE, int DT>
+// Completion of this thread's MMAs arrives on the barrier at this offset in
+// both CTAs of the pair.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(uint16_t(3))
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, int x, int y, int z,
+                                                uint32_t cluster_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
+        : "memory");
+}
+
+// Clears the reduced rows [from, to), 128 bytes each, of `boxes` MN-major boxes at `base`, by one warp.
+__device__ __forceinline__ void clear_rows(uint32_t base, int boxes, int from, int to, int lane) {
+    const int n = to - from;
+    for (int i = lane; i < n * 8 * boxes; i += 32) {
+        const int box = i / (n * 8), r = (i >> 3) % n, c = i & 7;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + box * kMmBoxBytes + (from + r) * 128 + c * 16),
+                     "r"(0)
+                     : "memory");
+    }
+}
+
+template <int MODE, int DT, int CG>
 __global__ void __launch_bounds__(kMmThreads, 1)
 grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                   const MmArgs a) {
     constexpr bool kDynamic = MODE == kMmWgrad;
+    using GEO = MmGeo<CG>;
+    constexpr int kStages = GEO::kStages;
+    constexpr uint32_t kBBytes = GEO::kBBytes;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char* sA = base;
-    unsigned char* sB = sA + kMmStages * kMmABytes;
-    unsigned char* s_stage = sB + kMmStages * kMmBBytes;
+    unsigned char* sA = base;  // [stages][A, B]: B follows A, so a stage's boxes are consecutive
+    constexpr uint32_t kStage = kMmABytes + kBBytes;
+    unsigned char* s_stage = base + kStages * kStage;
     MmSmem* ctl = reinterpret_cast<MmSmem*>(s_stage + kStageBytes);
     int32_t* blk_prefix = reinterpret_cast<int32_t*>(ctl + 1);  // [nseg + 1] row blocks before a segment
     int32_t* s_start = blk_prefix + (a.nseg + 1);               // [nseg] first row
@@ -146,20 +199,25 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &ctl->abort_flag;
+    // Pair coordinates: rank 0 is the leader, which issues the MMAs and finds the tiles.
+    const uint32_t crank = CG == 2 ? cluster_rank() : 0u;
+    const int tile0 = CG == 2 ? int(cluster_id_x()) : int(blockIdx.x);
+    const int tile_step = CG == 2 ? int(num_clusters_x()) : int(gridDim.x);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kMmStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(&ctl->full[s], 1);
             mbar_init(&ctl->empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&ctl->tmem_full[b], 1);
-            mbar_init(&ctl->tmem_empty[b], 4);
+            mbar_init(&ctl->tmem_empty[b], 4 * CG);
         }
         for (int b = 0; b < kSchedSlots; ++b) {
             mbar_init(&ctl->sched_full[b], 1);
             mbar_init(&ctl->sched_empty[b], 7);  // one arrival per warp
         }
+        mbar_init(&ctl->clc_full, 1);
         ctl->abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tmap_a);
@@ -176,7 +234,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 s_start[i] = lo;
                 s_rows[i] = max(hi - lo, 0);
                 s_exp[i] = a.seg_expert ? a.seg_expert[i] : i;
-                cnt = (s_rows[i] + kMmTileM - 1) / kMmTileM;
+                cnt = (s_rows[i] + GEO::kBlockRows - 1) / GEO::kBlockRows;
             }
             int incl = cnt;
 #pragma unroll
@@ -193,31 +251,39 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         }
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(&ctl->tmem_base)),
-                     "r"(kMmTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(&ctl->tmem_base)),
+                         "r"(kMmTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(&ctl->tmem_base)),
+                         "r"(kMmTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync();  // both CTAs' barriers initialised before any cross-CTA signal
     tc_fence_after();
 
     const uint32_t tmem = ctl->tmem_base;
     const int total_tiles = MODE == kMmWgrad ? a.nseg * a.m_blocks * a.n_blocks : ctl->total_blocks * a.n_blocks;
-    const int first_tile = int(blockIdx.x) < total_tiles ? int(blockIdx.x) : -1;
+    const int first_tile = tile0 < total_tiles ? tile0 : -1;
 
     // The tile after `tile`, or -1.  Called by whole warps.
     uint32_t sidx = 0;
     auto next_tile = [&](int tile) -> int {
         if (!kDynamic) {
-            const int n = tile + int(gridDim.x);
+            const int n = tile + tile_step;
             return n < total_tiles && !__any_sync(0xffffffffu, *abort_flag) ? n : -1;
         }
         const int slot = int(sidx % kSchedSlots);
         const bool ok = wait_or_abort(&ctl->sched_full[slot], (sidx / kSchedSlots) & 1u, abort_flag, a.status);
-        const int n = ok ? clc_result(&ctl->sched[slot]) : -1;
-        fence_proxy_async_smem();  // the answer is read before the next one is written
+        const int n = ok ? *const_cast<volatile int*>(&ctl->next[slot]) : -1;
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->sched_empty[slot]);
         ++sidx;
@@ -238,6 +304,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         m = g - blk_prefix[s];
         return (a.kdim + kMmTileK - 1) / kMmTileK;
     };
+    const uint32_t leader_full0 = CG == 2 ? map_to_rank(&ctl->full[0], 0) : 0u;
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
@@ -247,96 +314,132 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const int nk = locate(tile, s, m, n);
             if (lane == 0) {
                 const int e = s_exp[s], row0 = s_start[s];
+                const int a0 = m * GEO::kBlockRows + int(crank) * kMmTileM;    // rows of A (wgrad: columns of dy)
+                const int b0 = n * kMmTileN + int(crank) * GEO::kBCols;        // columns of the output
                 for (int kb = 0; kb < nk; ++kb, ++it) {
-                    const int st = int(it % kMmStages);
-                    if (!wait_or_abort(&ctl->empty[st], ((it / kMmStages) & 1u) ^ 1u, abort_flag, a.status)) break;
-                    uint64_t* bar = &ctl->full[st];
-                    mbar_arrive_expect_tx(bar, kMmABytes + kMmBBytes);
-                    unsigned char* pa = sA + st * kMmABytes;
-                    unsigned char* pb = sB + st * kMmBBytes;
-                    if (MODE == kMmWgrad) {
-                        for (int i = 0; i < kMmTileM / 64; ++i)
-                            tma_load_2d(pa + i * kMmBoxBytes, &tmap_a, m * kMmTileM + i * 64, row0 + kb * kMmTileK, bar);
-                        for (int i = 0; i < kMmTileN / 64; ++i)
-                            tma_load_2d(pb + i * kMmBoxBytes, &tmap_b, n * kMmTileN + i * 64, row0 + kb * kMmTileK, bar);
-                    } else {
-                        tma_load_2d(pa, &tmap_a, kb * kMmTileK, row0 + m * kMmTileM, bar);
-                        if (MODE == kMmForward) {
-                            tma_load_3d(pb, &tmap_b, kb * kMmTileK, n * kMmTileN, e, bar);
+                    const int st = int(it % kStages);
+                    if (!wait_or_abort(&ctl->empty[st], ((it / kStages) & 1u) ^ 1u, abort_flag, a.status)) break;
+                    unsigned char* pa = sA + st * kStage;
+                    unsigned char* pb = pa + kMmABytes;
+                    const int k0 = kb * kMmTileK;
+                    if (CG == 1) {
+                        uint64_t* bar = &ctl->full[st];
+                        mbar_arrive_expect_tx(bar, kStage);
+                        if (MODE == kMmWgrad) {
+                            for (int i = 0; i < kMmTileM / 64; ++i)
+                                tma_load_2d(pa + i * kMmBoxBytes, &tmap_a, a0 + i * 64, row0 + k0, bar);
+                            for (int i = 0; i < GEO::kBCols / 64; ++i)
+                                tma_load_2d(pb + i * kMmBoxBytes, &tmap_b, b0 + i * 64, row0 + k0, bar);
                         } else {
-                            for (int i = 0; i < kMmTileN / 64; ++i)
-                                tma_load_3d(pb + i * kMmBoxBytes, &tmap_b, n * kMmTileN + i * 64, kb * kMmTileK, e, bar);
+                            tma_load_2d(pa, &tmap_a, k0, row0 + a0, bar);
+                            if (MODE == kMmForward) {
+                                tma_load_3d(pb, &tmap_b, k0, b0, e, bar);
+                            } else {
+                                for (int i = 0; i < GEO::kBCols / 64; ++i)
+                                    tma_load_3d(pb + i * kMmBoxBytes, &tmap_b, b0 + i * 64, k0, e, bar);
+                            }
+                        }
+                    } else {
+                        // Both CTAs' bytes land on the leader's barrier.
+                        const uint32_t bar = leader_full0 + uint32_t(st) * 8u;
+                        if (crank == 0) mbar_arrive_expect_tx(&ctl->full[st], 2 * kStage);
+                        tma_load_2d_pair(pa, &tmap_a, k0, row0 + a0, bar);
+                        if (MODE == kMmForward) {
+                            tma_load_3d_pair(pb, &tmap_b, k0, b0, e, bar);
+                        } else {
+                            for (int i = 0; i < GEO::kBCols / 64; ++i)
+                                tma_load_3d_pair(pb + i * kMmBoxBytes, &tmap_b, b0 + i * 64, k0, e, bar);
                         }
                     }
                 }
             }
             __syncwarp();
         }
-        if (lane == 0 && *abort_flag) drain_stages(ctl->full, it, kMmStages);
+        // (the pair's loads complete on the leader's barriers; the last cluster
+        // barrier keeps the peer resident until the leader has drained them)
+        if (lane == 0 && crank == 0 && *abort_flag) drain_stages(ctl->full, it, kStages);
     } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
+        // ---------------- MMA issuer (the pair's leader) ----------------
         // Bits 15 / 16 of the instruction descriptor: A / B is MN-major.
-        const uint32_t idesc = umma_idesc_mn(DT == MOE_B200_BF16 ? 1 : 0, kMmTileM, kMmTileN) |
+        const uint32_t idesc = umma_idesc_mn(DT == MOE_B200_BF16 ? 1 : 0, GEO::kBlockRows, kMmTileN) |
                                (MODE == kMmWgrad ? 1u << 15 : 0u) | (MODE != kMmForward ? 1u << 16 : 0u);
-        constexpr uint32_t a_step = MODE == kMmWgrad ? 2048 : 32;  // bytes per 16 reduced indices
-        constexpr uint32_t b_step = MODE != kMmForward ? 2048 : 32;
-        uint32_t it = 0, j = 0;
-        bool ok = true;
+        // Descriptor steps (16-byte units) per 16 reduced indices and per stage.
+        constexpr uint32_t a_step = (MODE == kMmWgrad ? 2048 : 32) >> 4, b_step = (MODE != kMmForward ? 2048 : 32) >> 4;
+        constexpr uint32_t stage_step = kStage >> 4;
+        const uint64_t adesc0 = MODE == kMmWgrad ? umma_desc_mn_sw128(smem_u32(sA)) : umma_desc_sw128(smem_u32(sA));
+        const uint64_t bdesc0 = MODE != kMmForward ? umma_desc_mn_sw128(smem_u32(sA) + kMmABytes)
+                                                   : umma_desc_sw128(smem_u32(sA) + kMmABytes);
+        int st = 0;
+        uint32_t phase = 0, j = 0;
+        bool ok = crank == 0;
+        auto issue = [&](uint32_t d_tmem, int kk, uint32_t acc) {
+            const uint64_t ad = adesc0 + uint32_t(st) * stage_step + uint32_t(kk) * a_step;
+            const uint64_t bd = bdesc0 + uint32_t(st) * stage_step + uint32_t(kk) * b_step;
+            if (CG == 1) umma_f16(d_tmem, ad, bd, idesc, acc);
+            else umma_f16_pair(d_tmem, ad, bd, idesc, acc);
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (CG == 1) umma_commit(bar);
+            else umma_commit_both(bar);
+        };
+        auto next_stage = [&]() {
+            if (++st == kStages) st = 0, phase ^= 1;
+        };
         for (int tile = first_tile; ok && tile >= 0; tile = next_tile(tile)) {
             int s, m, n;
             const int nk = locate(tile, s, m, n);
             if (nk == 0) continue;  // an empty segment: the epilogue writes zeros
             const int buf = int(j & 1u);
-            ok = __all_sync(0xffffffffu, wait_or_abort(&ctl->tmem_empty[buf], ((j >> 1) & 1u) ^ 1u, abort_flag, a.status));
-            ++j;
-            tc_fence_after();
+            const int rem = MODE == kMmWgrad ? s_rows[s] % kMmTileK : 0;  // rows of a last, partial step
+            const int nfull = nk - (rem > 0 ? 1 : 0);
             const uint32_t d_tmem = tmem + uint32_t(buf) * kMmTileN;
-            for (int kb = 0; ok && kb < nk; ++kb, ++it) {
-                const int st = int(it % kMmStages);
-                ok = __all_sync(0xffffffffu, wait_or_abort(&ctl->full[st], (it / kMmStages) & 1u, abort_flag, a.status));
-                if (!ok) break;
-                const uint32_t a_addr = smem_u32(sA + st * kMmABytes), b_addr = smem_u32(sB + st * kMmBBytes);
-                int k16 = kMmTileK / 16;
-                if (MODE == kMmWgrad) {
-                    const int rem = s_rows[s] - kb * kMmTileK;
-                    if (rem < kMmTileK) {
-                        k16 = (rem + 15) / 16;
-                        // rows [rem, 16 * k16) of the 6 boxes: 128 bytes each, 8 lanes a row
-                        const int clear = k16 * 16 - rem;
-                        for (int i = lane; i < clear * 8 * 6; i += 32) {
-                            const int box = i / (clear * 8), r = (i >> 3) % clear, c = i & 7;
-                            const uint32_t at = (box < 2 ? a_addr + box * kMmBoxBytes : b_addr + (box - 2) * kMmBoxBytes) +
-                                                (rem + r) * 128 + c * 16;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                        }
+            if (lane == 0) {
+                ok = wait_or_abort(&ctl->tmem_empty[buf], ((j >> 1) & 1u) ^ 1u, abort_flag, a.status);
+                tc_fence_after();
+                for (int kb = 0; ok && kb < nfull; ++kb) {
+                    ok = wait_or_abort(&ctl->full[st], phase, abort_flag, a.status);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < kMmTileK / 16; ++kk) issue(d_tmem, kk, (kb | kk) != 0 ? 1u : 0u);
+                    commit(&ctl->empty[st]);
+                    next_stage();
+                }
+            }
+            ++j;
+            if (MODE == kMmWgrad) {
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                st = __shfl_sync(0xffffffffu, st, 0);
+                phase = __shfl_sync(0xffffffffu, phase, 0);
+                if (ok && rem > 0) {
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&ctl->full[st], phase, abort_flag, a.status));
+                    if (ok) {
+                        const int k16 = (rem + 15) / 16;
+                        clear_rows(smem_u32(sA) + st * kStage, int(kStage / kMmBoxBytes), rem, k16 * 16, lane);
                         fence_proxy_async_smem();
                         __syncwarp();
+                        tc_fence_after();
+                        if (lane == 0) {
+                            for (int kk = 0; kk < k16; ++kk) issue(d_tmem, kk, (nfull | kk) != 0 ? 1u : 0u);
+                            commit(&ctl->empty[st]);
+                        }
+                        next_stage();
                     }
                 }
-                tc_fence_after();
-                if (lane == 0) {
-                    for (int kk = 0; kk < k16; ++kk) {
-                        const uint64_t ad = MODE == kMmWgrad ? umma_desc_mn_sw128(a_addr + kk * a_step)
-                                                             : umma_desc_sw128(a_addr + kk * a_step);
-                        const uint64_t bd = MODE != kMmForward ? umma_desc_mn_sw128(b_addr + kk * b_step)
-                                                               : umma_desc_sw128(b_addr + kk * b_step);
-                        umma_f16(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-                    }
-                    umma_commit(&ctl->empty[st]);
-                    if (kb == nk - 1) umma_commit(&ctl->tmem_full[buf]);
-                }
-                __syncwarp();
             }
+            if (lane == 0 && ok) commit(&ctl->tmem_full[buf]);
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         }
     } else if (warp < 6) {
         // ---------------- epilogue (warps 2..5) ----------------
         const int quad = warp & 3;  // TMEM lanes 32*quad .. 32*quad+31
         unsigned char* stg = s_stage + quad * kWarpStageBytes;
+        const uint32_t leader_tmem_empty0 = CG == 2 ? map_to_rank(&ctl->tmem_empty[0], 0) : 0u;
         uint32_t j = 0;
         for (int tile = first_tile; tile >= 0; tile = next_tile(tile)) {
             int s, m, n;
             const int nk = locate(tile, s, m, n);
-            const int w_row0 = m * kMmTileM + quad * 32;
+            const int w_row0 = m * GEO::kBlockRows + int(crank) * kMmTileM + quad * 32;
             const int nrows_w = (MODE == kMmWgrad ? a.m_out : s_rows[s]) - w_row0;
             const int64_t out_row = (MODE == kMmWgrad ? int64_t(s) * a.m_out : int64_t(s_start[s])) + w_row0;
             uint16_t* dst = a.out + out_row * a.n_out;
@@ -350,7 +453,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const uint32_t t_row = tmem + uint32_t(buf) * kMmTileN + (uint32_t(quad * 32) << 16);
 #pragma unroll 1
             for (int c = 0; c < kMmTileN; c += 64) {
-                if (n * kMmTileN + c >= a.n_out) break;
+                if (n * kMmTileN + c >= a.n_out || nrows_w <= 0) break;
                 uint32_t v[4][16];
                 if (nk > 0) {
 #pragma unroll
@@ -376,22 +479,39 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             if (nk > 0) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->tmem_empty[buf]);
+                if (lane == 0) {
+                    if (CG == 1) mbar_arrive(&ctl->tmem_empty[buf]);
+                    else mbar_arrive_cluster(leader_tmem_empty0 + uint32_t(buf) * 8u);
+                }
             }
         }
     } else if (kDynamic) {
         // ---------------- tile scheduler (warp 6) ----------------
-        // Fills the answer slots ahead of the other warps and stops after the
+        // Keeps the slots filled ahead of the other warps and stops after the
         // first answer that names no CTA.
         int tile = first_tile;
+        uint32_t asked = 0;
         while (tile >= 0) {
             const int slot = int(sidx % kSchedSlots);
-            const bool ok =
-                wait_or_abort(&ctl->sched_empty[slot], ((sidx / kSchedSlots) & 1u) ^ 1u, abort_flag, a.status);
+            bool ok = wait_or_abort(&ctl->sched_empty[slot], ((sidx / kSchedSlots) & 1u) ^ 1u, abort_flag, a.status);
             if (!__all_sync(0xffffffffu, ok)) break;
             if (lane == 0) {
-                mbar_arrive_expect_tx(&ctl->sched_full[slot], 16);
-                clc_try_cancel(&ctl->sched[slot], &ctl->sched_full[slot]);
+                mbar_arrive_expect_tx(&ctl->clc_full, 16);
+                clc_try_cancel(&ctl->clc, &ctl->clc_full);
+            }
+            __syncwarp();
+            ok = wait_or_abort(&ctl->clc_full, asked & 1u, abort_flag, a.status);
+            if (!__all_sync(0xffffffffu, ok)) {
+                mbar_wait(&ctl->clc_full, asked & 1u);  // the answer still in flight has landed
+                break;
+            }
+            ++asked;
+            const int next = clc_result(&ctl->clc);
+            fence_proxy_async_smem();  // the answer is read before the next one is written
+            __syncwarp();
+            if (lane == 0) {
+                *const_cast<volatile int*>(&ctl->next[slot]) = next;
+                mbar_arrive(&ctl->sched_full[slot]);
             }
             __syncwarp();
             tile = next_tile(tile);
@@ -400,10 +520,16 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync();  // no CTA leaves while its pair may still signal it
     tc_fence_after();
     if (warp == 1) {
         __syncwarp();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMmTmemCols) : "memory");
+        if (CG == 1)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMmTmemCols)
+                         : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMmTmemCols)
+                         : "memory");
     }
 }
 
@@ -430,22 +556,63 @@ static int sm_count_mm() {
     return n > 0 ? n : 148;
 }
 
-template <int MODE, int DT>
-static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, cudaStream_t s) {
-    auto kern = grouped_mm_kernel<MODE, DT>;
-    const size_t smem = 1024 + size_t(kMmStages) * (kMmABytes + kMmBBytes) + kStageBytes + sizeof(MmSmem) +
-                        size_t(4 * a.nseg + 1) * 4;
+template <int MODE, int DT, int CG>
+static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArgs a, cudaStream_t s) {
+    auto kern = grouped_mm_kernel<MODE, DT, CG>;
+    const size_t smem = 1024 + size_t(MmGeo<CG>::kStages) * (kMmABytes + MmGeo<CG>::kBBytes) + kStageBytes +
+                        sizeof(MmSmem) + size_t(4 * a.nseg + 1) * 4;
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (err != cudaSuccess) return err;
-    int64_t grid;
-    if (MODE == kMmWgrad) {
-        grid = int64_t(a.nseg) * a.m_blocks * a.n_blocks;
-    } else {
-        grid = (int64_t(a.rows) / kMmTileM + a.nseg) * a.n_blocks;  // each segment may add one partial block
-        if (grid > sm_count_mm()) grid = sm_count_mm();
+    a.m_blocks = (a.m_out + MmGeo<CG>::kBlockRows - 1) / MmGeo<CG>::kBlockRows;
+    cudaLaunchConfig_t cfg = pdl_config(dim3(1), dim3(kMmThreads), smem, s);
+    cudaLaunchAttribute attr[1];
+    if (CG == 2) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
     }
-    kern<<<unsigned(grid), kMmThreads, smem, s>>>(ma, mb, a);
-    return cudaGetLastError();
+    int64_t groups;
+    if (MODE == kMmWgrad) {
+        groups = int64_t(a.nseg) * a.m_blocks * a.n_blocks;
+    } else {
+        groups = (int64_t(a.rows) / MmGeo<CG>::kBlockRows + a.nseg) * a.n_blocks;  // a segment may add one partial block
+        int fit = sm_count_mm() / CG;
+        if (CG == 2) {  // not every SM has a partner: a pair left waiting would run its share behind all others
+            static std::atomic<int> pairs{0};
+            int n = pairs.load(std::memory_order_relaxed);
+            if (n == 0) {
+                cfg.gridDim = dim3(unsigned(2 * fit));
+                if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) n = fit;
+                cudaGetLastError();
+                pairs.store(n, std::memory_order_relaxed);
+            }
+            if (n < fit) fit = n;
+        }
+        if (groups > fit) groups = fit;
+    }
+    cfg.gridDim = dim3(unsigned(CG * groups));
+    return cudaLaunchKernelEx(&cfg, kern, ma, mb, a);
+}
+
+template <int MODE>
+static cudaError_t launch_mm_as(int dtype, int cg, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a,
+                                cudaStream_t s) {
+    if constexpr (MODE != kMmWgrad) {
+        if (cg == 2)
+            return dtype == MOE_B200_BF16 ? launch_mm<MODE, MOE_B200_BF16, 2>(ma, mb, a, s)
+                                          : launch_mm<MODE, MOE_B200_F16, 2>(ma, mb, a, s);
+    }
+    return dtype == MOE_B200_BF16 ? launch_mm<MODE, MOE_B200_BF16, 1>(ma, mb, a, s)
+                                  : launch_mm<MODE, MOE_B200_F16, 1>(ma, mb, a, s);
+}
+
+// SM pairs, where 256-row tiles waste little: segments of 512 rows on average
+// (forward, dgrad).
+static int mm_cta_group(int mode, int rows, int nseg) {
+    return mode != kMmWgrad && rows >= 512 * int64_t(nseg) ? 2 : 1;
 }
 
 static int grouped_mm_impl(const char* who, int mode, const void* pa, const void* pb, const int32_t* seg_start,
@@ -475,8 +642,8 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     a.n_blocks = (wide + kMmTileN - 1) / kMmTileN;
     a.kdim = mode == kMmForward ? K : N;
     a.m_out = N;
-    a.m_blocks = (N + kMmTileM - 1) / kMmTileM;
-    if ((int64_t(rows) / kMmTileM + nseg) * a.n_blocks > INT32_MAX || int64_t(nseg) * a.m_blocks * a.n_blocks > INT32_MAX)
+    const int64_t most_m = (int64_t(N) + kMmTileM - 1) / kMmTileM;
+    if ((int64_t(rows) / kMmTileM + nseg) * a.n_blocks > INT32_MAX || nseg * most_m * a.n_blocks > INT32_MAX)
         return fail(MOE_B200_ERR_UNSUPPORTED, "%s: too many tiles", who);
     if (rows == 0) {  // wgrad: sums over no row
         const cudaError_t err = cudaMemsetAsync(out, 0, size_t(nseg) * size_t(N) * size_t(K) * 2, s);
@@ -484,22 +651,18 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     }
     a.status = device_status_word();
     if (!a.status) return fail(MOE_B200_ERR_CUDA, "%s: device status word unavailable", who);
+    const int cg = mm_cta_group(mode, rows, nseg);
     CUtensorMap ma, mb;
     bool ok;
     if (mode == kMmWgrad)
         ok = make_map(&ma, pa, rows, N, kMmTileK, dtype) && make_map(&mb, pb, rows, K, kMmTileK, dtype);
     else
         ok = make_map(&ma, pa, rows, a.kdim, kMmTileM, dtype) &&
-             make_map_experts(&mb, pb, E, N, K, mode == kMmForward ? kMmTileN : kMmTileK, dtype);
+             make_map_experts(&mb, pb, E, N, K, mode == kMmForward ? kMmTileN / cg : kMmTileK, dtype);
     if (!ok) return fail(MOE_B200_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
-    const bool bf = dtype == MOE_B200_BF16;
-    cudaError_t err;
-    if (mode == kMmForward)
-        err = bf ? launch_mm<kMmForward, MOE_B200_BF16>(ma, mb, a, s) : launch_mm<kMmForward, MOE_B200_F16>(ma, mb, a, s);
-    else if (mode == kMmDgrad)
-        err = bf ? launch_mm<kMmDgrad, MOE_B200_BF16>(ma, mb, a, s) : launch_mm<kMmDgrad, MOE_B200_F16>(ma, mb, a, s);
-    else
-        err = bf ? launch_mm<kMmWgrad, MOE_B200_BF16>(ma, mb, a, s) : launch_mm<kMmWgrad, MOE_B200_F16>(ma, mb, a, s);
+    const cudaError_t err = mode == kMmForward ? launch_mm_as<kMmForward>(dtype, cg, ma, mb, a, s)
+                            : mode == kMmDgrad ? launch_mm_as<kMmDgrad>(dtype, cg, ma, mb, a, s)
+                                               : launch_mm_as<kMmWgrad>(dtype, cg, ma, mb, a, s);
     return err == cudaSuccess ? MOE_B200_OK : cuda_fail(err, who);
 }
 
