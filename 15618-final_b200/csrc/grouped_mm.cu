@@ -16,13 +16,17 @@
 //
 // One CTA per SM, 7 warps: TMA producer, MMA issuer, 4 epilogue warps (TMEM
 // accumulator double-buffered, so the epilogue of one tile runs under the MMAs
-// of the next), tile scheduler.  Two forms share the code:
-//   CG=1  one SM per 128 x 256 tile, 48 KB a K step, 4 stages: for short
-//         segments, where a taller tile would be half empty
-//   CG=2  an SM pair (cluster of 2) per 256 x 256 tile: each CTA stages its 128
-//         rows of A and half of B, 32 KB a K step, 6 stages.  One SM cannot
-//         feed its tensor core at full rate (48 KB are written to and read from
-//         shared memory per 512 cycles); a pair can.
+// of the next), tile scheduler.  Three forms share the code:
+//   few     one SM per 32 x 128 tile: for segments of a few rows, where the time
+//           is that of reading the weights; only 32 rows of A are loaded (the
+//           MMA's other 96 rows are whatever lies behind them and are not
+//           read back), and narrow tiles spread over the SMs evenly
+//   single  one SM per 128 x 256 tile, 48 KB a K step, 4 stages: for short
+//           segments, where a taller tile would be half empty
+//   pair    an SM pair (cluster of 2) per 256 x 256 tile: each CTA stages its
+//           128 rows of A and half of B, 32 KB a K step, 6 stages.  One SM
+//           cannot feed its tensor core at full rate (48 KB are written to and
+//           read from shared memory per 512 cycles); a pair can.
 // Forward and dgrad tiles cost the same, and a persistent grid deals them
 // round-robin.  A wgrad tile costs as much as its segment has rows; there the
 // grid is one CTA (pair) per tile and running ones take over waiting ones
@@ -55,22 +59,26 @@ int cuda_fail(cudaError_t err, const char* where);
 
 enum { kMmForward = 0, kMmDgrad = 1, kMmWgrad = 2 };
 
-constexpr int kMmTileM = 128;  // rows of A per CTA
-constexpr int kMmTileN = 256;
 constexpr int kMmTileK = 64;
 constexpr int kMmThreads = 7 * 32;
-constexpr uint32_t kMmABytes = kMmTileM * kMmTileK * 2;  // 16 KB
 constexpr uint32_t kMmBoxBytes = 64 * 64 * 2;            // one MN-major box: 64 columns x 64 reduced rows
 constexpr uint32_t kMmTmemCols = 512;
+constexpr int kMmBufCols = 256;                          // TMEM columns of one accumulator
 constexpr int kMmMaxSegments = 1024;
-constexpr int kSchedSlots = 2;
-template <int CG> struct MmGeo {
-    static constexpr int kBlockRows = kMmTileM * CG;          // rows per tile
-    static constexpr int kBCols = kMmTileN / CG;              // columns of B a CTA holds
+constexpr int kSchedSlots = 4;
+enum { kMmFew = 0, kMmSingle = 1, kMmPair = 2 };
+template <int FORM> struct MmGeo {
+    static constexpr int kCtas = FORM == kMmPair ? 2 : 1;
+    static constexpr int kTileM = FORM == kMmFew ? 32 : 128;  // rows of A per CTA
+    static constexpr int kTileN = FORM == kMmFew ? 128 : 256;
+    static constexpr int kBlockRows = kTileM * kCtas;         // rows per tile
+    static constexpr int kBCols = kTileN / kCtas;             // columns of B a CTA holds
+    static constexpr uint32_t kABytes = kTileM * kMmTileK * 2;
     static constexpr uint32_t kBBytes = kBCols * kMmTileK * 2;
-    static constexpr int kStages = CG == 1 ? 4 : 6;           // 192 KB either way
+    static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = FORM == kMmFew ? 9 : FORM == kMmSingle ? 4 : 6;  // 180 or 192 KB
 };
-constexpr int kMmMaxStages = 6;
+constexpr int kMmMaxStages = 9;
 
 struct MmSmem {
     uint64_t full[kMmMaxStages];
@@ -92,8 +100,8 @@ struct MmArgs {
     const int32_t* seg_expert;
     int nseg, rows;
     int kdim;      // reduced length (forward, dgrad)
-    int m_blocks;  // wgrad: 128-row blocks of dw
-    int n_blocks;  // 256-column blocks of the output
+    int m_blocks;  // wgrad: row blocks of dw
+    int n_blocks;  // column blocks of the output
     int m_out;     // wgrad: rows of dw per expert
     int n_out;     // output columns
     uint16_t* out;
@@ -177,19 +185,18 @@ __device__ __forceinline__ void clear_rows(uint32_t base, int boxes, int from, i
     }
 }
 
-template <int MODE, int DT, int CG>
+template <int MODE, int DT, int FORM>
 __global__ void __launch_bounds__(kMmThreads, 1)
 grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                   const MmArgs a) {
     constexpr bool kDynamic = MODE == kMmWgrad;
-    using GEO = MmGeo<CG>;
-    constexpr int kStages = GEO::kStages;
-    constexpr uint32_t kBBytes = GEO::kBBytes;
+    using GEO = MmGeo<FORM>;
+    constexpr int CG = GEO::kCtas, kStages = GEO::kStages, kMmTileN = GEO::kTileN;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* sA = base;  // [stages][A, B]: B follows A, so a stage's boxes are consecutive
-    constexpr uint32_t kStage = kMmABytes + kBBytes;
+    constexpr uint32_t kStage = GEO::kStageBytes;
     unsigned char* s_stage = base + kStages * kStage;
     MmSmem* ctl = reinterpret_cast<MmSmem*>(s_stage + kStageBytes);
     int32_t* blk_prefix = reinterpret_cast<int32_t*>(ctl + 1);  // [nseg + 1] row blocks before a segment
@@ -314,19 +321,19 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const int nk = locate(tile, s, m, n);
             if (lane == 0) {
                 const int e = s_exp[s], row0 = s_start[s];
-                const int a0 = m * GEO::kBlockRows + int(crank) * kMmTileM;    // rows of A (wgrad: columns of dy)
+                const int a0 = m * GEO::kBlockRows + int(crank) * GEO::kTileM;    // rows of A (wgrad: columns of dy)
                 const int b0 = n * kMmTileN + int(crank) * GEO::kBCols;        // columns of the output
                 for (int kb = 0; kb < nk; ++kb, ++it) {
                     const int st = int(it % kStages);
                     if (!wait_or_abort(&ctl->empty[st], ((it / kStages) & 1u) ^ 1u, abort_flag, a.status)) break;
                     unsigned char* pa = sA + st * kStage;
-                    unsigned char* pb = pa + kMmABytes;
+                    unsigned char* pb = pa + GEO::kABytes;
                     const int k0 = kb * kMmTileK;
                     if (CG == 1) {
                         uint64_t* bar = &ctl->full[st];
                         mbar_arrive_expect_tx(bar, kStage);
                         if (MODE == kMmWgrad) {
-                            for (int i = 0; i < kMmTileM / 64; ++i)
+                            for (int i = 0; i < GEO::kTileM / 64; ++i)
                                 tma_load_2d(pa + i * kMmBoxBytes, &tmap_a, a0 + i * 64, row0 + k0, bar);
                             for (int i = 0; i < GEO::kBCols / 64; ++i)
                                 tma_load_2d(pb + i * kMmBoxBytes, &tmap_b, b0 + i * 64, row0 + k0, bar);
@@ -361,14 +368,14 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     } else if (warp == 1) {
         // ---------------- MMA issuer (the pair's leader) ----------------
         // Bits 15 / 16 of the instruction descriptor: A / B is MN-major.
-        const uint32_t idesc = umma_idesc_mn(DT == MOE_B200_BF16 ? 1 : 0, GEO::kBlockRows, kMmTileN) |
+        const uint32_t idesc = umma_idesc_mn(DT == MOE_B200_BF16 ? 1 : 0, 128 * CG, kMmTileN) |
                                (MODE == kMmWgrad ? 1u << 15 : 0u) | (MODE != kMmForward ? 1u << 16 : 0u);
         // Descriptor steps (16-byte units) per 16 reduced indices and per stage.
         constexpr uint32_t a_step = (MODE == kMmWgrad ? 2048 : 32) >> 4, b_step = (MODE != kMmForward ? 2048 : 32) >> 4;
         constexpr uint32_t stage_step = kStage >> 4;
         const uint64_t adesc0 = MODE == kMmWgrad ? umma_desc_mn_sw128(smem_u32(sA)) : umma_desc_sw128(smem_u32(sA));
-        const uint64_t bdesc0 = MODE != kMmForward ? umma_desc_mn_sw128(smem_u32(sA) + kMmABytes)
-                                                   : umma_desc_sw128(smem_u32(sA) + kMmABytes);
+        const uint64_t bdesc0 = MODE != kMmForward ? umma_desc_mn_sw128(smem_u32(sA) + GEO::kABytes)
+                                                   : umma_desc_sw128(smem_u32(sA) + GEO::kABytes);
         int st = 0;
         uint32_t phase = 0, j = 0;
         bool ok = crank == 0;
@@ -392,7 +399,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const int buf = int(j & 1u);
             const int rem = MODE == kMmWgrad ? s_rows[s] % kMmTileK : 0;  // rows of a last, partial step
             const int nfull = nk - (rem > 0 ? 1 : 0);
-            const uint32_t d_tmem = tmem + uint32_t(buf) * kMmTileN;
+            const uint32_t d_tmem = tmem + uint32_t(buf) * kMmBufCols;
             if (lane == 0) {
                 ok = wait_or_abort(&ctl->tmem_empty[buf], ((j >> 1) & 1u) ^ 1u, abort_flag, a.status);
                 tc_fence_after();
@@ -439,7 +446,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         for (int tile = first_tile; tile >= 0; tile = next_tile(tile)) {
             int s, m, n;
             const int nk = locate(tile, s, m, n);
-            const int w_row0 = m * GEO::kBlockRows + int(crank) * kMmTileM + quad * 32;
+            const int w_row0 = m * GEO::kBlockRows + int(crank) * GEO::kTileM + quad * 32;
             const int nrows_w = (MODE == kMmWgrad ? a.m_out : s_rows[s]) - w_row0;
             const int64_t out_row = (MODE == kMmWgrad ? int64_t(s) * a.m_out : int64_t(s_start[s])) + w_row0;
             uint16_t* dst = a.out + out_row * a.n_out;
@@ -450,7 +457,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 ++j;
                 tc_fence_after();
             }
-            const uint32_t t_row = tmem + uint32_t(buf) * kMmTileN + (uint32_t(quad * 32) << 16);
+            const uint32_t t_row = tmem + uint32_t(buf) * kMmBufCols + (uint32_t(quad * 32) << 16);
 #pragma unroll 1
             for (int c = 0; c < kMmTileN; c += 64) {
                 if (n * kMmTileN + c >= a.n_out || nrows_w <= 0) break;
@@ -556,14 +563,17 @@ static int sm_count_mm() {
     return n > 0 ? n : 148;
 }
 
-template <int MODE, int DT, int CG>
+template <int MODE, int DT, int FORM>
 static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArgs a, cudaStream_t s) {
-    auto kern = grouped_mm_kernel<MODE, DT, CG>;
-    const size_t smem = 1024 + size_t(MmGeo<CG>::kStages) * (kMmABytes + MmGeo<CG>::kBBytes) + kStageBytes +
-                        sizeof(MmSmem) + size_t(4 * a.nseg + 1) * 4;
+    using GEO = MmGeo<FORM>;
+    constexpr int CG = GEO::kCtas;
+    auto kern = grouped_mm_kernel<MODE, DT, FORM>;
+    const size_t smem = 1024 + size_t(GEO::kStages) * GEO::kStageBytes + kStageBytes + sizeof(MmSmem) +
+                        size_t(4 * a.nseg + 1) * 4;
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (err != cudaSuccess) return err;
-    a.m_blocks = (a.m_out + MmGeo<CG>::kBlockRows - 1) / MmGeo<CG>::kBlockRows;
+    a.m_blocks = (a.m_out + GEO::kBlockRows - 1) / GEO::kBlockRows;
+    a.n_blocks = (a.n_out + GEO::kTileN - 1) / GEO::kTileN;
     cudaLaunchConfig_t cfg = pdl_config(dim3(1), dim3(kMmThreads), smem, s);
     cudaLaunchAttribute attr[1];
     if (CG == 2) {
@@ -578,7 +588,7 @@ static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArg
     if (MODE == kMmWgrad) {
         groups = int64_t(a.nseg) * a.m_blocks * a.n_blocks;
     } else {
-        groups = (int64_t(a.rows) / MmGeo<CG>::kBlockRows + a.nseg) * a.n_blocks;  // a segment may add one partial block
+        groups = (int64_t(a.rows) / GEO::kBlockRows + a.nseg) * a.n_blocks;  // a segment may add one partial block
         int fit = sm_count_mm() / CG;
         if (CG == 2) {  // not every SM has a partner: a pair left waiting would run its share behind all others
             static std::atomic<int> pairs{0};
@@ -598,21 +608,33 @@ static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArg
 }
 
 template <int MODE>
-static cudaError_t launch_mm_as(int dtype, int cg, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a,
+static cudaError_t launch_mm_as(int dtype, int form, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a,
                                 cudaStream_t s) {
+    const bool bf = dtype == MOE_B200_BF16;
     if constexpr (MODE != kMmWgrad) {
-        if (cg == 2)
-            return dtype == MOE_B200_BF16 ? launch_mm<MODE, MOE_B200_BF16, 2>(ma, mb, a, s)
-                                          : launch_mm<MODE, MOE_B200_F16, 2>(ma, mb, a, s);
+        if (form == kMmPair)
+            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmPair>(ma, mb, a, s)
+                      : launch_mm<MODE, MOE_B200_F16, kMmPair>(ma, mb, a, s);
+        if (form == kMmFew)
+            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmFew>(ma, mb, a, s)
+                      : launch_mm<MODE, MOE_B200_F16, kMmFew>(ma, mb, a, s);
     }
-    return dtype == MOE_B200_BF16 ? launch_mm<MODE, MOE_B200_BF16, 1>(ma, mb, a, s)
-                                  : launch_mm<MODE, MOE_B200_F16, 1>(ma, mb, a, s);
+    return bf ? launch_mm<MODE, MOE_B200_BF16, kMmSingle>(ma, mb, a, s)
+              : launch_mm<MODE, MOE_B200_F16, kMmSingle>(ma, mb, a, s);
 }
 
-// SM pairs, where 256-row tiles waste little: segments of 512 rows on average
-// (forward, dgrad).
-static int mm_cta_group(int mode, int rows, int nseg) {
-    return mode != kMmWgrad && rows >= 512 * int64_t(nseg) ? 2 : 1;
+// Rows a tile loads and columns of its B that a CTA loads.
+static int form_rows(int form) { return form == kMmFew ? MmGeo<kMmFew>::kTileM : MmGeo<kMmSingle>::kTileM; }
+static int form_cols(int form) {
+    return form == kMmFew ? MmGeo<kMmFew>::kBCols : form == kMmPair ? MmGeo<kMmPair>::kBCols : MmGeo<kMmSingle>::kBCols;
+}
+
+// Forward and dgrad by the rows a segment has on average: 512 and more fill
+// pair tiles (at most an eighth of a last, half-empty one is lost); up to 16
+// fit the small tiles also when they are spread unevenly.
+static int mm_form(int mode, int rows, int nseg) {
+    if (mode == kMmWgrad) return kMmSingle;
+    return rows >= 512 * int64_t(nseg) ? kMmPair : rows <= 16 * int64_t(nseg) ? kMmFew : kMmSingle;
 }
 
 static int grouped_mm_impl(const char* who, int mode, const void* pa, const void* pb, const int32_t* seg_start,
@@ -639,11 +661,10 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     a.out = static_cast<uint16_t*>(out);
     const int wide = mode == kMmForward ? N : K;  // output columns
     a.n_out = wide;
-    a.n_blocks = (wide + kMmTileN - 1) / kMmTileN;
     a.kdim = mode == kMmForward ? K : N;
     a.m_out = N;
-    const int64_t most_m = (int64_t(N) + kMmTileM - 1) / kMmTileM;
-    if ((int64_t(rows) / kMmTileM + nseg) * a.n_blocks > INT32_MAX || nseg * most_m * a.n_blocks > INT32_MAX)
+    const int64_t n_most = (int64_t(wide) + 127) / 128, m_most = (int64_t(N) + 127) / 128;  // of the smallest tiles
+    if ((int64_t(rows) / 32 + nseg) * n_most > INT32_MAX || nseg * m_most * n_most > INT32_MAX)
         return fail(MOE_B200_ERR_UNSUPPORTED, "%s: too many tiles", who);
     if (rows == 0) {  // wgrad: sums over no row
         const cudaError_t err = cudaMemsetAsync(out, 0, size_t(nseg) * size_t(N) * size_t(K) * 2, s);
@@ -651,18 +672,18 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     }
     a.status = device_status_word();
     if (!a.status) return fail(MOE_B200_ERR_CUDA, "%s: device status word unavailable", who);
-    const int cg = mm_cta_group(mode, rows, nseg);
+    const int form = mm_form(mode, rows, nseg);
     CUtensorMap ma, mb;
     bool ok;
     if (mode == kMmWgrad)
         ok = make_map(&ma, pa, rows, N, kMmTileK, dtype) && make_map(&mb, pb, rows, K, kMmTileK, dtype);
     else
-        ok = make_map(&ma, pa, rows, a.kdim, kMmTileM, dtype) &&
-             make_map_experts(&mb, pb, E, N, K, mode == kMmForward ? kMmTileN / cg : kMmTileK, dtype);
+        ok = make_map(&ma, pa, rows, a.kdim, form_rows(form), dtype) &&
+             make_map_experts(&mb, pb, E, N, K, mode == kMmForward ? form_cols(form) : kMmTileK, dtype);
     if (!ok) return fail(MOE_B200_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
-    const cudaError_t err = mode == kMmForward ? launch_mm_as<kMmForward>(dtype, cg, ma, mb, a, s)
-                            : mode == kMmDgrad ? launch_mm_as<kMmDgrad>(dtype, cg, ma, mb, a, s)
-                                               : launch_mm_as<kMmWgrad>(dtype, cg, ma, mb, a, s);
+    const cudaError_t err = mode == kMmForward ? launch_mm_as<kMmForward>(dtype, form, ma, mb, a, s)
+                            : mode == kMmDgrad ? launch_mm_as<kMmDgrad>(dtype, form, ma, mb, a, s)
+                                               : launch_mm_as<kMmWgrad>(dtype, form, ma, mb, a, s);
     return err == cudaSuccess ? MOE_B200_OK : cuda_fail(err, who);
 }
 
