@@ -23,9 +23,10 @@ EPS = 1e-6
 
 
 def _mb():
-    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "15618-final_b200")
-    if "moe_b200" not in sys.modules and root not in sys.path:
-        sys.path.insert(0, root)
+    if "moe_b200" not in sys.modules:
+        root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "15618-final_b200")
+        if root not in sys.path:
+            sys.path.insert(0, root)
     import moe_b200
     return moe_b200
 
