@@ -717,12 +717,6 @@ block_norm_columns_kernel(const float* __restrict__ part, int nparts, int d, flo
 
 // ----------------------------------------------------------------- host ----
 
-static int sm_count_norm() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n > 0 ? n : 148;
-}
-
 // Smallest power of two >= 32 of threads that covers d with V chunks of 8.
 static int row_threads_for(int d, int v) {
     int nt = 32;
@@ -754,7 +748,7 @@ static NormGradPlan plan_norm_backward(int T, int d) {
     p.cta_threads = p.row_threads == 32 ? 128 : p.row_threads;
     const int groups = p.cta_threads / p.row_threads;
     const int64_t need = (int64_t(T) + groups - 1) / groups;
-    const int64_t fit = int64_t(sm_count_norm()) * (512 / p.cta_threads);
+    const int64_t fit = int64_t(device_sm_count()) * (512 / p.cta_threads);
     p.grid = int(need < fit ? need : fit);
     if (p.grid < 1) p.grid = 1;
     return p;
@@ -779,8 +773,10 @@ static int check_norm(const char* who, int T, int d, int dtype, int gate_form, c
 template <int DT, bool RES32, bool AL, bool RING, bool WARP, int MAXT, int FORM>
 static cudaError_t launch_norm_as(NormArgs a, int cta, int64_t grid, size_t smem, cudaStream_t s) {
     auto kern = block_norm_kernel<DT, RES32, AL, RING, WARP, 2, MAXT, FORM>;
-    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (err != cudaSuccess) return err;
+    if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
+        const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (err != cudaSuccess) return err;
+    }
     kern<<<unsigned(grid), cta, smem, s>>>(a);
     return cudaGetLastError();
 }
@@ -798,7 +794,7 @@ static cudaError_t launch_norm(const NormArgs& a0, cudaStream_t s) {
     NormArgs a = a0;
     const int nt = row_threads_for(a.d, 2), cta = nt == 32 ? 128 : nt, groups = cta / nt;
     const int per_sm = cta <= 256 ? 768 / cta : 1024 / cta;  // what the registers allow
-    const int64_t need = (int64_t(a.T) + groups - 1) / groups, most = int64_t(sm_count_norm()) * per_sm;
+    const int64_t need = (int64_t(a.T) + groups - 1) / groups, most = int64_t(device_sm_count()) * per_sm;
     if constexpr (AL) {
         a.off_y = a.d * (RES32 ? 4 : 2);
         a.off_gate = a.off_y + (a.y ? a.d * 2 : 0);

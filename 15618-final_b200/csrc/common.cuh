@@ -192,6 +192,7 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 }
 
 uint32_t* device_status_word();  // status.cu
+int device_sm_count();                  // status.cu: SMs of the current device (148 if it cannot be asked)
 
 // ------------------------------------------- expert-parallel flag words ----
 // System-scope acquire / release on epoch words that other GPUs read or write

@@ -449,12 +449,6 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
 
 // ----------------------------------------------------------------- host ----
 
-static int sm_count_w4() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n > 0 ? n : 148;
-}
-
 // Shared memory of a CTA and its layout; xs: with x staged.
 static size_t w4_layout(W4Args& a, int nt, bool xs) {
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
@@ -482,7 +476,7 @@ static cudaError_t launch_w4(const CUtensorMap& map, W4Args a, dim3 grid, cudaSt
 template <int DT, int G>
 static cudaError_t run_w4(const CUtensorMap& map, W4Args a, cudaStream_t s) {
     const int served = a.slots < a.E ? a.slots : a.E;  // experts that may have work
-    int64_t grid = 2 * sm_count_w4();
+    int64_t grid = 2 * device_sm_count();
     // Warps that share a tile's k: few, as each joint costs about as much as a
     // step, but so that every CTA gets several units, and none that loses more
     // than an eighth of its steps to an uneven split.

@@ -557,12 +557,6 @@ static bool make_map_experts(CUtensorMap* map, const void* base, int64_t experts
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int sm_count_mm() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n > 0 ? n : 148;
-}
-
 template <int MODE, int DT, int FORM>
 static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArgs a, cudaStream_t s) {
     using GEO = MmGeo<FORM>;
@@ -589,7 +583,7 @@ static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArg
         groups = int64_t(a.nseg) * a.m_blocks * a.n_blocks;
     } else {
         groups = (int64_t(a.rows) / GEO::kBlockRows + a.nseg) * a.n_blocks;  // a segment may add one partial block
-        int fit = sm_count_mm() / CG;
+        int fit = device_sm_count() / CG;
         if (CG == 2) {  // not every SM has a partner: a pair left waiting would run its share behind all others
             static std::atomic<int> pairs{0};
             int n = pairs.load(std::memory_order_relaxed);

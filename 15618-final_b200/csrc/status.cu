@@ -2,6 +2,7 @@
 // without a caller workspace (unpermute, grouped FFN).  Kernels OR
 // MOE_B200_DEV_* bits into it instead of trapping; moe_b200_device_status()
 // reads and clears it.
+#include <atomic>
 #include <mutex>
 
 #include <cuda_runtime.h>
@@ -33,6 +34,18 @@ uint32_t* device_status_word() {
         g_addr[dev] = static_cast<uint32_t*>(p);
     }
     return g_addr[dev];
+}
+
+int device_sm_count() {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+    n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 }  // namespace moe_b200
 

@@ -496,13 +496,11 @@ def _rows(what, name, t, shape, dtype, strided=False):
 
 
 def _same_device(what, *tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        _refuse(what, f"tensors must be on a CUDA device, got {dev}")
+    index = tensors[0].get_device()  # -1: the CPU
     for t in tensors:
-        if t is not None and t.device != dev:
-            _refuse(what, f"tensors on {dev} and {t.device}")
-    return dev
+        if t is not None and (t.get_device() != index or index < 0):
+            _refuse(what, f"tensors must be on one CUDA device, got {tensors[0].device} and {t.device}")
+    return tensors[0].device
 
 
 def _enqueue(what, fn, dev, stream, fresh, *args):
@@ -560,21 +558,33 @@ class BlockNormGrads(NamedTuple):
     d_gate: object
 
 
-def _check_block_norm(what, residual, y, w_post, w_pre, gate, dtype):
+def _check_block_norm(what, residual, y, w_post, w_pre, gate):
+    """The checks both directions share: (T, d, dtype, its code, fp32 residual, gate form)."""
     import torch
-    T, d = residual.shape
-    dtype_code(dtype)
-    if residual.dtype not in (dtype, torch.float32):
-        _refuse(what, f"residual must be {dtype} or float32, got {residual.dtype}")
-    _rows(what, "residual", residual, (T, d), residual.dtype, strided=True)
-    if y is None and (w_post is not None or gate is not None):
-        _refuse(what, "w_post and gate need y")
+    if residual.dim() != 2:
+        _refuse(what, "the residual must be [T, d]")
+    some = y if y is not None else w_pre
+    if some is None:
+        _refuse(what, "nothing to do without y and w_pre")
+    dtype = some.dtype
+    code = BF16 if dtype == torch.bfloat16 else dtype_code(dtype)
+    shape = residual.shape
+    T, d = shape
+    res_dtype = residual.dtype
+    res32 = res_dtype == torch.float32
+    if not res32 and res_dtype != dtype:
+        _refuse(what, f"the residual must be {dtype} or float32, got {res_dtype}")
+    if not residual.is_contiguous():
+        _rows(what, "the residual", residual, shape, res_dtype, strided=True)
     if y is not None:
-        _rows(what, "y", y, (T, d), dtype, strided=True)
-    for name, w in (("w_post", w_post), ("w_pre", w_pre)):
-        if w is not None:
-            _rows(what, name, w, (d,), dtype)
-    return T, d
+        _rows(what, "y", y, shape, dtype, strided=True)
+        if w_post is not None:
+            _rows(what, "w_post", w_post, (d,), dtype)
+    elif w_post is not None or gate is not None:
+        _refuse(what, "w_post and gate need y")
+    if w_pre is not None:
+        _rows(what, "w_pre", w_pre, (d,), dtype)
+    return T, d, dtype, code, int(res32), GATE_NONE if gate is None else _gate_form(what, gate, T, d, dtype)
 
 
 def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, eps=1e-6, out=None, stream=None):
@@ -585,20 +595,13 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
     the residual), gate [T, 1], [1, d] / [d] or [T, d].  residual and y may be
     row-strided.  out: a BlockNormResult of contiguous tensors to write."""
     import torch
-    if residual.dim() != 2:
-        _refuse("block_norm", "residual must be [T, d]")
-    some = y if y is not None else w_pre
-    if some is None:
-        _refuse("block_norm", "nothing to do without y and w_pre")
-    dtype = some.dtype
-    T, d = _check_block_norm("block_norm", residual, y, w_post, w_pre, gate, dtype)
-    form = _gate_form("block_norm", gate, T, d, dtype)
+    T, d, dtype, code, res32, form = _check_block_norm("block_norm", residual, y, w_post, w_pre, gate)
     dev = _same_device("block_norm", residual, y, w_post, w_pre, gate)
     fresh = ()
     if out is None:
         fresh = out = BlockNormResult(
             residual_out=torch.empty_like(residual, memory_format=torch.contiguous_format) if y is not None else None,
-            normed=torch.empty_like(some if some is y else residual, dtype=dtype, memory_format=torch.contiguous_format)
+            normed=torch.empty_like(residual, dtype=dtype, memory_format=torch.contiguous_format)
             if w_pre is not None else None)
     else:
         if (out.residual_out is None) != (y is None) or (out.normed is None) != (w_pre is None):
@@ -612,8 +615,8 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
         return out if y is not None else BlockNormResult(residual, out.normed)
     _enqueue("block_norm", lib().moe_b200_block_norm, dev, stream, fresh,
              _ptr(y), _row_stride(y) if y is not None else 0, _ptr(residual), _row_stride(residual),
-             int(residual.dtype == torch.float32), _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d,
-             dtype_code(dtype), _ptr(out.residual_out), _ptr(out.normed))
+             res32, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d, code, _ptr(out.residual_out),
+             _ptr(out.normed))
     return out if y is not None else BlockNormResult(residual, out.normed)
 
 
@@ -626,14 +629,7 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     16-bit [T, d]."""
     import torch
     what = "block_norm_backward"
-    if residual_out.dim() != 2:
-        _refuse(what, "residual_out must be [T, d]")
-    some = y if y is not None else w_pre
-    if some is None:
-        _refuse(what, "nothing to do without y and w_pre")
-    dtype = some.dtype
-    T, d = _check_block_norm(what, residual_out, y, w_post, w_pre, gate, dtype)
-    form = _gate_form(what, gate, T, d, dtype)
+    T, d, dtype, code, res32, form = _check_block_norm(what, residual_out, y, w_post, w_pre, gate)
     if (d_normed is None) != (w_pre is None):
         _refuse(what, "d_normed and w_pre go together")
     if d_residual_out is None and w_pre is None:
@@ -643,7 +639,6 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     if d_normed is not None:
         _rows(what, "d_normed", d_normed, (T, d), dtype)
     dev = _same_device(what, residual_out, d_residual_out, d_normed, y, w_post, w_pre, gate)
-    res32 = int(residual_out.dtype == torch.float32)
     nbytes = int(lib().moe_b200_block_norm_backward_workspace_bytes(T, d, res32))
 
     def empty(shape, dt):
@@ -665,7 +660,7 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream, (*got, ws),
              _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), _row_stride(residual_out), res32, _ptr(y),
              _row_stride(y) if y is not None else 0, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d,
-             dtype_code(dtype), _ptr(got.d_residual), _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre),
+             code, _ptr(got.d_residual), _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre),
              _ptr(got.d_gate), _ptr(ws), ws.numel())
     return got
 
