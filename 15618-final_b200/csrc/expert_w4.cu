@@ -138,84 +138,131 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ uint64_t s_full[kW4Warps][kW4Stages];
     constexpr int kGroups = kW4Block / G;  // groups of a row per step
-    int* s_cnt = reinterpret_cast<int*>(smem + a.s_tab);  // [E] slots of an expert
-    int* s_first = s_cnt + a.E;                           // [E] its first place in s_slots
-    int* s_unit = s_first + a.E;                          // [E + 1] units of the experts before
-    int* s_cur = s_unit + a.E + 1;                        // [8][E] next place, by warp
+    int* s_expert = reinterpret_cast<int*>(smem + a.s_tab);  // [entries] experts served (or all of them)
+    int* s_cnt = s_expert + a.E;                             // [entries] slots of an expert
+    int* s_first = s_cnt + a.E;                              // [entries] its first place in s_slots
+    int* s_unit = s_first + a.E;                             // [entries + 1] units of the experts before
+    int* s_cur = s_unit + a.E + 1;                           // [8][E] next place, by warp
     uint16_t* s_slots = reinterpret_cast<uint16_t*>(s_cur + kW4Warps * a.E);  // [slots] by expert, ascending
+    __shared__ int s_entries, s_none;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
 
     // Slots by expert, ascending within an expert (every CTA has to find the
-    // same order: CTAs share an expert's slots by their places in it).  Each
-    // warp counts and deals one stretch of the slots.
-    const int part = ((a.slots + kW4Threads - 1) / kW4Threads) * 32;
-    const int s_lo = warp * part, s_hi = min(s_lo + part, a.slots);
-    for (int i = threadIdx.x; i < kW4Warps * a.E; i += kW4Threads) s_cur[i] = 0;
-    __syncthreads();
+    // same order: CTAs share an expert's slots by their places in it).
     bool none = false;
-    for (int s = s_lo + lane; s < s_hi; s += 32) {
-        const int e = a.asgn[s];
-        if (e >= 0 && e < a.E) atomicAdd(&s_cur[warp * a.E + e], 1);
-        else if (e != -1 && blockIdx.x == 0) atomicOr(a.status, MOE_B200_DEV_BAD_ASSIGNMENT);
-        none |= e < 0 || e >= a.E;
-    }
-    none = __syncthreads_or(none);
-    if (warp == 0) {
-        int rows = 0, units = 0;
-        for (int e0 = 0; e0 < a.E; e0 += 32) {
-            const int e = e0 + lane;
-            int c = 0;
-            if (e < a.E)
-                for (int w = 0; w < kW4Warps; ++w) c += s_cur[w * a.E + e];
-            int r = c, u = (c + NT * 8 - 1) / (NT * 8) * a.units;
+    if (a.slots <= 32) {
+        // One warp, a lane per slot; the experts in the order of their first slots.
+        if (warp == 0) {
+            const int e = lane < a.slots ? a.asgn[lane] : -1;
+            const bool ok = e >= 0 && e < a.E;
+            if (lane < a.slots && !ok && e != -1 && blockIdx.x == 0) atomicOr(a.status, MOE_B200_DEV_BAD_ASSIGNMENT);
+            const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1), lt = lanemask_lt();
+            const bool leads = ok && (same & lt) == 0;
+            const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+            const int c = leads ? __popc(same) : 0, u = (c + NT * 8 - 1) / (NT * 8) * a.units;
+            int rows = c, units = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int rv = __shfl_up_sync(0xffffffffu, r, o), uv = __shfl_up_sync(0xffffffffu, u, o);
-                if (lane >= o) r += rv, u += uv;
+                const int rv = __shfl_up_sync(0xffffffffu, rows, o), uv = __shfl_up_sync(0xffffffffu, units, o);
+                if (lane >= o) rows += rv, units += uv;
             }
-            if (e < a.E) {
-                s_cnt[e] = c;
-                int at = rows + r - c;
-                s_first[e] = at;
+            const int first = __shfl_sync(0xffffffffu, rows - c, __ffs(same) - 1);
+            if (leads) {
+                const int i = __popc(leaders & lt);
+                s_expert[i] = e;
+                s_cnt[i] = c;
+                s_first[i] = rows - c;
+                s_unit[i + 1] = units;
+            }
+            if (ok) s_slots[first + __popc(same & lt)] = uint16_t(lane);
+            none = __any_sync(0xffffffffu, lane < a.slots && !ok);
+            if (lane == 0) {
+                s_unit[0] = 0;
+                s_entries = __popc(leaders);
+                s_none = none;
+            }
+        }
+        __syncthreads();
+    } else {
+        // Each warp counts and deals one stretch of the slots.
+        const int part = ((a.slots + kW4Threads - 1) / kW4Threads) * 32;
+        const int s_lo = warp * part, s_hi = min(s_lo + part, a.slots);
+        const int first_e = s_lo + lane < s_hi ? a.asgn[s_lo + lane] : -1;
+        for (int i = threadIdx.x; i < kW4Warps * a.E; i += kW4Threads) s_cur[i] = 0;
+        __syncthreads();
+        for (int s = s_lo + lane; s < s_hi; s += 32) {
+            const int e = s == s_lo + lane ? first_e : a.asgn[s];
+            if (e >= 0 && e < a.E) atomicAdd(&s_cur[warp * a.E + e], 1);
+            else if (e != -1 && blockIdx.x == 0) atomicOr(a.status, MOE_B200_DEV_BAD_ASSIGNMENT);
+            none |= e < 0 || e >= a.E;
+        }
+        none = __syncthreads_or(none);
+        if (warp == 0) {
+            int rows = 0, units = 0;
+            for (int e0 = 0; e0 < a.E; e0 += 32) {
+                const int e = e0 + lane;
+                int n[kW4Warps], c = 0;
+#pragma unroll
                 for (int w = 0; w < kW4Warps; ++w) {
-                    const int n = s_cur[w * a.E + e];
-                    s_cur[w * a.E + e] = at;
-                    at += n;
+                    n[w] = e < a.E ? s_cur[w * a.E + e] : 0;
+                    c += n[w];
                 }
-                s_unit[e + 1] = units + u;
+                int r = c, u = (c + NT * 8 - 1) / (NT * 8) * a.units;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int rv = __shfl_up_sync(0xffffffffu, r, o), uv = __shfl_up_sync(0xffffffffu, u, o);
+                    if (lane >= o) r += rv, u += uv;
+                }
+                if (e < a.E) {
+                    s_expert[e] = e;
+                    s_cnt[e] = c;
+                    int at = rows + r - c;
+                    s_first[e] = at;
+#pragma unroll
+                    for (int w = 0; w < kW4Warps; ++w) {
+                        s_cur[w * a.E + e] = at;
+                        at += n[w];
+                    }
+                    s_unit[e + 1] = units + u;
+                }
+                rows += __shfl_sync(0xffffffffu, r, 31);
+                units += __shfl_sync(0xffffffffu, u, 31);
             }
-            rows += __shfl_sync(0xffffffffu, r, 31);
-            units += __shfl_sync(0xffffffffu, u, 31);
+            if (lane == 0) {
+                s_unit[0] = 0;
+                s_entries = a.E;
+                s_none = none;
+            }
         }
-        if (lane == 0) s_unit[0] = 0;
-    }
-    __syncthreads();
-    for (int s0 = s_lo; s0 < s_hi; s0 += 32) {
-        const int s = s0 + lane;
-        const int e = s < s_hi ? a.asgn[s] : -1;
-        const bool ok = e >= 0 && e < a.E;
-        const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
-        int base = 0;
-        if (ok) base = s_cur[warp * a.E + e];
-        __syncwarp();
-        if (ok) {
-            s_slots[base + __popc(same & lanemask_lt())] = uint16_t(s);
-            if ((same & lanemask_lt()) == 0) s_cur[warp * a.E + e] = base + __popc(same);
+        __syncthreads();
+        for (int s0 = s_lo; s0 < s_hi; s0 += 32) {
+            const int s = s0 + lane;
+            const int e = s0 == s_lo ? first_e : s < s_hi ? a.asgn[s] : -1;
+            const bool ok = e >= 0 && e < a.E;
+            const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
+            int base = 0;
+            if (ok) base = s_cur[warp * a.E + e];
+            __syncwarp();
+            if (ok) {
+                s_slots[base + __popc(same & lanemask_lt())] = uint16_t(s);
+                if ((same & lanemask_lt()) == 0) s_cur[warp * a.E + e] = base + __popc(same);
+            }
+            __syncwarp();
         }
-        __syncwarp();
+        __syncthreads();
     }
+    const int entries = s_entries;
     // Slots without an expert get rows of zeros, dealt over the grid.
-    for (int s = blockIdx.x; none && s < a.slots; s += gridDim.x) {
+    for (int s = blockIdx.x; s_none && s < a.slots; s += gridDim.x) {
         const int e = a.asgn[s];
         if (e >= 0 && e < a.E) continue;
         for (int c = threadIdx.x; c < a.n_out; c += kW4Threads)
             static_cast<uint16_t*>(a.out)[int64_t(s) * a.n_out + c] = 0;
     }
-    __syncthreads();
 
     // This CTA's even share of all units.
-    const int total = s_unit[a.E], share = total / int(gridDim.x), more = total - share * int(gridDim.x);
+    const int total = s_unit[entries], share = total / int(gridDim.x), more = total - share * int(gridDim.x);
     const int u_begin = share * int(blockIdx.x) + min(int(blockIdx.x), more);
     const int u_end = u_begin + share + (int(blockIdx.x) < more ? 1 : 0);
     if (u_begin >= u_end) return;
@@ -225,12 +272,12 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
     const int my_blocks = blocks > kw ? (blocks - kw + wk - 1) / wk : 0;
     const int ngroups = a.K / G;
 
-    // A place in the walk over units: expert, unit of its current pass, pass.
+    // A place in the walk over units: entry and its expert, unit of its current pass, pass.
     struct Place {
-        int u, e, tg, pass;
+        int u, i, e, tg, pass;
     };
-    auto expert_of = [&](int u) {  // last expert with s_unit[e] <= u
-        int lo = 0, hi = a.E - 1;
+    auto entry_of = [&](int u) {  // last entry with s_unit[i] <= u
+        int lo = 0, hi = entries - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (s_unit[mid] <= u) lo = mid;
@@ -241,8 +288,9 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
     auto place_at = [&](int u) {
         Place p;
         p.u = u;
-        p.e = expert_of(u);
-        const int local = u - s_unit[p.e];
+        p.i = entry_of(u);
+        p.e = s_expert[p.i];
+        const int local = u - s_unit[p.i];
         p.pass = local / a.units;
         p.tg = local - p.pass * a.units;
         return p;
@@ -252,8 +300,9 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
         if (++p.tg < a.units) return;
         p.tg = 0;
         ++p.pass;
-        if (p.u >= s_unit[p.e + 1] && p.u < u_end) {
-            p.e = expert_of(p.u);
+        if (p.u < u_end && p.u >= s_unit[p.i + 1]) {
+            p.i = entry_of(p.u);
+            p.e = s_expert[p.i];
             p.pass = 0;
         }
     };
@@ -305,8 +354,8 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
         advance(next);
         if (at.e != staged_e || at.pass != staged_pass) {
             staged_e = at.e, staged_pass = at.pass;
-            const int cnt = s_cnt[at.e];
-            list0 = s_first[at.e] + at.pass * NT * 8;
+            const int cnt = s_cnt[at.i];
+            list0 = s_first[at.i] + at.pass * NT * 8;
             nrows = min(cnt - at.pass * NT * 8, NT * 8);
             nt = (nrows + 7) >> 3;
             if (XS) {  // zeros past K; columns of the product past the last row are not written
@@ -459,7 +508,7 @@ static size_t w4_layout(W4Args& a, int nt, bool xs) {
     a.s_red = int(off);
     off += size_t(kW4Warps) * 2 * nt * 128 * 4;
     a.s_tab = int(off);
-    off += size_t((3 + kW4Warps) * a.E + 1) * 4 + ((size_t(a.slots) * 2 + 15) & ~size_t(15));
+    off += size_t((4 + kW4Warps) * a.E + 1) * 4 + ((size_t(a.slots) * 2 + 15) & ~size_t(15));
     return off;
 }
 

@@ -536,12 +536,12 @@ def _gate_form(what, gate, T, d, dtype):
     if gate.dtype != dtype or not gate.is_contiguous():
         _refuse(what, f"gate must be contiguous {dtype}")
     shape = tuple(gate.shape)
-    if shape == (T, d):
-        return GATE_FULL
-    if shape == (T, 1):
+    if shape == (T, 1):  # a shape that broadcasts counts as broadcast, also where it is [T, d]
         return GATE_TOKEN
     if shape in ((1, d), (d,)):
         return GATE_CHANNEL
+    if shape == (T, d):
+        return GATE_FULL
     _refuse(what, f"gate must be ({T}, 1), (1, {d}), ({d},) or ({T}, {d}), got {shape}")
 
 
