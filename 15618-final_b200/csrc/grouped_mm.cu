@@ -174,6 +174,14 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
         : "memory");
 }
 
+// Tiled TMA store of a staged box; its elements past the tensor's bounds are not written.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(z), "r"(smem_u32(smem_src))
+                 : "memory");
+}
+
 // Clears the reduced rows [from, to), 128 bytes each, of `boxes` MN-major boxes at `base`, by one warp.
 __device__ __forceinline__ void clear_rows(uint32_t base, int boxes, int from, int to, int lane) {
     const int n = to - from;
@@ -188,7 +196,7 @@ __device__ __forceinline__ void clear_rows(uint32_t base, int boxes, int from, i
 template <int MODE, int DT, int FORM>
 __global__ void __launch_bounds__(kMmThreads, 1)
 grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                  const MmArgs a) {
+                  const __grid_constant__ CUtensorMap tmap_c, const MmArgs a) {
     constexpr bool kDynamic = MODE == kMmWgrad;
     using GEO = MmGeo<FORM>;
     constexpr int CG = GEO::kCtas, kStages = GEO::kStages, kMmTileN = GEO::kTileN;
@@ -229,6 +237,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         mbar_fence_init();
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
+        prefetch_tmap(&tmap_c);
     }
     if (warp == 0) {
         // Offsets are held inside [0, rows], so that no bad table leads a store outside the output.
@@ -450,6 +459,11 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const int nrows_w = (MODE == kMmWgrad ? a.m_out : s_rows[s]) - w_row0;
             const int64_t out_row = (MODE == kMmWgrad ? int64_t(s) * a.m_out : int64_t(s_start[s])) + w_row0;
             uint16_t* dst = a.out + out_row * a.n_out;
+            // The staged 32 x 64 piece has the layout of a 128-byte-swizzled TMA
+            // box: one store instruction writes it.  Only a segment's last rows
+            // (forward, dgrad), behind which other segments' rows lie, are
+            // written by the lanes; dw ends with its tensor map.
+            const bool by_tma = MODE == kMmWgrad || nrows_w >= 32;
             const int buf = int(j & 1u);
             if (nk > 0) {
                 const bool ok = wait_or_abort(&ctl->tmem_full[buf], (j >> 1) & 1u, abort_flag, a.status);
@@ -472,6 +486,8 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #pragma unroll
                         for (int q = 0; q < 16; ++q) v[q4][q] = 0;
                 }
+                if (lane == 0) bulk_wait_read<0>();  // the piece before is read
+                __syncwarp();
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
                     uint32_t o[8];
@@ -481,7 +497,17 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                     stage_put(stg, lane, 2 * q4, make_uint4(o[0], o[1], o[2], o[3]));
                     stage_put(stg, lane, 2 * q4 + 1, make_uint4(o[4], o[5], o[6], o[7]));
                 }
-                stage_flush(stg, lane, dst, a.n_out, nrows_w, n * kMmTileN + c, a.n_out, nullptr);
+                if (by_tma) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&tmap_c, stg, n * kMmTileN + c, MODE == kMmWgrad ? w_row0 : int(out_row),
+                                     MODE == kMmWgrad ? s : 0);
+                        bulk_commit();
+                    }
+                } else {
+                    stage_flush(stg, lane, dst, a.n_out, nrows_w, n * kMmTileN + c, a.n_out, nullptr);
+                }
             }
             if (nk > 0) {
                 tc_fence_before();
@@ -492,6 +518,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 }
             }
         }
+        if (lane == 0) bulk_wait<0>();
     } else if (kDynamic) {
         // ---------------- tile scheduler (warp 6) ----------------
         // Keeps the slots filled ahead of the other warps and stops after the
@@ -558,7 +585,8 @@ static bool make_map_experts(CUtensorMap* map, const void* base, int64_t experts
 }
 
 template <int MODE, int DT, int FORM>
-static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArgs a, cudaStream_t s) {
+static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, MmArgs a,
+                             cudaStream_t s) {
     using GEO = MmGeo<FORM>;
     constexpr int CG = GEO::kCtas;
     auto kern = grouped_mm_kernel<MODE, DT, FORM>;
@@ -598,23 +626,23 @@ static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, MmArg
         if (groups > fit) groups = fit;
     }
     cfg.gridDim = dim3(unsigned(CG * groups));
-    return cudaLaunchKernelEx(&cfg, kern, ma, mb, a);
+    return cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, a);
 }
 
 template <int MODE>
-static cudaError_t launch_mm_as(int dtype, int form, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a,
-                                cudaStream_t s) {
+static cudaError_t launch_mm_as(int dtype, int form, const CUtensorMap& ma, const CUtensorMap& mb,
+                                const CUtensorMap& mc, const MmArgs& a, cudaStream_t s) {
     const bool bf = dtype == MOE_B200_BF16;
     if constexpr (MODE != kMmWgrad) {
         if (form == kMmPair)
-            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmPair>(ma, mb, a, s)
-                      : launch_mm<MODE, MOE_B200_F16, kMmPair>(ma, mb, a, s);
+            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmPair>(ma, mb, mc, a, s)
+                      : launch_mm<MODE, MOE_B200_F16, kMmPair>(ma, mb, mc, a, s);
         if (form == kMmFew)
-            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmFew>(ma, mb, a, s)
-                      : launch_mm<MODE, MOE_B200_F16, kMmFew>(ma, mb, a, s);
+            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmFew>(ma, mb, mc, a, s)
+                      : launch_mm<MODE, MOE_B200_F16, kMmFew>(ma, mb, mc, a, s);
     }
-    return bf ? launch_mm<MODE, MOE_B200_BF16, kMmSingle>(ma, mb, a, s)
-              : launch_mm<MODE, MOE_B200_F16, kMmSingle>(ma, mb, a, s);
+    return bf ? launch_mm<MODE, MOE_B200_BF16, kMmSingle>(ma, mb, mc, a, s)
+              : launch_mm<MODE, MOE_B200_F16, kMmSingle>(ma, mb, mc, a, s);
 }
 
 // Rows a tile loads and columns of its B that a CTA loads.
@@ -667,17 +695,18 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     a.status = device_status_word();
     if (!a.status) return fail(MOE_B200_ERR_CUDA, "%s: device status word unavailable", who);
     const int form = mm_form(mode, rows, nseg);
-    CUtensorMap ma, mb;
-    bool ok;
+    CUtensorMap ma, mb, mc;
+    bool ok = mode == kMmWgrad ? make_map_experts(&mc, out, nseg, N, K, 32, dtype)
+                               : make_map_experts(&mc, out, 1, rows, wide, 32, dtype);
     if (mode == kMmWgrad)
-        ok = make_map(&ma, pa, rows, N, kMmTileK, dtype) && make_map(&mb, pb, rows, K, kMmTileK, dtype);
+        ok = ok && make_map(&ma, pa, rows, N, kMmTileK, dtype) && make_map(&mb, pb, rows, K, kMmTileK, dtype);
     else
-        ok = make_map(&ma, pa, rows, a.kdim, form_rows(form), dtype) &&
+        ok = ok && make_map(&ma, pa, rows, a.kdim, form_rows(form), dtype) &&
              make_map_experts(&mb, pb, E, N, K, mode == kMmForward ? form_cols(form) : kMmTileK, dtype);
     if (!ok) return fail(MOE_B200_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
-    const cudaError_t err = mode == kMmForward ? launch_mm_as<kMmForward>(dtype, form, ma, mb, a, s)
-                            : mode == kMmDgrad ? launch_mm_as<kMmDgrad>(dtype, form, ma, mb, a, s)
-                                               : launch_mm_as<kMmWgrad>(dtype, form, ma, mb, a, s);
+    const cudaError_t err = mode == kMmForward ? launch_mm_as<kMmForward>(dtype, form, ma, mb, mc, a, s)
+                            : mode == kMmDgrad ? launch_mm_as<kMmDgrad>(dtype, form, ma, mb, mc, a, s)
+                                               : launch_mm_as<kMmWgrad>(dtype, form, ma, mb, mc, a, s);
     return err == cudaSuccess ? MOE_B200_OK : cuda_fail(err, who);
 }
 
