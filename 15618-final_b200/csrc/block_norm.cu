@@ -703,7 +703,7 @@ block_norm_columns_kernel(const float* __restrict__ part, int nparts, int d, flo
     const float* p = part + int64_t(blockIdx.y) * nparts * d;
     float v = 0.f;
     if (col < d) {
-#pragma unroll 4
+#pragma unroll 8
         for (int i = warp; i < nparts; i += 32) v += p[int64_t(i) * d + col];
     }
     s[warp][lane] = v;
@@ -823,8 +823,10 @@ template <int DT, bool RES32, bool AL, bool RING, bool WARP, int V, int GATE = -
 static cudaError_t launch_norm_backward_as(const NormGradArgs& a, const NormGradPlan& p, size_t smem, cudaStream_t s) {
     constexpr int kMax = WARP ? 128 : 512;
     auto kern = block_norm_backward_kernel<DT, RES32, AL, RING, WARP, V, kMax, GATE>;
-    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (err != cudaSuccess) return err;
+    if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
+        const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (err != cudaSuccess) return err;
+    }
     kern<<<p.grid, p.cta_threads, smem, s>>>(a);
     return cudaGetLastError();
 }
@@ -925,7 +927,7 @@ extern "C" int moe_b200_block_norm(const void* y, int64_t y_stride, const void* 
     return err == cudaSuccess ? MOE_B200_OK : cuda_fail(err, "block_norm launch");
 }
 
-extern "C" size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d, int /*residual_f32*/) {
+extern "C" size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d) {
     using namespace moe_b200;
     if (T < 0 || d < 1 || d > kNormMaxD) return 0;
     return align256(size_t(3) * size_t(plan_norm_backward(T, d).grid) * size_t(d) * 4);

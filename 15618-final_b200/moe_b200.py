@@ -134,7 +134,7 @@ def lib() -> ctypes.CDLL:
     L.moe_b200_block_norm.restype = cint
     L.moe_b200_block_norm.argtypes = [vp, i64, vp, i64, cint, vp, vp, vp, cint, f32, f32, cint, cint, cint, vp, vp, vp]
     L.moe_b200_block_norm_backward_workspace_bytes.restype = sz
-    L.moe_b200_block_norm_backward_workspace_bytes.argtypes = [cint, cint, cint]
+    L.moe_b200_block_norm_backward_workspace_bytes.argtypes = [cint, cint]
     L.moe_b200_block_norm_backward.restype = cint
     L.moe_b200_block_norm_backward.argtypes = [vp, vp, vp, i64, cint, vp, i64, vp, vp, vp, cint, f32, f32, cint, cint,
                                                cint, vp, vp, vp, vp, vp, vp, sz, vp]
@@ -639,29 +639,28 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     if d_normed is not None:
         _rows(what, "d_normed", d_normed, (T, d), dtype)
     dev = _same_device(what, residual_out, d_residual_out, d_normed, y, w_post, w_pre, gate)
-    nbytes = int(lib().moe_b200_block_norm_backward_workspace_bytes(T, d, res32))
+    nbytes = int(lib().moe_b200_block_norm_backward_workspace_bytes(T, d))
 
-    def empty(shape, dt):
-        return torch.empty(shape, dtype=dt, device=dev)
-
+    like, plain = torch.empty_like, torch.contiguous_format
+    f32 = torch.float32
     got = BlockNormGrads(
-        d_residual=empty((T, d), residual_out.dtype),
-        d_y=empty((T, d), dtype) if y is not None else None,
-        d_w_post=empty((d,), torch.float32) if w_post is not None else None,
-        d_w_pre=empty((d,), torch.float32) if w_pre is not None else None,
-        d_gate=empty(gate.shape, dtype if form == GATE_FULL else torch.float32) if gate is not None else None)
+        d_residual=like(residual_out, memory_format=plain),
+        d_y=like(y, memory_format=plain) if y is not None else None,
+        d_w_post=like(w_post, dtype=f32) if w_post is not None else None,
+        d_w_pre=like(w_pre, dtype=f32) if w_pre is not None else None,
+        d_gate=None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32))
     if T == 0:  # sums over no token
         with torch.cuda.stream(stream if not isinstance(stream, int) else torch.cuda.ExternalStream(stream, device=dev)):
             for t in got[2:]:
                 if t is not None:
                     t.zero_()
         return got
-    ws = empty((max(nbytes, 256),), torch.uint8)
+    ws = residual_out.new_empty((max(nbytes, 256),), dtype=torch.uint8)
     _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream, (*got, ws),
              _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), _row_stride(residual_out), res32, _ptr(y),
              _row_stride(y) if y is not None else 0, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d,
              code, _ptr(got.d_residual), _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre),
-             _ptr(got.d_gate), _ptr(ws), ws.numel())
+             _ptr(got.d_gate), _ptr(ws), nbytes)
     return got
 
 

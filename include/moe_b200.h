@@ -408,10 +408,10 @@ int moe_b200_block_norm(const void* y, int64_t y_stride, const void* residual, i
  *   d_w_post, d_w_pre [d] fp32               (with w_post / w_pre)
  *   d_gate  fp32 [T] / fp32 [d] / 16-bit [T, d] by gate_form
  * Sums over tokens are taken in a fixed order.  workspace:
- * moe_b200_block_norm_backward_workspace_bytes(T, d, residual_f32) bytes,
+ * moe_b200_block_norm_backward_workspace_bytes(T, d) bytes (on this device),
  * 256-byte aligned, needs no initial value; concurrent calls use distinct
  * ones.                                                                     */
-size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d, int residual_f32);
+size_t moe_b200_block_norm_backward_workspace_bytes(int T, int d);
 int moe_b200_block_norm_backward(const void* d_residual_out, const void* d_normed, const void* residual_out,
                                  int64_t residual_stride, int residual_f32, const void* y, int64_t y_stride,
                                  const void* w_post, const void* w_pre, const void* gate, int gate_form, float scale,

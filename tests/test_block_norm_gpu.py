@@ -301,9 +301,9 @@ def test_c_refusals():
     assert fwd(eps=-1.0) == fwd(eps=float("nan")) == fwd(r=None) == fwd(ro=None) == fwd(no=None) == mb.ERR_INVALID_ARG
     assert fwd(y=None) == fwd(y=None, wo=None, wn=None) == fwd(rs=15) == fwd(ys=8) == mb.ERR_INVALID_ARG
     assert fwd(d=16385, rs=1 << 20, ys=1 << 20) == mb.ERR_UNSUPPORTED
-    need = L.moe_b200_block_norm_backward_workspace_bytes(4, 16, 0)
+    need = L.moe_b200_block_norm_backward_workspace_bytes(4, 16)
     assert need > 0 and need % 256 == 0
-    assert L.moe_b200_block_norm_backward_workspace_bytes(-1, 16, 0) == 0
+    assert L.moe_b200_block_norm_backward_workspace_bytes(-1, 16) == 0
 
     def bwd(dr=p, dn=p, ro=p, y=p, wo=p, wn=p, out=p, dy=p, dwo=p, dwn=p, ws=p, nb=need, T=4):
         return L.moe_b200_block_norm_backward(dr, dn, ro, 16, 0, y, 16, wo, wn, None, 0, 1.0, 1e-6, T, 16, 1, out, dy, dwo,

@@ -7,10 +7,14 @@ Tolerance: the longest way from an input to a gradient passes 10 roundings to
 linear in what was rounded before it (norms nearly so) and the roundings are
 independent of the data, so in the 2-norm the result is off by at most about
 their sum, 10 half steps; fp32 errors are far below."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import moe_b200 as mb
+from conftest import PKG
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +146,42 @@ def test_decode_step_captured_and_replayed(cuda, T):
     assert off(got.residual_out, r2) < bound
     assert off(got.normed, rms(r2, p["w2"].double(), eps)) < bound
     assert torch.equal(got.residual_out[live:], p["r"][live:])  # padding: the block adds nothing
+
+
+FIRST_CALLS = """
+import sys; sys.path.insert(0, sys.argv[1])
+import torch, moe_b200 as mb
+mb.lib()
+x = torch.randn((40, 256), device="cuda").bfloat16()
+w = torch.randn((2, 128, 256), device="cuda").bfloat16()
+one = torch.ones((256,), device="cuda").bfloat16()
+dy = torch.randn((40, 128), device="cuda").bfloat16()
+seg = torch.tensor([0, 15, 40], dtype=torch.int32, device="cuda")
+big = torch.randn((3000, 256), device="cuda").bfloat16()
+bseg = torch.tensor([0, 1500, 3000], dtype=torch.int32, device="cuda")
+asgn = torch.zeros((40, 1), dtype=torch.int32, device="cuda")
+wq = torch.randint(0, 256, (2, 64, 128), dtype=torch.uint8, device="cuda")
+ws = torch.ones((2, 64, 2), device="cuda").bfloat16()
+torch.cuda.synchronize()
+
+def calls():
+    f = mb.block_norm(big, big, one, one)
+    b = mb.block_norm_backward(big, big, big, big, one, one)
+    return [f.residual_out, f.normed, *b[:4], mb.grouped_mm(x, seg, w), mb.grouped_mm(big, bseg, w), mb.grouped_mm_dgrad(dy, seg, w),
+            mb.grouped_mm_wgrad(dy, x, seg), mb.expert_linear_w4(x, asgn, wq, ws)]
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+graph.replay()
+want = calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want)) and mb.device_status() == 0
+print("captured first")
+"""
+
+
+def test_first_calls_may_be_captured(cuda):
+    """A process whose first call of each operator is made during a capture."""
+    out = subprocess.run([sys.executable, "-c", FIRST_CALLS, PKG], capture_output=True, text=True, timeout=300)
+    assert "captured first" in out.stdout, out.stderr[-2000:]

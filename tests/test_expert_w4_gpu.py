@@ -137,6 +137,14 @@ def test_bad_rows_stay_alone(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,K,E,d", [(1024, 4, 1024, 64), (32, 1, 1024, 2048), (33, 1, 1, 256), (8, 4, 3, 128), (2048, 2, 2, 96)])
+def test_table_limits(cuda, T, K, E, d):
+    """The most slots and experts, and the border of the one-warp slot lists."""
+    check(*make(T, K, E, d, 16, 32, torch.bfloat16, zeros=True, seed=E, asgn=torch.randint(-1, E, (T, K), device="cuda", dtype=torch.int32)))
+    assert mb.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_no_tokens(cuda):
     p = make(0, 2, 3, 128, 16, 32, torch.float16)
     assert mb.expert_linear_w4(*p).shape == (0, 16)

@@ -79,6 +79,22 @@ def test_more_tiles_than_sms_and_long_sums(cuda):
 
 
 @pytest.mark.gpu
+def test_most_segments(cuda):
+    """1024 segments of 0 to 40 rows."""
+    counts = np.random.default_rng(1).integers(0, 41, size=1024)
+    check(*make(list(counts), 40, 72, torch.bfloat16, seed=6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [8, 300, 2000])
+def test_pair_single_and_few_row_forms(cuda, rows):
+    """The three tile forms on the same segments in turn (chosen by the rows a
+    segment has on average), each with one segment far from the average."""
+    check(*make([rows, 3 * rows, 1, 0, rows // 2], 264, 520, torch.float16, seed=rows))
+    check(*make([5 * rows + 3], 200, 136, torch.bfloat16, seed=rows))
+
+
+@pytest.mark.gpu
 def test_every_segment_empty(cuda):
     x, dy, w, seg = make([0, 0, 0], 64, 48, torch.bfloat16, extra=5)
     out = torch.full((5, 48), 7.0, dtype=x.dtype, device="cuda")
