@@ -40,8 +40,7 @@ namespace moe_b200 {
 int fail(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t err, const char* where);
 
-constexpr int kW4Warps = 8;
-constexpr int kW4Threads = kW4Warps * 32;
+constexpr int kW4Parts = 8;         // stretches of slots that are listed side by side
 constexpr int kW4Stages = 2;
 constexpr int kW4Block = 256;       // k per step
 constexpr int kW4TileRows = 32;     // weight rows per warp step: two 16-row operands
@@ -132,18 +131,21 @@ template <int DT> __device__ __forceinline__ uint16_t w4_to16(float f) {
 
 // XS: x is staged in shared memory; otherwise (rows too long for it) each lane
 // reads its pieces of x from global memory, where they stay in L1 / L2.
-template <int DT, int G, int NT, bool XS>
-__global__ void __launch_bounds__(kW4Threads, 2)
+// W: warps of the CTA.  With 16 rows of x a CTA fills an SM by itself, and 16
+// warps share them (147 tokens of 60 experts of 2048 x 1408: see the launch).
+template <int DT, int G, int NT, bool XS, int W>
+__global__ void __launch_bounds__(W * 32, 16 / W)
 expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ uint64_t s_full[kW4Warps][kW4Stages];
+    __shared__ uint64_t s_full[W][kW4Stages];
     constexpr int kGroups = kW4Block / G;  // groups of a row per step
+    constexpr int kThreads = W * 32;
     int* s_expert = reinterpret_cast<int*>(smem + a.s_tab);  // [entries] experts served (or all of them)
     int* s_cnt = s_expert + a.E;                             // [entries] slots of an expert
     int* s_first = s_cnt + a.E;                              // [entries] its first place in s_slots
     int* s_unit = s_first + a.E;                             // [entries + 1] units of the experts before
-    int* s_cur = s_unit + a.E + 1;                           // [8][E] next place, by warp
-    uint16_t* s_slots = reinterpret_cast<uint16_t*>(s_cur + kW4Warps * a.E);  // [slots] by expert, ascending
+    int* s_cur = s_unit + a.E + 1;                           // [kW4Parts][E] next place, by stretch
+    uint16_t* s_slots = reinterpret_cast<uint16_t*>(s_cur + kW4Parts * a.E);  // [slots] by expert, ascending
     __shared__ int s_entries, s_none;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -185,11 +187,11 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
         }
         __syncthreads();
     } else {
-        // Each warp counts and deals one stretch of the slots.
-        const int part = ((a.slots + kW4Threads - 1) / kW4Threads) * 32;
-        const int s_lo = warp * part, s_hi = min(s_lo + part, a.slots);
+        // The first warps count and deal one stretch of the slots each.
+        const int part = ((a.slots + kW4Parts * 32 - 1) / (kW4Parts * 32)) * 32;
+        const int s_lo = warp < kW4Parts ? warp * part : a.slots, s_hi = min(s_lo + part, a.slots);
         const int first_e = s_lo + lane < s_hi ? a.asgn[s_lo + lane] : -1;
-        for (int i = threadIdx.x; i < kW4Warps * a.E; i += kW4Threads) s_cur[i] = 0;
+        for (int i = threadIdx.x; i < kW4Parts * a.E; i += kThreads) s_cur[i] = 0;
         __syncthreads();
         for (int s = s_lo + lane; s < s_hi; s += 32) {
             const int e = s == s_lo + lane ? first_e : a.asgn[s];
@@ -202,9 +204,9 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
             int rows = 0, units = 0;
             for (int e0 = 0; e0 < a.E; e0 += 32) {
                 const int e = e0 + lane;
-                int n[kW4Warps], c = 0;
+                int n[kW4Parts], c = 0;
 #pragma unroll
-                for (int w = 0; w < kW4Warps; ++w) {
+                for (int w = 0; w < kW4Parts; ++w) {
                     n[w] = e < a.E ? s_cur[w * a.E + e] : 0;
                     c += n[w];
                 }
@@ -220,7 +222,7 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
                     int at = rows + r - c;
                     s_first[e] = at;
 #pragma unroll
-                    for (int w = 0; w < kW4Warps; ++w) {
+                    for (int w = 0; w < kW4Parts; ++w) {
                         s_cur[w * a.E + e] = at;
                         at += n[w];
                     }
@@ -257,7 +259,7 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
     for (int s = blockIdx.x; s_none && s < a.slots; s += gridDim.x) {
         const int e = a.asgn[s];
         if (e >= 0 && e < a.E) continue;
-        for (int c = threadIdx.x; c < a.n_out; c += kW4Threads)
+        for (int c = threadIdx.x; c < a.n_out; c += kThreads)
             static_cast<uint16_t*>(a.out)[int64_t(s) * a.n_out + c] = 0;
     }
 
@@ -267,7 +269,7 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
     const int u_end = u_begin + share + (int(blockIdx.x) < more ? 1 : 0);
     if (u_begin >= u_end) return;
 
-    const int wk = a.wk, wn_count = kW4Warps / wk, kw = warp % wk, wn = warp / wk;
+    const int wk = a.wk, wn_count = W / wk, kw = warp % wk, wn = warp / wk;
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     const int my_blocks = blocks > kw ? (blocks - kw + wk - 1) / wk : 0;
     const int ngroups = a.K / G;
@@ -360,12 +362,12 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
             nt = (nrows + 7) >> 3;
             if (XS) {  // zeros past K; columns of the product past the last row are not written
                 const int chunks = blocks * (kW4Block / 8), all = nrows * chunks;
-                for (int c0 = threadIdx.x; c0 < all; c0 += 4 * kW4Threads) {
+                for (int c0 = threadIdx.x; c0 < all; c0 += 4 * kThreads) {
                     uint4 v[4];
                     int r[4], k8[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {  // four loads in flight
-                        const int c = c0 + i * kW4Threads;
+                        const int c = c0 + i * kThreads;
                         r[i] = c / chunks, k8[i] = c - r[i] * chunks;
                         v[i] = make_uint4(0, 0, 0, 0);
                         if (c < all && k8[i] * 8 < a.K)
@@ -374,7 +376,7 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (c0 + i * kW4Threads < all)
+                        if (c0 + i * kThreads < all)
                             *reinterpret_cast<uint4*>(smem + a.s_x + r[i] * a.x_pitch + k8[i] * 16) = x_pairs(v[i]);
                 }
                 __syncthreads();
@@ -471,7 +473,7 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
                     make_float4(acc[m][q][0], acc[m][q][1], acc[m][q][2], acc[m][q][3]);
         __syncthreads();
         // A thread sums one value of (tile, q) for both m and writes them, or their SwiGLU.
-        for (int o = threadIdx.x; o < wn_count * NT * 128; o += kW4Threads) {
+        for (int o = threadIdx.x; o < wn_count * NT * 128; o += kThreads) {
             const int q = (o >> 7) % NT, w2 = (o >> 7) / NT, l = (o & 127) >> 2, j = o & 3;
             const int tl = at.tg * wn_count + w2, col = q * 8 + (l & 3) * 2 + (j & 1), rr = (l >> 2) + (j >> 1) * 8;
             if (col >= nrows || tl >= a.tiles) continue;
@@ -498,51 +500,53 @@ expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a
 
 // ----------------------------------------------------------------- host ----
 
-// Shared memory of a CTA and its layout; xs: with x staged.
-static size_t w4_layout(W4Args& a, int nt, bool xs) {
+// Shared memory of a CTA of `warps` and its layout; xs: with x staged.
+static size_t w4_layout(W4Args& a, int nt, bool xs, int warps) {
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     a.x_pitch = blocks * kW4Block * 2 + 64;  // 64 bytes off a multiple of 128: rows of a fragment on other banks
-    size_t off = size_t(kW4Warps) * kW4Stages * kW4StageBytes;
+    size_t off = size_t(warps) * kW4Stages * kW4StageBytes;
     a.s_x = int(off);
     off += xs ? size_t(nt) * 8 * a.x_pitch : 0;
     a.s_red = int(off);
-    off += size_t(kW4Warps) * 2 * nt * 128 * 4;
+    off += size_t(warps) * 2 * nt * 128 * 4;
     a.s_tab = int(off);
-    off += size_t((4 + kW4Warps) * a.E + 1) * 4 + ((size_t(a.slots) * 2 + 15) & ~size_t(15));
+    off += size_t((4 + kW4Parts) * a.E + 1) * 4 + ((size_t(a.slots) * 2 + 15) & ~size_t(15));
     return off;
 }
 
-template <int DT, int G, int NT, bool XS>
-static cudaError_t launch_w4(const CUtensorMap& map, W4Args a, dim3 grid, cudaStream_t s) {
-    const size_t smem = w4_layout(a, NT, XS);
-    auto kern = expert_linear_w4_kernel<DT, G, NT, XS>;
+template <int DT, int G, int NT, bool XS, int W>
+static cudaError_t launch_w4(const CUtensorMap& map, W4Args a, int served, cudaStream_t s) {
+    const size_t smem = w4_layout(a, NT, XS, W);
+    auto kern = expert_linear_w4_kernel<DT, G, NT, XS, W>;
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (err != cudaSuccess) return err;
-    kern<<<grid, kW4Threads, smem, s>>>(map, a);
+    int64_t grid = 16 / W * device_sm_count();
+    // Warps that share a tile's k: few, as each joint costs about as much as a
+    // step, but so that every CTA gets several units, and none that loses more
+    // than an eighth of its steps to an uneven split.
+    const int blocks = (a.K + kW4Block - 1) / kW4Block;
+    a.wk = 8;
+    while (a.wk > 1 && (8 * blocks < 7 * a.wk * ((blocks + a.wk - 1) / a.wk) ||
+                        int64_t(a.tiles) * served * a.wk > 16 * W * grid))
+        a.wk /= 2;
+    a.units = (a.tiles + W / a.wk - 1) / (W / a.wk);
+    const int64_t most = int64_t(a.units) * (a.slots < a.E ? a.slots : a.E + a.slots / 8);
+    if (grid > most) grid = most;
+    kern<<<unsigned(grid), W * 32, smem, s>>>(map, a);
     return cudaGetLastError();
 }
 
 template <int DT, int G>
 static cudaError_t run_w4(const CUtensorMap& map, W4Args a, cudaStream_t s) {
     const int served = a.slots < a.E ? a.slots : a.E;  // experts that may have work
-    int64_t grid = 2 * device_sm_count();
-    // Warps that share a tile's k: few, as each joint costs about as much as a
-    // step, but so that every CTA gets several units, and none that loses more
-    // than an eighth of its steps to an uneven split.
-    const int blocks = (a.K + kW4Block - 1) / kW4Block;
-    a.wk = kW4Warps;
-    while (a.wk > 1 && (8 * blocks < 7 * a.wk * ((blocks + a.wk - 1) / a.wk) ||
-                        int64_t(a.tiles) * served * a.wk > 2 * kW4Warps * 8 * grid))
-        a.wk /= 2;
-    a.units = (a.tiles + kW4Warps / a.wk - 1) / (kW4Warps / a.wk);
-    // Rows served per read of the weights: 8, or 16 when experts have more than that on average.
-    const bool two = a.slots > 8 * served && w4_layout(a, 2, true) <= kW4SmemLimit;
-    const bool staged = two || w4_layout(a, 1, true) <= kW4SmemLimit;
-    const int64_t most = int64_t(a.units) * (a.slots < a.E ? a.slots : a.E + a.slots / 8);
-    if (grid > most) grid = most;
-    if (two) return launch_w4<DT, G, 2, true>(map, a, dim3(unsigned(grid)), s);
-    return staged ? launch_w4<DT, G, 1, true>(map, a, dim3(unsigned(grid)), s)
-                  : launch_w4<DT, G, 1, false>(map, a, dim3(unsigned(grid)), s);
+    // Rows served per read of the weights: 8, or 16 when experts have more than
+    // 8 on average and they fit (with 16 warps where those fit too).
+    if (a.slots > 8 * served) {
+        if (w4_layout(a, 2, true, 16) <= kW4SmemLimit) return launch_w4<DT, G, 2, true, 16>(map, a, served, s);
+        if (w4_layout(a, 2, true, 8) <= kW4SmemLimit) return launch_w4<DT, G, 2, true, 8>(map, a, served, s);
+    }
+    if (w4_layout(a, 1, true, 8) <= kW4SmemLimit) return launch_w4<DT, G, 1, true, 8>(map, a, served, s);
+    return launch_w4<DT, G, 1, false, 8>(map, a, served, s);
 }
 
 // 3-D map over w_q [E, N, d/2] bytes; box = 128 bytes x 16 rows of one expert, 128B swizzle.
