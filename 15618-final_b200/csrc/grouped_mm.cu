@@ -17,10 +17,10 @@
 // One CTA per SM, 7 warps: TMA producer, MMA issuer, 4 epilogue warps (TMEM
 // accumulator double-buffered, so the epilogue of one tile runs under the MMAs
 // of the next), tile scheduler.  Three forms share the code:
-//   few     one SM per 32 x 128 tile: for segments of a few rows, where the time
-//           is that of reading the weights; only 32 rows of A are loaded (the
-//           MMA's other 96 rows are whatever lies behind them and are not
-//           read back), and narrow tiles spread over the SMs evenly
+//   few     one SM per 32 x 128 tile: for a few rows of a few experts, where the
+//           time is that of reading the weights and narrow tiles bring more
+//           SMs to it; only 32 rows of A are loaded (the MMA's other 96 rows
+//           are whatever lies behind them and are not read back)
 //   single  one SM per 128 x 256 tile, 48 KB a K step, 4 stages: for short
 //           segments, where a taller tile would be half empty
 //   pair    an SM pair (cluster of 2) per 256 x 256 tile: each CTA stages its
@@ -651,12 +651,23 @@ static int form_cols(int form) {
     return form == kMmFew ? MmGeo<kMmFew>::kBCols : form == kMmPair ? MmGeo<kMmPair>::kBCols : MmGeo<kMmSingle>::kBCols;
 }
 
-// Forward and dgrad by the rows a segment has on average: 512 and more fill
-// pair tiles (at most an eighth of a last, half-empty one is lost); up to 16
-// fit the small tiles also when they are spread unevenly.
-static int mm_form(int mode, int rows, int nseg) {
+// The form of forward and dgrad, from what the host knows (measured on one B200,
+// bf16, routing even / Zipf):
+//  few     while single tiles would be fewer than the SMs and segments have at
+//          most 16 rows on average: 4 experts of 2816 x 2048, one row each:
+//          21 us against 28; 8 experts of 1024 x 4096, 4 rows: 30 against 42.
+//          With tiles enough for all SMs it loses (60 experts, 16 rows: 125 /
+//          151 us against 120 / 118), as it does with more rows.
+//  pair    segments of 384 rows on average and two rounds of pair tiles: 60 x
+//          384 rows 282 / 287 us against 292 / 300; with 128 rows 140 / 171
+//          against 140 / 169; with one round (16 x 512 rows of 1024 x 1024) 26
+//          against 21.
+static int mm_form(int mode, int rows, int nseg, int wide) {
     if (mode == kMmWgrad) return kMmSingle;
-    return rows >= 512 * int64_t(nseg) ? kMmPair : rows <= 16 * int64_t(nseg) ? kMmFew : kMmSingle;
+    const int sms = device_sm_count();
+    const int64_t columns = (int64_t(wide) + 255) / 256;
+    if (rows <= 16 * int64_t(nseg) && (rows < nseg ? rows : nseg) * columns <= sms) return kMmFew;
+    return rows >= 384 * int64_t(nseg) && rows / 256 * columns >= sms ? kMmPair : kMmSingle;
 }
 
 static int grouped_mm_impl(const char* who, int mode, const void* pa, const void* pb, const int32_t* seg_start,
@@ -694,7 +705,7 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     }
     a.status = device_status_word();
     if (!a.status) return fail(MOE_B200_ERR_CUDA, "%s: device status word unavailable", who);
-    const int form = mm_form(mode, rows, nseg);
+    const int form = mm_form(mode, rows, nseg, wide);
     CUtensorMap ma, mb, mc;
     bool ok = mode == kMmWgrad ? make_map_experts(&mc, out, nseg, N, K, 32, dtype)
                                : make_map_experts(&mc, out, 1, rows, wide, 32, dtype);

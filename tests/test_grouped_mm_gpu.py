@@ -86,10 +86,10 @@ def test_most_segments(cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [8, 300, 2000])
+@pytest.mark.parametrize("rows", [8, 300, 2000, 9000])
 def test_pair_single_and_few_row_forms(cuda, rows):
-    """The three tile forms on the same segments in turn (chosen by the rows a
-    segment has on average), each with one segment far from the average."""
+    """The three tile forms (chosen by the rows a segment has on average and
+    the number of tiles), each with segments far from the average."""
     check(*make([rows, 3 * rows, 1, 0, rows // 2], 264, 520, torch.float16, seed=rows))
     check(*make([5 * rows + 3], 200, 136, torch.bfloat16, seed=rows))
 
