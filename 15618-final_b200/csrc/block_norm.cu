@@ -12,9 +12,23 @@
 //   dy = a * (v - yh * mean(v * yh))
 //   dw_pre = sum_t dn * c * r',  dw_post = sum_t q * yh,  dgate = scale * ds * z (summed where it was broadcast)
 //
-// Both directions are bound by memory: every row is read once into registers
-// and every result is written once; all sums are fp32, outputs are rounded
-// once (n comes from the unrounded r').
+// Both directions are bound by memory: every row is read once and every result
+// is written once; all sums are fp32, outputs are rounded once (n comes from
+// the unrounded r').
+//
+// A row belongs to a warp or to a CTA, so that its sums are one or two short
+// reductions, and a thread to fixed columns.  Rows come through a ring of
+// shared-memory stages that bulk copies fill: loads in flight cost no registers.
+// The instructions count nearly as much as the bytes (per element 4 to 7 values
+// are unpacked, and 12 to 30 fp32 operations done): conversions are packed, the
+// backward works on pairs of fp32, calls of the usual form have kernels
+// without branches.  Barriers are whole-CTA ones: a named barrier with a
+// register for its number reserves 16 of them, which left 25% occupancy.
+// Measured on one B200 (bf16, cases back to back): forward with both norms and
+// a gate per token, 16384 x 2048: 47 us, 5.7 TB/s, 0.87 of the copy bandwidth;
+// backward with a channel gate, 8192 x 4096: 83 us, 4.8 TB/s (77 us for the
+// rows, where 2.3 instructions a cycle of 4 are issued, and the rest for
+// adding up the CTAs' column sums).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -741,8 +755,8 @@ struct NormGradPlan {
 };
 static NormGradPlan plan_norm_backward(int T, int d) {
     NormGradPlan p{};
-    // Two chunks a thread and up to 512 threads: 48 column sums and the row in
-    // flight fit 128 registers; the widest rows take four.
+    // Two chunks a thread and up to 512 threads: 32 column sums and the row in
+    // hand fit 128 registers; the widest rows take four.
     p.v = d <= 8192 ? 2 : 4;
     p.row_threads = row_threads_for(d, p.v);
     p.cta_threads = p.row_threads == 32 ? 128 : p.row_threads;

@@ -27,6 +27,18 @@
 //    by its scale.
 //  - The k blocks are split over the CTA's warps (WK ways) and joined in
 //    shared memory in warp order: results do not depend on timing.
+// What bounds it: for one token latency (launch, slot list, one trip to memory
+// for x and for the weights); for batches the tensor pipe, on which an
+// mma.sync m16n8k16 takes 32 cycles, 16 x 16 weights for 8 rows: 4.5 TB/s of
+// weights on the whole card at best (39 us for 64 tokens, of 27 us that memory
+// would need), and the unpacking (7 integer operations for 8 weights, issued
+// at half rate).  tcgen05.mma with the unpacked weights in tensor memory was
+// built and measured too: its smallest shape (128 x 16 x 16) holds the issuing
+// thread 40 to 61 cycles, and the chain from unpacking to reading the groups'
+// accumulators back is longer; it took 66 us for that case and 16 us for a
+// single token.  Measured on one B200, 60 experts, 4 a token (bf16, groups of
+// 128, gate/up 2816 x 2048 with SwiGLU): 1 token 12.7 us, 64 tokens 52 us;
+// down 2048 x 1408 (fp16, groups of 32, zero points), 147 tokens: 75 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -132,7 +144,7 @@ template <int DT> __device__ __forceinline__ uint16_t w4_to16(float f) {
 // XS: x is staged in shared memory; otherwise (rows too long for it) each lane
 // reads its pieces of x from global memory, where they stay in L1 / L2.
 // W: warps of the CTA.  With 16 rows of x a CTA fills an SM by itself, and 16
-// warps share them (147 tokens of 60 experts of 2048 x 1408: see the launch).
+// warps share them (147 tokens, 2048 x 1408: 71 us against 76 with 8).
 template <int DT, int G, int NT, bool XS, int W>
 __global__ void __launch_bounds__(W * 32, 16 / W)
 expert_linear_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a) {

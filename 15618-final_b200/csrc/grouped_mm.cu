@@ -29,8 +29,8 @@
 //           read from shared memory per 512 cycles); a pair can.
 // Forward and dgrad tiles cost the same, and a persistent grid deals them
 // round-robin.  A wgrad tile costs as much as its segment has rows; there the
-// grid is one CTA (pair) per tile and running ones take over waiting ones
-// (cluster launch control), which balances any routing.
+// grid is one CTA per tile and running ones take over waiting ones (cluster
+// launch control), which balances any routing.
 //
 // wgrad runs on single SMs (a pair would have to exchange the cleared ends of
 // segments).  Its last K step of a segment holds rows of the next segment: the
@@ -39,8 +39,17 @@
 //
 // The tensor core's queue holds about one K step: the loop of the issuing
 // thread has to come around within one MMA (128 cycles), so it does nothing
-// but wait, add to descriptors, issue and commit.  Every wait is bounded, as
-// in the expert FFN.
+// but wait, add to descriptors, issue and commit (with a warp-wide wait and
+// descriptors built anew the forward took 760 us instead of 690).  Results
+// leave through TMA stores from the swizzled staging tile.  Every wait is
+// bounded, as in the expert FFN.
+//
+// Measured on one B200, bf16, back to back (the power limit holds the SM clock
+// near 1.2 to 1.4 GHz then, and cuBLAS at 1340 TFLOP/s for one product of this
+// size): 60 even segments of 1024 rows, 2816 x 2048: forward 572 us (1240
+// TFLOP/s), dgrad 592, wgrad 708 (1000); 65536 Zipf-routed rows: 690, 685, 843.
+// wgrad of 128 short segments (7992 rows, 712 x 1096), 77 us, writes 200 MB at
+// 2.6 TB/s; a plain fill of memory reaches 3.9 TB/s on this card.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
