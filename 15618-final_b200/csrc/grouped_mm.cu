@@ -341,6 +341,9 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 const int e = s_exp[s], row0 = s_start[s];
                 const int a0 = m * GEO::kBlockRows + int(crank) * GEO::kTileM;    // rows of A (wgrad: columns of dy)
                 const int b0 = n * kMmTileN + int(crank) * GEO::kBCols;        // columns of the output
+                // A pair's second half past the segment reads zeros from beyond the
+                // tensor instead of other segments' rows: no traffic, and less power.
+                const int a_row = CG == 1 || a0 < s_rows[s] ? row0 + a0 : a.rows;
                 for (int kb = 0; kb < nk; ++kb, ++it) {
                     const int st = int(it % kStages);
                     if (!wait_or_abort(&ctl->empty[st], ((it / kStages) & 1u) ^ 1u, abort_flag, a.status)) break;
@@ -356,7 +359,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                             for (int i = 0; i < GEO::kBCols / 64; ++i)
                                 tma_load_2d(pb + i * kMmBoxBytes, &tmap_b, b0 + i * 64, row0 + k0, bar);
                         } else {
-                            tma_load_2d(pa, &tmap_a, k0, row0 + a0, bar);
+                            tma_load_2d(pa, &tmap_a, k0, a_row, bar);
                             if (MODE == kMmForward) {
                                 tma_load_3d(pb, &tmap_b, k0, b0, e, bar);
                             } else {
@@ -368,7 +371,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                         // Both CTAs' bytes land on the leader's barrier.
                         const uint32_t bar = leader_full0 + uint32_t(st) * 8u;
                         if (crank == 0) mbar_arrive_expect_tx(&ctl->full[st], 2 * kStage);
-                        tma_load_2d_pair(pa, &tmap_a, k0, row0 + a0, bar);
+                        tma_load_2d_pair(pa, &tmap_a, k0, a_row, bar);
                         if (MODE == kMmForward) {
                             tma_load_3d_pair(pb, &tmap_b, k0, b0, e, bar);
                         } else {
