@@ -16,11 +16,13 @@
 //
 // One CTA per SM, 7 warps: TMA producer, MMA issuer, 4 epilogue warps (TMEM
 // accumulator double-buffered, so the epilogue of one tile runs under the MMAs
-// of the next), tile scheduler.  Three forms share the code:
-//   few     one SM per 32 x 128 tile: for a few rows of a few experts, where the
+// of the next), tile scheduler.  Four forms share the code:
+//   few     one SM per 32 x 128 tile: for segments of a few rows, where the
 //           time is that of reading the weights and narrow tiles bring more
 //           SMs to it; only 32 rows of A are loaded (the MMA's other 96 rows
 //           are whatever lies behind them and are not read back)
+//   narrow  one SM per 128 x 64 tile: for products of so few wider tiles that
+//           most SMs would be idle
 //   single  one SM per 128 x 256 tile, 48 KB a K step, 4 stages: for short
 //           segments, where a taller tile would be half empty
 //   pair    an SM pair (cluster of 2) per 256 x 256 tile: each CTA stages its
@@ -39,15 +41,17 @@
 //
 // The tensor core's queue holds about one K step: the loop of the issuing
 // thread has to come around within one MMA (128 cycles), so it does nothing
-// but wait, add to descriptors, issue and commit (with a warp-wide wait and
-// descriptors built anew the forward took 760 us instead of 690).  Results
-// leave through TMA stores from the swizzled staging tile.  Every wait is
-// bounded, as in the expert FFN.
+// but wait, add to descriptors, issue and commit, and it runs under the
+// warp's elected thread (see elect_one): a K step of a small tile takes 300
+// cycles so, 600 under `lane == 0` (one row, 4096 x 4096: 13.5 us against 22.3).
+// Results leave through TMA stores from the swizzled staging tile.  Every wait
+// is bounded, as in the expert FFN.
 //
 // Measured on one B200, bf16, back to back (the power limit holds the SM clock
 // near 1.2 to 1.4 GHz then, and cuBLAS at 1340 TFLOP/s for one product of this
-// size): 60 even segments of 1024 rows, 2816 x 2048: forward 572 us (1240
-// TFLOP/s), dgrad 592, wgrad 708 (1000); 65536 Zipf-routed rows: 690, 685, 843.
+// size): 60 even segments of 1024 rows, 2816 x 2048: forward 570 to 610 us (1160
+// to 1240 TFLOP/s), dgrad 590, wgrad 695 (1020); 65536 Zipf-routed rows: 665,
+// 660, 813.
 // wgrad of 128 short segments (7992 rows, 712 x 1096), 77 us, writes 200 MB at
 // 2.6 TB/s; a plain fill of memory reaches 3.9 TB/s on this card.
 #include <cuda.h>
@@ -75,17 +79,18 @@ constexpr uint32_t kMmTmemCols = 512;
 constexpr int kMmBufCols = 256;                          // TMEM columns of one accumulator
 constexpr int kMmMaxSegments = 1024;
 constexpr int kSchedSlots = 4;
-enum { kMmFew = 0, kMmSingle = 1, kMmPair = 2 };
+enum { kMmFew = 0, kMmSingle = 1, kMmPair = 2, kMmNarrow = 3 };
 template <int FORM> struct MmGeo {
     static constexpr int kCtas = FORM == kMmPair ? 2 : 1;
     static constexpr int kTileM = FORM == kMmFew ? 32 : 128;  // rows of A per CTA
-    static constexpr int kTileN = FORM == kMmFew ? 128 : 256;
+    static constexpr int kTileN = FORM == kMmNarrow ? 64 : FORM == kMmFew ? 128 : 256;
     static constexpr int kBlockRows = kTileM * kCtas;         // rows per tile
     static constexpr int kBCols = kTileN / kCtas;             // columns of B a CTA holds
     static constexpr uint32_t kABytes = kTileM * kMmTileK * 2;
     static constexpr uint32_t kBBytes = kBCols * kMmTileK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = FORM == kMmFew ? 9 : FORM == kMmSingle ? 4 : 6;  // 180 or 192 KB
+    static constexpr int kStages =                            // 180 or 192 KB
+        FORM == kMmFew ? 9 : FORM == kMmNarrow ? 8 : FORM == kMmSingle ? 4 : 6;
 };
 constexpr int kMmMaxStages = 9;
 
@@ -334,10 +339,11 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         uint32_t it = 0;
+        int leader = 0;
         for (int tile = first_tile; tile >= 0; tile = next_tile(tile)) {
             int s, m, n;
             const int nk = locate(tile, s, m, n);
-            if (lane == 0) {
+            if (elect_one(leader)) {
                 const int e = s_exp[s], row0 = s_start[s];
                 const int a0 = m * GEO::kBlockRows + int(crank) * GEO::kTileM;    // rows of A (wgrad: columns of dy)
                 const int b0 = n * kMmTileN + int(crank) * GEO::kBCols;        // columns of the output
@@ -385,7 +391,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         }
         // (the pair's loads complete on the leader's barriers; the last cluster
         // barrier keeps the peer resident until the leader has drained them)
-        if (lane == 0 && crank == 0 && *abort_flag) drain_stages(ctl->full, it, kStages);
+        if (lane == leader && crank == 0 && *abort_flag) drain_stages(ctl->full, it, kStages);
     } else if (warp == 1) {
         // ---------------- MMA issuer (the pair's leader) ----------------
         // Bits 15 / 16 of the instruction descriptor: A / B is MN-major.
@@ -400,6 +406,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         int st = 0;
         uint32_t phase = 0, j = 0;
         bool ok = crank == 0;
+        int leader = 0;
         auto issue = [&](uint32_t d_tmem, int kk, uint32_t acc) {
             const uint64_t ad = adesc0 + uint32_t(st) * stage_step + uint32_t(kk) * a_step;
             const uint64_t bd = bdesc0 + uint32_t(st) * stage_step + uint32_t(kk) * b_step;
@@ -421,7 +428,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const int rem = MODE == kMmWgrad ? s_rows[s] % kMmTileK : 0;  // rows of a last, partial step
             const int nfull = nk - (rem > 0 ? 1 : 0);
             const uint32_t d_tmem = tmem + uint32_t(buf) * kMmBufCols;
-            if (lane == 0) {
+            if (elect_one(leader)) {
                 ok = wait_or_abort(&ctl->tmem_empty[buf], ((j >> 1) & 1u) ^ 1u, abort_flag, a.status);
                 tc_fence_after();
                 for (int kb = 0; ok && kb < nfull; ++kb) {
@@ -436,9 +443,9 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             }
             ++j;
             if (MODE == kMmWgrad) {
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                st = __shfl_sync(0xffffffffu, st, 0);
-                phase = __shfl_sync(0xffffffffu, phase, 0);
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, leader) != 0;
+                st = __shfl_sync(0xffffffffu, st, leader);
+                phase = __shfl_sync(0xffffffffu, phase, leader);
                 if (ok && rem > 0) {
                     ok = __all_sync(0xffffffffu, wait_or_abort(&ctl->full[st], phase, abort_flag, a.status));
                     if (ok) {
@@ -447,7 +454,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                         fence_proxy_async_smem();
                         __syncwarp();
                         tc_fence_after();
-                        if (lane == 0) {
+                        if (elect_one(leader)) {
                             for (int kk = 0; kk < k16; ++kk) issue(d_tmem, kk, (nfull | kk) != 0 ? 1u : 0u);
                             commit(&ctl->empty[st]);
                         }
@@ -455,8 +462,8 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                     }
                 }
             }
-            if (lane == 0 && ok) commit(&ctl->tmem_full[buf]);
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, leader) != 0;
+            if (ok && elect_one(leader)) commit(&ctl->tmem_full[buf]);
         }
     } else if (warp < 6) {
         // ---------------- epilogue (warps 2..5) ----------------
@@ -652,6 +659,9 @@ static cudaError_t launch_mm_as(int dtype, int form, const CUtensorMap& ma, cons
         if (form == kMmFew)
             return bf ? launch_mm<MODE, MOE_B200_BF16, kMmFew>(ma, mb, mc, a, s)
                       : launch_mm<MODE, MOE_B200_F16, kMmFew>(ma, mb, mc, a, s);
+        if (form == kMmNarrow)
+            return bf ? launch_mm<MODE, MOE_B200_BF16, kMmNarrow>(ma, mb, mc, a, s)
+                      : launch_mm<MODE, MOE_B200_F16, kMmNarrow>(ma, mb, mc, a, s);
     }
     return bf ? launch_mm<MODE, MOE_B200_BF16, kMmSingle>(ma, mb, mc, a, s)
               : launch_mm<MODE, MOE_B200_F16, kMmSingle>(ma, mb, mc, a, s);
@@ -660,16 +670,22 @@ static cudaError_t launch_mm_as(int dtype, int form, const CUtensorMap& ma, cons
 // Rows a tile loads and columns of its B that a CTA loads.
 static int form_rows(int form) { return form == kMmFew ? MmGeo<kMmFew>::kTileM : MmGeo<kMmSingle>::kTileM; }
 static int form_cols(int form) {
-    return form == kMmFew ? MmGeo<kMmFew>::kBCols : form == kMmPair ? MmGeo<kMmPair>::kBCols : MmGeo<kMmSingle>::kBCols;
+    return form == kMmFew      ? MmGeo<kMmFew>::kBCols
+           : form == kMmNarrow ? MmGeo<kMmNarrow>::kBCols
+           : form == kMmPair   ? MmGeo<kMmPair>::kBCols
+                               : MmGeo<kMmSingle>::kBCols;
 }
 
 // The form of forward and dgrad, from what the host knows (measured on one B200,
 // bf16, routing even / Zipf):
-//  few     while single tiles would be fewer than the SMs and segments have at
-//          most 16 rows on average: 4 experts of 2816 x 2048, one row each:
-//          21 us against 28; 8 experts of 1024 x 4096, 4 rows: 30 against 42.
-//          With tiles enough for all SMs it loses (60 experts, 16 rows: 125 /
-//          151 us against 120 / 118), as it does with more rows.
+//  few     segments of at most 16 rows on average: 60 experts of 1408 x 2048:
+//          4 rows 58 / 49 us against 66 / 48 as single tiles, 15 rows 59 / 68
+//          against 68 / 67, 20 rows 63 / 69 against 68 / 68, 40 rows 76 / 90
+//          against 70 / 68; 4 experts of 2816 x 1024, 16 rows: 7.1 against 9.9.
+//          (All 900 rows on one of the 60 experts: 30 against 19.)
+//  narrow  at most two narrow tiles an SM: 1024 rows of one expert, 1408 x 2048
+//          (176 tiles): 13.9 against 14.7 as single tiles; 256 rows (44 tiles)
+//          8.6 against 14.5; 2048 rows (352 tiles) 19.1 against 15.1.
 //  pair    segments of 384 rows on average and two rounds of pair tiles: 60 x
 //          384 rows 282 / 287 us against 292 / 300; with 128 rows 140 / 171
 //          against 140 / 169; with one round (16 x 512 rows of 1024 x 1024) 26
@@ -678,7 +694,9 @@ static int mm_form(int mode, int rows, int nseg, int wide) {
     if (mode == kMmWgrad) return kMmSingle;
     const int sms = device_sm_count();
     const int64_t columns = (int64_t(wide) + 255) / 256;
-    if (rows <= 16 * int64_t(nseg) && (rows < nseg ? rows : nseg) * columns <= sms) return kMmFew;
+    if (rows <= 16 * int64_t(nseg)) return kMmFew;
+    const int64_t blocks = rows / 128 + (rows < nseg ? rows : nseg);  // at most
+    if (blocks * ((int64_t(wide) + 63) / 64) <= 2 * int64_t(sms)) return kMmNarrow;
     return rows >= 384 * int64_t(nseg) && rows / 256 * columns >= sms ? kMmPair : kMmSingle;
 }
 
@@ -709,7 +727,7 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     a.kdim = mode == kMmForward ? K : N;
     a.m_out = N;
     const int64_t n_most = (int64_t(wide) + 127) / 128, m_most = (int64_t(N) + 127) / 128;  // of the smallest tiles
-    if ((int64_t(rows) / 32 + nseg) * n_most > INT32_MAX || nseg * m_most * n_most > INT32_MAX)
+    if ((int64_t(rows) / 32 + nseg) * 2 * n_most > INT32_MAX || nseg * m_most * n_most > INT32_MAX)
         return fail(MOE_B200_ERR_UNSUPPORTED, "%s: too many tiles", who);
     if (rows == 0) {  // wgrad: sums over no row
         const cudaError_t err = cudaMemsetAsync(out, 0, size_t(nseg) * size_t(N) * size_t(K) * 2, s);

@@ -93,6 +93,18 @@ __device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* m
         : "memory");
 }
 
+// One thread of the (converged) warp, the same one in every call, and its lane.
+// The instructions that one thread issues (TMA, MMA, commit) take their operands
+// from the warp's uniform registers.  Under this condition the compiler knows
+// that a single thread runs; under `lane == 0` it does not, and a tcgen05.mma
+// held its issuer for 64 cycles instead of about 20.
+__device__ __forceinline__ bool elect_one(int& leader) {
+    uint32_t l, p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync %0|p, 0xffffffff;\n\tselp.u32 %1, 1, 0, p;\n\t}" : "=r"(l), "=r"(p));
+    leader = int(l);
+    return p != 0;
+}
+
 // --- CTA pair (cluster of 2) helpers ---
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
