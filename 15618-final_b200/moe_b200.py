@@ -526,8 +526,12 @@ def _enqueue(what, fn, dev, stream, fresh, *args):
         _check(status, what)
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _row_stride(what, name, t, shape, dtype):
+    """Elements from row to row of a tensor whose rows may lie apart."""
+    if t.shape == shape and t.dtype == dtype and t.is_contiguous():
+        return shape[1]
+    _rows(what, name, t, shape, dtype, strided=True)
+    return t.stride(0) if shape[0] > 1 else shape[1]
 
 
 def _gate_form(what, gate, T, d, dtype):
@@ -559,7 +563,8 @@ class BlockNormGrads(NamedTuple):
 
 
 def _check_block_norm(what, residual, y, w_post, w_pre, gate):
-    """The checks both directions share: (T, d, dtype, its code, fp32 residual, gate form)."""
+    """The checks both directions share: (T, d, dtype, its code, residual is
+    fp32, gate form, row strides of residual and y)."""
     import torch
     if residual.dim() != 2:
         _refuse(what, "the residual must be [T, d]")
@@ -574,17 +579,19 @@ def _check_block_norm(what, residual, y, w_post, w_pre, gate):
     res32 = res_dtype == torch.float32
     if not res32 and res_dtype != dtype:
         _refuse(what, f"the residual must be {dtype} or float32, got {res_dtype}")
+    res_stride, y_stride = d, 0
     if not residual.is_contiguous():
-        _rows(what, "the residual", residual, shape, res_dtype, strided=True)
+        res_stride = _row_stride(what, "the residual", residual, shape, res_dtype)
     if y is not None:
-        _rows(what, "y", y, shape, dtype, strided=True)
+        y_stride = _row_stride(what, "y", y, shape, dtype)
         if w_post is not None:
             _rows(what, "w_post", w_post, (d,), dtype)
     elif w_post is not None or gate is not None:
         _refuse(what, "w_post and gate need y")
     if w_pre is not None:
         _rows(what, "w_pre", w_pre, (d,), dtype)
-    return T, d, dtype, code, int(res32), GATE_NONE if gate is None else _gate_form(what, gate, T, d, dtype)
+    form = GATE_NONE if gate is None else _gate_form(what, gate, T, d, dtype)
+    return T, d, dtype, code, int(res32), form, res_stride, y_stride
 
 
 def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, eps=1e-6, out=None, stream=None):
@@ -595,14 +602,15 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
     the residual), gate [T, 1], [1, d] / [d] or [T, d].  residual and y may be
     row-strided.  out: a BlockNormResult of contiguous tensors to write."""
     import torch
-    T, d, dtype, code, res32, form = _check_block_norm("block_norm", residual, y, w_post, w_pre, gate)
+    T, d, dtype, code, res32, form, res_stride, y_stride = _check_block_norm("block_norm", residual, y, w_post, w_pre,
+                                                                              gate)
     dev = _same_device("block_norm", residual, y, w_post, w_pre, gate)
     fresh = ()
     if out is None:
+        like, plain = torch.empty_like, torch.contiguous_format
         fresh = out = BlockNormResult(
-            residual_out=torch.empty_like(residual, memory_format=torch.contiguous_format) if y is not None else None,
-            normed=torch.empty_like(residual, dtype=dtype, memory_format=torch.contiguous_format)
-            if w_pre is not None else None)
+            like(residual, memory_format=plain) if y is not None else None,
+            like(residual, dtype=dtype, memory_format=plain) if w_pre is not None else None)
     else:
         if (out.residual_out is None) != (y is None) or (out.normed is None) != (w_pre is None):
             _refuse("block_norm", "out needs residual_out with y and normed with w_pre, and neither without")
@@ -614,9 +622,8 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
     if T == 0:
         return out if y is not None else BlockNormResult(residual, out.normed)
     _enqueue("block_norm", lib().moe_b200_block_norm, dev, stream, fresh,
-             _ptr(y), _row_stride(y) if y is not None else 0, _ptr(residual), _row_stride(residual),
-             res32, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d, code, _ptr(out.residual_out),
-             _ptr(out.normed))
+             _ptr(y), y_stride, _ptr(residual), res_stride, res32, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale,
+             eps, T, d, code, _ptr(out.residual_out), _ptr(out.normed))
     return out if y is not None else BlockNormResult(residual, out.normed)
 
 
@@ -629,7 +636,7 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     16-bit [T, d]."""
     import torch
     what = "block_norm_backward"
-    T, d, dtype, code, res32, form = _check_block_norm(what, residual_out, y, w_post, w_pre, gate)
+    T, d, dtype, code, res32, form, res_stride, y_stride = _check_block_norm(what, residual_out, y, w_post, w_pre, gate)
     if (d_normed is None) != (w_pre is None):
         _refuse(what, "d_normed and w_pre go together")
     if d_residual_out is None and w_pre is None:
@@ -644,11 +651,11 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     like, plain = torch.empty_like, torch.contiguous_format
     f32 = torch.float32
     got = BlockNormGrads(
-        d_residual=like(residual_out, memory_format=plain),
-        d_y=like(y, memory_format=plain) if y is not None else None,
-        d_w_post=like(w_post, dtype=f32) if w_post is not None else None,
-        d_w_pre=like(w_pre, dtype=f32) if w_pre is not None else None,
-        d_gate=None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32))
+        like(residual_out, memory_format=plain),
+        like(y, memory_format=plain) if y is not None else None,
+        like(w_post, dtype=f32) if w_post is not None else None,
+        like(w_pre, dtype=f32) if w_pre is not None else None,
+        None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32))
     if T == 0:  # sums over no token
         with torch.cuda.stream(stream if not isinstance(stream, int) else torch.cuda.ExternalStream(stream, device=dev)):
             for t in got[2:]:
@@ -657,10 +664,9 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
         return got
     ws = residual_out.new_empty((max(nbytes, 256),), dtype=torch.uint8)
     _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream, (*got, ws),
-             _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), _row_stride(residual_out), res32, _ptr(y),
-             _row_stride(y) if y is not None else 0, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d,
-             code, _ptr(got.d_residual), _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre),
-             _ptr(got.d_gate), _ptr(ws), nbytes)
+             _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), res_stride, res32, _ptr(y), y_stride,
+             _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d, code, _ptr(got.d_residual),
+             _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre), _ptr(got.d_gate), _ptr(ws), nbytes)
     return got
 
 
@@ -684,7 +690,7 @@ def _grouped_mm(what, fn, rows_in, seg_start, w, seg_expert, out, stream, forwar
     dev = _same_device(what, rows_in, seg_start, w, seg_expert, out)
     fresh = ()
     if out is None:
-        out = torch.empty((rows, width_out), dtype=dtype, device=dev)
+        out = rows_in.new_empty((rows, width_out))
         fresh = (out,)
     else:
         _rows(what, "out", out, (rows, width_out), dtype)
@@ -728,7 +734,7 @@ def grouped_mm_wgrad(dy, x, seg_start, out=None, stream=None):
     dev = _same_device(what, x, dy, seg_start, out)
     fresh = ()
     if out is None:
-        out = torch.empty((nseg, N, K), dtype=dtype, device=dev)
+        out = x.new_empty((nseg, N, K))
         fresh = (out,)
     else:
         _rows(what, "out", out, (nseg, N, K), dtype)
@@ -771,7 +777,7 @@ def expert_linear_w4(x, asgn, w_q, w_scale, w_zero=None, act=None, out=None, str
     dev = _same_device(what, x, asgn, w_q, w_scale, w_zero, out)
     fresh = ()
     if out is None:
-        out = torch.empty((T * K, n_out), dtype=dtype, device=dev)
+        out = x.new_empty((T * K, n_out))
         fresh = (out,)
     else:
         _rows(what, "out", out, (T * K, n_out), dtype)
