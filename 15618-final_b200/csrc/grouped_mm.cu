@@ -475,7 +475,8 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             int s, m, n;
             const int nk = locate(tile, s, m, n);
             const int w_row0 = m * GEO::kBlockRows + int(crank) * GEO::kTileM + quad * 32;
-            const int nrows_w = (MODE == kMmWgrad ? a.m_out : s_rows[s]) - w_row0;
+            // Of a 32-row tile only the first warp has rows; behind them lie the next tile's.
+            const int nrows_w = quad * 32 < GEO::kTileM ? (MODE == kMmWgrad ? a.m_out : s_rows[s]) - w_row0 : 0;
             const int64_t out_row = (MODE == kMmWgrad ? int64_t(s) * a.m_out : int64_t(s_start[s])) + w_row0;
             uint16_t* dst = a.out + out_row * a.n_out;
             // The staged 32 x 64 piece has the layout of a 128-byte-swizzled TMA

@@ -95,6 +95,14 @@ def test_pair_single_and_few_row_forms(cuda, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hot", [33, 40, 64, 100, 700])
+@pytest.mark.parametrize("K,N", [(64, 72), (200, 264), (1024, 512)])
+def test_long_segments_among_many_short_ones(cuda, hot, K, N):
+    """Few rows a segment on average, and segments of more rows than that form's tile has."""
+    check(*make([7, 0, hot] + [3] * 60 + [hot - 1, 0], K, N, torch.bfloat16, seed=hot))
+
+
+@pytest.mark.gpu
 def test_every_segment_empty(cuda):
     x, dy, w, seg = make([0, 0, 0], 64, 48, torch.bfloat16, extra=5)
     out = torch.full((5, 48), 7.0, dtype=x.dtype, device="cuda")
