@@ -254,15 +254,24 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         prefetch_tmap(&tmap_c);
     }
     if (warp == 0) {
-        // Offsets are held inside [0, rows], so that no bad table leads a store outside the output.
-        int run = 0;
+        // Offsets are held ascending inside [0, rows]: no bad table leads a
+        // store outside the output or makes more tiles than the host counted.
+        int run = 0, reached = 0;
         for (int s0 = 0; s0 < a.nseg; s0 += 32) {
             const int i = s0 + lane;
             int cnt = 0;
+            int lo = i < a.nseg ? min(max(a.seg_start[i], 0), a.rows) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, lo, o);
+                if (lane >= o) lo = max(lo, v);
+            }
+            lo = max(lo, reached);
+            const int hi = i < a.nseg ? max(min(a.seg_start[i + 1], a.rows), lo) : lo;
+            reached = __shfl_sync(0xffffffffu, hi, 31);
             if (i < a.nseg) {
-                const int lo = min(max(a.seg_start[i], 0), a.rows), hi = min(max(a.seg_start[i + 1], 0), a.rows);
                 s_start[i] = lo;
-                s_rows[i] = max(hi - lo, 0);
+                s_rows[i] = hi - lo;
                 s_exp[i] = a.seg_expert ? a.seg_expert[i] : i;
                 cnt = (s_rows[i] + GEO::kBlockRows - 1) / GEO::kBlockRows;
             }

@@ -242,7 +242,7 @@ int moe_b200_ffn_weights_from_reference(const void* w1, const void* w2, int E, i
  * layer's products (moe_b200_grouped_ffn's up and down products are two of
  * them) can be trained; the gradient of a packed row's token is
  * moe_b200_unpermute with weights of 1.
- * seg_start [nseg + 1] ascending within [0, rows] (held inside it otherwise);
+ * seg_start [nseg + 1] ascending within [0, rows] (held so otherwise);
  * rows outside every segment are left as they were, and a segment whose
  * expert is outside [0, E) gives zeros.  N and K multiples of 8; nseg <= 1024;
  * pointers 16-byte aligned; no workspace.  Replaces the per-expert

@@ -88,7 +88,7 @@ def test_most_segments(cuda):
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [8, 300, 2000, 9000])
 def test_pair_single_and_few_row_forms(cuda, rows):
-    """The three tile forms (chosen by the rows a segment has on average and
+    """The tile forms (chosen by the rows a segment has on average and
     the number of tiles), each with segments far from the average."""
     check(*make([rows, 3 * rows, 1, 0, rows // 2], 264, 520, torch.float16, seed=rows))
     check(*make([5 * rows + 3], 200, 136, torch.bfloat16, seed=rows))
@@ -172,6 +172,22 @@ def test_offsets_outside_the_rows_are_held_inside(cuda):
     bad = torch.tensor([-100, 30, 1 << 30], dtype=torch.int32, device="cuda")
     assert torch.equal(mb.grouped_mm(x, bad, w), want)
     assert torch.equal(mb.grouped_mm_wgrad(dy, x, bad), mb.grouped_mm_wgrad(dy, x, seg))
+    assert mb.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_offsets_that_fall_are_held_ascending(cuda):
+    """A start below an earlier one counts as that one, also 32 segments later."""
+    counts = [7, 0, 40] + [3] * 40
+    x, dy, w, seg = make(counts, 64, 72, torch.bfloat16)
+    bad = seg.clone()
+    bad[2] = 5        # inside segment 0: segment 1 is empty, segment 2 begins at 7 all the same
+    seg[35] = seg[34]
+    bad[35] = 0       # far back: segment 34 is empty and 35 begins where it did
+    for got, want in ((mb.grouped_mm(x, bad, w), mb.grouped_mm(x, seg, w)),
+                      (mb.grouped_mm_dgrad(dy, bad, w), mb.grouped_mm_dgrad(dy, seg, w)),
+                      (mb.grouped_mm_wgrad(dy, x, bad), mb.grouped_mm_wgrad(dy, x, seg))):
+        assert torch.equal(got, want)
     assert mb.device_status() == 0
 
 
