@@ -148,6 +148,30 @@ def test_widths(cuda, d, res):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["token", "channel", "full"])
+@pytest.mark.parametrize("T,d", [(2500, 177), (1200, 255), (1200, 1001), (700, 2050), (400, 4097), (300, 8201)])
+def test_rows_that_begin_inside_a_word(cuda, gate, T, d):
+    """Columns in pairs: with odd d every other row begins inside a word, and a
+    CTA has several rows; with even d the rows end inside a 16-byte step."""
+    check(make(T, d, torch.float16, torch.float32, gate, True, True, seed=d))
+    check(make(T, d, torch.bfloat16, torch.bfloat16, gate, True, True, seed=d + 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,stride", [(65, 66), (65, 67), (66, 67), (64, 66)])
+def test_strides_and_starts_of_either_kind(cuda, d, stride):
+    """Row strides that agree with d in pairs and that do not, and a tensor that begins inside a word."""
+    g = torch.Generator(device="cuda").manual_seed(stride)
+    for start in (0, 1, 2):
+        p = make(90, d, torch.bfloat16, torch.bfloat16, "full", True, True, seed=d + start)
+        p["y"] = torch.as_strided(rand(g, (start + 90 * stride,), torch.bfloat16), (90, d), (stride, 1), start)
+        check(p)
+        flat = rand(g, (start + 90 * d,), torch.bfloat16)
+        p["d_normed"] = flat[start:].view(90, d)
+        check(p)
+
+
+@pytest.mark.gpu
 def test_many_rows_share_the_columns(cuda):
     """More rows than a grid holds at once: column sums over many rows a CTA."""
     check(make(5000, 72, torch.bfloat16, torch.bfloat16, "channel", True, True))
