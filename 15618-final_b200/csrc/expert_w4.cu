@@ -28,17 +28,20 @@
 //  - The k blocks are split over the CTA's warps (WK ways) and joined in
 //    shared memory in warp order: results do not depend on timing.
 // What bounds it: for one token latency (launch, slot list, one trip to memory
-// for x and for the weights); for batches the tensor pipe, on which an
-// mma.sync m16n8k16 takes 32 cycles, 16 x 16 weights for 8 rows: 4.5 TB/s of
-// weights on the whole card at best (39 us for 64 tokens, of 27 us that memory
-// would need), and the unpacking (7 integer operations for 8 weights, issued
-// at half rate).  tcgen05.mma with the unpacked weights in tensor memory was
-// built and measured too: its smallest shape (128 x 16 x 16) holds the issuing
-// thread 40 to 61 cycles, and the chain from unpacking to reading the groups'
-// accumulators back is longer; it took 66 us for that case and 16 us for a
-// single token.  Measured on one B200, 60 experts, 4 a token (bf16, groups of
-// 128, gate/up 2816 x 2048 with SwiGLU): 1 token 12.7 us, 64 tokens 52 us;
-// down 2048 x 1408 (fp16, groups of 32, zero points), 147 tokens: 75 us.
+// for x and for the weights); for batches the work between the MMAs, spread
+// over all of it: about half of the issue slots are used, by 4 warps a
+// scheduler (128 registers each), with 4 instructions a weight and lane
+// (unpacking, x and scales from shared memory and by shuffles, the groups' sums)
+// and stalls on all of these.  The tensor pipe is not it: mma.sync m16n8k16 takes
+// 8 cycles a scheduler, a quarter of the time, and a unit with 8 rows of x costs
+// about as much as one with 16, so that shares weighted by rows are worse (66 to
+// 78 us against 62).  tcgen05.mma with the unpacked weights in tensor memory was
+// built and measured too: the chain from unpacking to reading the groups'
+// accumulators back is longer (64 tokens 75 us, one token 11, in a graph;
+// this form 50 and 7).  Measured on one B200, 60 experts, 4 a token (bf16, groups
+// of 128, gate/up 2816 x 2048 with SwiGLU): 1 token 12.7 us, 64 tokens 52 us;
+// down 2048 x 1408 (fp16, groups of 32, zero points), 147 tokens: 73 to 81 us by
+// routing.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

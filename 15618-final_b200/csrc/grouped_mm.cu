@@ -52,8 +52,8 @@
 // size): 60 even segments of 1024 rows, 2816 x 2048: forward 570 to 610 us (1160
 // to 1240 TFLOP/s), dgrad 590, wgrad 695 (1020); 65536 Zipf-routed rows: 665,
 // 660, 813.
-// wgrad of 128 short segments (7992 rows, 712 x 1096), 77 us, writes 200 MB at
-// 2.6 TB/s; a plain fill of memory reaches 3.9 TB/s on this card.
+// wgrad of 128 short segments (7992 rows, 712 x 1096), 79 us, writes 200 MB at
+// 2.5 TB/s; a plain fill of memory reaches 3.9 TB/s on this card.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -463,7 +463,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                         fence_proxy_async_smem();
                         __syncwarp();
                         tc_fence_after();
-                        if (elect_one(leader)) {
+                        if (lane == leader) {  // (elect_one costs the few MMAs more than it saves: 81 us against 79 ragged)
                             for (int kk = 0; kk < k16; ++kk) issue(d_tmem, kk, (nfull | kk) != 0 ? 1u : 0u);
                             commit(&ctl->empty[st]);
                         }
