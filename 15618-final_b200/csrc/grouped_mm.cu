@@ -112,7 +112,7 @@ struct MmSmem {
 struct MmArgs {
     const int32_t* seg_start;
     const int32_t* seg_expert;
-    int nseg, rows;
+    int nseg, rows, experts;
     int kdim;      // reduced length (forward, dgrad)
     int m_blocks;  // wgrad: row blocks of dw
     int n_blocks;  // column blocks of the output
@@ -272,7 +272,8 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             if (i < a.nseg) {
                 s_start[i] = lo;
                 s_rows[i] = hi - lo;
-                s_exp[i] = a.seg_expert ? a.seg_expert[i] : i;
+                const int e = a.seg_expert ? a.seg_expert[i] : i;
+                s_exp[i] = e >= 0 && e < a.experts ? e : -1;
                 cnt = (s_rows[i] + GEO::kBlockRows - 1) / GEO::kBlockRows;
             }
             int incl = cnt;
@@ -341,7 +342,9 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         n = tile % a.n_blocks;
         s = find_segment(blk_prefix, a.nseg, g);
         m = g - blk_prefix[s];
-        return (a.kdim + kMmTileK - 1) / kMmTileK;
+        // No expert: no steps, and the epilogue writes zeros.  (Weights that read
+        // as zeros would not do: a NaN or infinity in the rows would meet them.)
+        return s_exp[s] < 0 ? 0 : (a.kdim + kMmTileK - 1) / kMmTileK;
     };
     const uint32_t leader_full0 = CG == 2 ? map_to_rank(&ctl->full[0], 0) : 0u;
 
@@ -432,7 +435,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         for (int tile = first_tile; ok && tile >= 0; tile = next_tile(tile)) {
             int s, m, n;
             const int nk = locate(tile, s, m, n);
-            if (nk == 0) continue;  // an empty segment: the epilogue writes zeros
+            if (nk == 0) continue;  // an empty segment or no expert: the epilogue writes zeros
             const int buf = int(j & 1u);
             const int rem = MODE == kMmWgrad ? s_rows[s] % kMmTileK : 0;  // rows of a last, partial step
             const int nfull = nk - (rem > 0 ? 1 : 0);
@@ -731,6 +734,7 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     a.seg_expert = seg_expert;
     a.nseg = nseg;
     a.rows = rows;
+    a.experts = E;
     a.out = static_cast<uint16_t*>(out);
     const int wide = mode == kMmForward ? N : K;  // output columns
     a.n_out = wide;

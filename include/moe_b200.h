@@ -244,7 +244,8 @@ int moe_b200_ffn_weights_from_reference(const void* w1, const void* w2, int E, i
  * moe_b200_unpermute with weights of 1.
  * seg_start [nseg + 1] ascending within [0, rows] (held so otherwise);
  * rows outside every segment are left as they were, and a segment whose
- * expert is outside [0, E) gives zeros.  N and K multiples of 8; nseg <= 1024;
+ * expert is outside [0, E) gives zeros, whatever its rows hold.  N and K
+ * multiples of 8; nseg <= 1024;
  * pointers 16-byte aligned; no workspace.  Replaces the per-expert
  * cublasHgemm calls of apps/bench_e2e.cu:274-301 as single products; the
  * reference has no gradients.  Device-side conditions:

@@ -133,6 +133,40 @@ def test_expert_map_and_experts_out_of_range(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts,K,N", [
+    ([9, 20, 7, 0, 12], 72, 136),                # 32-row tiles
+    ([100, 40, 129, 64, 1], 72, 136),            # narrow tiles
+    ([300, 260, 130, 0, 600] * 3, 72, 1544),     # 128 x 256 tiles in the forward
+    ([300, 260, 130, 0, 600] * 3, 1544, 72),     # and in dgrad
+    ([5000, 5000, 3000], 72, 1544),              # SM pairs, the same
+    ([5000, 5000, 3000], 1544, 72),
+])
+def test_rows_of_experts_out_of_range_may_hold_anything(cuda, counts, K, N):
+    """A segment whose expert is outside [0, E) gives zeros whatever its rows
+    hold (padding: NaN, infinities), and its neighbours are not touched."""
+    n = len(counts)
+    x, dy, w, seg = make(counts, K, N, torch.bfloat16, E=2, seed=n)
+    ss = seg.tolist()
+    for bad in (2, -1, 2 ** 31 - 1, -2 ** 31):
+        experts = [s % 2 for s in range(n)]
+        out = [0, n - 1]
+        for i, s in enumerate(out):
+            experts[s] = bad
+            x[ss[s]:ss[s + 1]] = float("nan") if i else float("inf")
+            dy[ss[s]:ss[s + 1]] = float("-inf") if i else float("nan")
+        se = torch.tensor(experts, dtype=torch.int32, device="cuda")
+        y, dx = mb.grouped_mm(x, seg, w, se), mb.grouped_mm_dgrad(dy, seg, w, se)
+        assert mb.device_status() == 0
+        for s in range(n):
+            lo, hi = ss[s], ss[s + 1]
+            if s in out:
+                assert (y[lo:hi] == 0).all() and (dx[lo:hi] == 0).all()
+            elif hi > lo:
+                assert_close(y[lo:hi], x[lo:hi], w[experts[s]].T, f"y of {s}")
+                assert_close(dx[lo:hi], dy[lo:hi], w[experts[s]], f"dx of {s}")
+
+
+@pytest.mark.gpu
 def test_rows_outside_the_segments(cuda):
     """Rows before and behind the segments: not written by the forward and
     dgrad, and what they hold (NaN here) reaches no sum of wgrad."""
