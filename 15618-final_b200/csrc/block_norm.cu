@@ -221,7 +221,8 @@ template <int DT, bool RES32, int AL, bool RING, bool WARP, int MAXT, int FORM>
 static cudaError_t launch_norm_as(NormArgs a, int cta, int64_t grid, size_t smem, cudaStream_t s) {
     auto kern = block_norm_kernel<DT, RES32, AL, RING, WARP, 2, MAXT, FORM>;
     if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
-        const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        static SmemLimit limit;
+        const cudaError_t err = limit.open(reinterpret_cast<const void*>(kern));
         if (err != cudaSuccess) return err;
     }
     kern<<<unsigned(grid), cta, smem, s>>>(a);

@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "per_device.cuh"
 
 namespace moe_b200 {
 

@@ -379,7 +379,8 @@ static cudaError_t launch_norm_backward_as(const NormGradArgs& a, const NormGrad
     constexpr int kMax = WARP ? 128 : 512;
     auto kern = block_norm_backward_kernel<DT, RES32, AL, RING, WARP, V, kMax, GATE>;
     if (smem > 40 * 1024) {  // beyond what a kernel may use unasked
-        const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        static SmemLimit limit;
+        const cudaError_t err = limit.open(reinterpret_cast<const void*>(kern));
         if (err != cudaSuccess) return err;
     }
     kern<<<p.grid, p.cta_threads, smem, s>>>(a);

@@ -48,6 +48,7 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "per_device.cuh"
 #include "tcgen05.cuh"
 
 namespace moe_b200 {
@@ -533,7 +534,8 @@ template <int DT, int G, int NT, bool XS, int W>
 static cudaError_t launch_w4(const CUtensorMap& map, W4Args a, int served, cudaStream_t s) {
     const size_t smem = w4_layout(a, NT, XS, W);
     auto kern = expert_linear_w4_kernel<DT, G, NT, XS, W>;
-    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    static SmemLimit limit;
+    const cudaError_t err = limit.open(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     int64_t grid = 16 / W * device_sm_count();
     // Warps that share a tile's k: few, as each joint costs about as much as a

@@ -63,6 +63,7 @@
 
 #include "common.cuh"
 #include "gemm_epilogue.cuh"
+#include "per_device.cuh"
 #include "tcgen05.cuh"
 
 namespace moe_b200 {
@@ -624,7 +625,8 @@ static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, const
     auto kern = grouped_mm_kernel<MODE, DT, FORM>;
     const size_t smem = 1024 + size_t(GEO::kStages) * GEO::kStageBytes + kStageBytes + sizeof(MmSmem) +
                         size_t(4 * a.nseg + 1) * 4;
-    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    static SmemLimit limit;
+    const cudaError_t err = limit.open(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     a.m_blocks = (a.m_out + GEO::kBlockRows - 1) / GEO::kBlockRows;
     a.n_blocks = (a.n_out + GEO::kTileN - 1) / GEO::kTileN;
