@@ -45,6 +45,7 @@
 
 #include "common.cuh"
 #include "gemm_epilogue.cuh"
+#include "per_device.cuh"
 #include "tcgen05.cuh"
 
 namespace moe_b200 {
@@ -491,7 +492,8 @@ static cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb_, co
     EpWait no_wait{};
     const size_t smem = ffn_smem_bytes<CG>(nseg);
     auto kern = grouped_gemm_kernel<EPI, DT, CG>;
-    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    static SmemLimit limit;
+    const cudaError_t err = limit.open(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     // Upper bound on tiles: every segment may add one partial block.
     const int64_t max_tiles = (int64_t(rows) / Geo<CG>::kBlockRows + nseg) * n_blocks;

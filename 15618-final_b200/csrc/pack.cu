@@ -34,6 +34,7 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "per_device.cuh"
 
 namespace moe_b200 {
 
@@ -538,8 +539,8 @@ cudaError_t launch_pack(const void* emb, const int32_t* asgn, const float* wts, 
     const bool want_bulk = !(sel && sel[0] == 'r');
     if (vec && want_bulk && ring >= 4) {
         const int smem = int(ring * rowb + ring * 8 + E * 4 + 128);
-        err = cudaFuncSetAttribute(pack_rows_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   smem);
+        static SmemLimit limit;
+        err = limit.open(reinterpret_cast<const void*>(pack_rows_bulk_kernel));
         if (err != cudaSuccess) return err;
         int per_sm = 0;
         err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, pack_rows_bulk_kernel, 32, smem);

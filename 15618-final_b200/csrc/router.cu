@@ -35,6 +35,7 @@
 #include <cstdint>
 
 #include "common.cuh"
+#include "per_device.cuh"
 #include "tcgen05.cuh"
 
 namespace moe_b200 {
@@ -596,7 +597,8 @@ extern "C" int moe_b200_route(const void* emb, int T, int d, int E, int K, int d
         cfg.numAttrs = 1;
     }
     auto kern = route_kernel_for(dtype, K);
-    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    static SmemLimit limits[2][9];  // by type and K, as the kernels
+    cudaError_t err = limits[dtype == MOE_B200_F16][K].open(reinterpret_cast<const void*>(kern));
     if (err == cudaSuccess)
         err = cudaLaunchKernelEx(&cfg, kern, mx, mw, hdr, T, d, E, E_pad, P, stages, nsplit, uint32_t(area),
                                  assignments, weights, st);

@@ -15,6 +15,7 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "per_device.cuh"
 
 namespace moe_b200 {
 
@@ -318,7 +319,8 @@ cudaError_t launch_unpermute(const void* y, const float* packed_w, const int32_t
         const int smem = bulk_smem_bytes(K, d, stages);
         auto kern = dtype == MOE_B200_F16 ? unpermute_bulk_kernel<MOE_B200_F16>
                                           : unpermute_bulk_kernel<MOE_B200_BF16>;
-        cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        static SmemLimit limits[2];
+        cudaError_t err = limits[dtype == MOE_B200_F16].open(reinterpret_cast<const void*>(kern));
         if (err != cudaSuccess) return err;
         int per_sm = 0;
         err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kBulkThreads, smem);

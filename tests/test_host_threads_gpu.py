@@ -115,3 +115,35 @@ def test_norm_gradients(cuda):
                  *ptr(d_r, d_y, d_post, d_pre), None, *ptr(ws), nbytes), [d_r, d_y, d_post, d_pre], (dr, dn, r, y, w, ws))
 
     run_together([job(40, d) for d in (2816, 4096, 2304, 4096)])
+
+
+@pytest.mark.parametrize("op", ["pack", "ffn", "unpermute", "route"])
+def test_layer(cuda, op):
+    """The layer's own operators."""
+    L = mb.lib()
+
+    def job(T, d, E, K):
+        x, g = rand((T, d), d), torch.Generator(device="cuda").manual_seed(d)
+        asgn = torch.rand((T, E), generator=g, device="cuda").topk(K, dim=1).indices.to(torch.int32).contiguous()
+        wts = torch.rand((T, K), generator=g, device="cuda")
+        if op == "pack":
+            nbytes = L.moe_b200_pack_workspace_bytes(T, K, E)
+            ws, packed, pw = torch.zeros(nbytes, device="cuda", dtype=torch.uint8), empty(T * K, d), empty(T * K, dtype=torch.float32)
+            idx = [empty(n, dtype=torch.int32) for n in (T * K, E, E + 1, T * K)]
+            return (L.moe_b200_pack, (*ptr(x, asgn, wts), T, K, E, d, *ptr(packed, pw, *idx), *ptr(ws), nbytes), [packed, pw, *idx],
+                    (x, asgn, wts, ws))
+        if op == "route":
+            r = mb.RouterWeights(torch.randn((d, E), generator=g, device="cuda") * d ** -0.5, torch.bfloat16)
+            a, w = empty(T, K, dtype=torch.int32), empty(T, K, dtype=torch.float32)
+            return L.moe_b200_route, (*ptr(x), T, d, E, K, mb.BF16, *ptr(r.buf), *ptr(a, w)), [a, w], (x, r)
+        if op == "unpermute":
+            y, pos, out = rand((T * K, d), 3), torch.randperm(T * K, generator=g, device="cuda").to(torch.int32), empty(T, d)
+            return L.moe_b200_unpermute, (*ptr(y, wts, pos), T, K, d, mb.BF16, *ptr(out)), [out], (y, wts, pos)
+        seg = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+        seg[-1] = T
+        up, down, mid, y = rand((E, 32, 64), 4, 0.1), rand((E, 64, 32), 5, 0.1), empty(T, 32), empty(T, 64)
+        x = rand((T, 64), 6)
+        return (L.moe_b200_grouped_ffn, (*ptr(x, seg), None, E, T, 64, 32, E, *ptr(up, down), mb.BF16, *ptr(mid, y)), [mid, y],
+                (x, seg, up, down))
+
+    run_together([job(40, 256, 4, 1), job(40, 2048, 16, 4), job(40, 512, 100, 2), job(40, 1024, 128, 4)])
