@@ -568,15 +568,10 @@ static cudaError_t run_w4(const CUtensorMap& map, W4Args a, cudaStream_t s) {
 
 // 3-D map over w_q [E, N, d/2] bytes; box = 128 bytes x 16 rows of one expert, 128B swizzle.
 static bool make_map_w4(CUtensorMap* map, const void* base, int E, int N, int K) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[3] = {cuuint64_t(K / 2), cuuint64_t(N), cuuint64_t(E)};
-    cuuint64_t strides[2] = {cuuint64_t(K / 2), cuuint64_t(K / 2) * cuuint64_t(N)};
-    cuuint32_t box[3] = {128u, 16u, 1u};
-    cuuint32_t estr[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t dims[3] = {cuuint64_t(K / 2), cuuint64_t(N), cuuint64_t(E)};
+    const cuuint64_t strides[2] = {cuuint64_t(K / 2), cuuint64_t(K / 2) * cuuint64_t(N)};
+    const cuuint32_t box[3] = {128u, 16u, 1u};
+    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box);
 }
 
 }  // namespace moe_b200

@@ -605,16 +605,10 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 // 3-D map over w [E, N, K] 16-bit; box = 64 columns x box_rows rows of one expert, 128B swizzle.
 static bool make_map_experts(CUtensorMap* map, const void* base, int64_t experts, int64_t rows, int64_t cols,
                              int box_rows, int dtype) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(experts)};
-    cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * cuuint64_t(rows) * 2};
-    cuuint32_t box[3] = {64u, cuuint32_t(box_rows), 1u};
-    cuuint32_t estr[3] = {1, 1, 1};
-    return fn(map, dtype == MOE_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-              const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(experts)};
+    const cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * cuuint64_t(rows) * 2};
+    const cuuint32_t box[3] = {64u, cuuint32_t(box_rows), 1u};
+    return encode_tiled(map, map_type(dtype), 3, base, dims, strides, box);
 }
 
 template <int MODE, int DT, int FORM>

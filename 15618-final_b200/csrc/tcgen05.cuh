@@ -199,20 +199,37 @@ inline EncodeTiledFn encode_fn() {
     return fn;
 }
 
+// Encodes a tiled tensor map of 16-bit or byte elements, 128-byte swizzle, zeros
+// out of bounds.  The encoder needs a current context, which a host thread has
+// only after its first call that uses the device (cudaGetDevice is none): where
+// it is missing, the current device's is made current and the map encoded again.
+inline bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                         const cuuint64_t* strides, const cuuint32_t* box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint32_t estr[3] = {1, 1, 1};
+    auto encode = [&] {
+        return fn(map, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    int dev = 0;
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+        r = encode();
+    return r == CUDA_SUCCESS;
+}
+inline CUtensorMapDataType map_type(int dtype) {
+    return dtype == MOE_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
 // 2-D K-major map over a row-major [rows, cols] 16-bit matrix; box = 64 x box_rows, 128B swizzle.
 inline bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows,
                      int dtype) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
-    cuuint64_t strides[1] = {cuuint64_t(cols) * 2};
-    cuuint32_t box[2] = {64u, cuuint32_t(box_rows)};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, dtype == MOE_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                    2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS;
+    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(cols) * 2};
+    const cuuint32_t box[2] = {64u, cuuint32_t(box_rows)};
+    return encode_tiled(map, map_type(dtype), 2, base, dims, strides, box);
 }
 
 }  // namespace moe_b200

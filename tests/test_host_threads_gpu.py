@@ -147,3 +147,41 @@ def test_layer(cuda, op):
                 (x, seg, up, down))
 
     run_together([job(40, 256, 4, 1), job(40, 2048, 16, 4), job(40, 512, 100, 2), job(40, 1024, 128, 4)])
+
+
+@pytest.mark.parametrize("op", ["grouped_mm", "dgrad", "wgrad", "w4", "norm", "norm_backward", "ffn", "route", "pack", "unpermute"])
+def test_a_threads_first_use_of_the_gpu(cuda, op):
+    """A call that is the first thing its host thread does on the device."""
+    x, w, w2 = rand((16, 64), 1), rand((2, 64, 64), 2, 0.1), rand((2, 64, 64), 3, 0.1)
+    one, seg, a = rand((64,), 4), torch.tensor([0, 7, 16], dtype=torch.int32, device="cuda"), ints((16, 1), 2, 5)
+    wq, ws = ints((2, 64, 32), 256, 6, torch.uint8), rand((2, 64, 2), 7, 0.01)
+    wts, pos = torch.ones(16, 1, device="cuda"), torch.arange(16, dtype=torch.int32, device="cuda")
+    router, space = mb.RouterWeights(torch.randn(64, 8, device="cuda"), torch.bfloat16), mb.Workspace(16, 1, 2)
+    calls = {
+        "grouped_mm": lambda: mb.grouped_mm(x, seg, w),
+        "dgrad": lambda: mb.grouped_mm_dgrad(x, seg, w),
+        "wgrad": lambda: mb.grouped_mm_wgrad(x, x, seg),
+        "w4": lambda: mb.expert_linear_w4(x, a, wq, ws),
+        "norm": lambda: mb.block_norm(x, x, one, one).normed,
+        "norm_backward": lambda: mb.block_norm_backward(x, x, x, x, one, one).d_y,
+        "ffn": lambda: mb.grouped_ffn(x, seg, w, w2)[1],
+        "route": lambda: mb.route(x, router, 2)[1],
+        "pack": lambda: mb.pack(x, a, wts, 2, workspace=space).packed,
+        "unpermute": lambda: mb.unpermute(x, wts, pos, 16, 1),
+    }
+    call, got = calls[op], []
+    want = call()
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            got.append(call())
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert isinstance(got[0], torch.Tensor), got[0]
+    assert torch.equal(got[0], want)
