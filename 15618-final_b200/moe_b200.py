@@ -503,6 +503,15 @@ def _same_device(what, *tensors):
     return tensors[0].device
 
 
+def _on_device(dev, fn, *args):
+    """fn(*args) with `dev` current."""
+    import torch
+    if torch._C._cuda_getDevice() == dev.index:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
 def _enqueue(what, fn, dev, stream, fresh, *args):
     """Calls fn(*args, stream) with `dev` current.  `fresh`: tensors that this
     call allocated, which the allocator must not hand out again before the
@@ -517,11 +526,7 @@ def _enqueue(what, fn, dev, stream, fresh, *args):
             for t in fresh:
                 if t is not None:
                     t.record_stream(s)
-    if torch._C._cuda_getDevice() == index:
-        status = fn(*args, handle)
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, handle)
+    status = _on_device(dev, fn, *args, handle)
     if status != OK:
         _check(status, what)
 
@@ -646,7 +651,8 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
     if d_normed is not None:
         _rows(what, "d_normed", d_normed, (T, d), dtype)
     dev = _same_device(what, residual_out, d_residual_out, d_normed, y, w_post, w_pre, gate)
-    nbytes = int(lib().moe_b200_block_norm_backward_workspace_bytes(T, d))
+    # of the tensors' device: the size follows its number of SMs
+    nbytes = int(_on_device(dev, lib().moe_b200_block_norm_backward_workspace_bytes, T, d))
 
     like, plain = torch.empty_like, torch.contiguous_format
     f32 = torch.float32
