@@ -59,8 +59,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
-
 #include "common.cuh"
 #include "gemm_epilogue.cuh"
 #include "per_device.cuh"
@@ -641,14 +639,14 @@ static cudaError_t launch_mm(const CUtensorMap& ma, const CUtensorMap& mb, const
         groups = (int64_t(a.rows) / GEO::kBlockRows + a.nseg) * a.n_blocks;  // a segment may add one partial block
         int fit = device_sm_count() / CG;
         if (CG == 2) {  // not every SM has a partner: a pair left waiting would run its share behind all others
-            static std::atomic<int> pairs{0};
-            int n = pairs.load(std::memory_order_relaxed);
-            if (n == 0) {
+            static DeviceCount pairs;
+            const int n = pairs.get([&] {
+                int most = 0;
                 cfg.gridDim = dim3(unsigned(2 * fit));
-                if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) n = fit;
+                if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess || most < 1) most = fit;
                 cudaGetLastError();
-                pairs.store(n, std::memory_order_relaxed);
-            }
+                return most;
+            });
             if (n < fit) fit = n;
         }
         if (groups > fit) groups = fit;

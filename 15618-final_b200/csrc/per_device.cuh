@@ -6,6 +6,24 @@
 
 namespace moe_b200 {
 
+constexpr int kPerDevice = 64;  // devices whose values are kept
+
+// A count that belongs to the current device: asked for by ask() (> 0) at its
+// first use there.
+class DeviceCount {
+public:
+    template <typename Ask> int get(Ask&& ask) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kPerDevice) return ask();
+        int n = known_[dev].load(std::memory_order_relaxed);
+        if (n == 0) known_[dev].store(n = ask(), std::memory_order_relaxed);
+        return n;
+    }
+
+private:
+    std::atomic<int> known_[kPerDevice] = {};
+};
+
 // Lets a kernel use as much dynamic shared memory as a block of the current
 // device can have.  The limit belongs to the kernel and the device, not to a
 // call: set to what one call needs, another host thread may lower it between
@@ -18,7 +36,7 @@ public:
         int dev = 0;
         cudaError_t err = cudaGetDevice(&dev);
         if (err != cudaSuccess) return err;
-        const bool kept = dev >= 0 && dev < kDevices;
+        const bool kept = dev >= 0 && dev < kPerDevice;
         if (kept && open_[dev].load(std::memory_order_acquire)) return cudaSuccess;
         int most = 0;
         cudaFuncAttributes of_kernel{};
@@ -32,8 +50,7 @@ public:
     }
 
 private:
-    static constexpr int kDevices = 64;
-    std::atomic<bool> open_[kDevices] = {};
+    std::atomic<bool> open_[kPerDevice] = {};
 };
 
 }  // namespace moe_b200

@@ -78,6 +78,19 @@ SMEM_LIMIT = r"""
     CHECK(bad == 0 && g_lowered == 0);
 """
 
+DEVICE_COUNT = r"""
+    static DeviceCount count, other;
+    int asked = 0;
+    auto ask = [&] { ++asked; return 10 + t_device; };
+    CHECK(count.get(ask) == 10 && count.get(ask) == 10 && asked == 1);
+    t_device = 3;                                        // another device does not get the first one's
+    CHECK(count.get(ask) == 13 && count.get(ask) == 13 && asked == 2);
+    t_device = 0;
+    CHECK(count.get(ask) == 10 && asked == 2 && other.get(ask) == 10 && asked == 3);
+    t_device = 100;
+    CHECK(count.get(ask) == 110 && count.get(ask) == 110 && asked == 5);
+"""
+
 
 def run(tmp_path, body):
     gxx = shutil.which("g++")
@@ -93,3 +106,7 @@ def run(tmp_path, body):
 
 def test_shared_memory_limit_is_set_once_and_never_lowered(tmp_path):
     run(tmp_path, SMEM_LIMIT)
+
+
+def test_counts_belong_to_their_device(tmp_path):
+    run(tmp_path, DEVICE_COUNT)
