@@ -281,11 +281,13 @@ extern "C" int moe_b200_block_norm(const void* y, int64_t y_stride, const void* 
     if (residual_stride < d || (y && y_stride < d))
         return fail(MOE_B200_ERR_INVALID_ARG, "block_norm: row strides below d=%d", d);
     if (T == 0) return MOE_B200_OK;
-    uint32_t* status = device_status_word();
-    if (!status) return fail(MOE_B200_ERR_CUDA, "block_norm: device status word unavailable");
-    const NormArgs a{y, residual, w_post, w_pre, gate, y ? y_stride : 0, residual_stride, gate_form, scale, eps, T, d,
-                     y ? residual_out : nullptr, w_pre ? normed : nullptr, 0, 0, 0, 0, status};
+    NormArgs a{y, residual, w_post, w_pre, gate, y ? y_stride : 0, residual_stride, gate_form, scale, eps, T, d,
+               y ? residual_out : nullptr, w_pre ? normed : nullptr, 0, 0, 0, 0, nullptr};
     const bool res32 = residual_f32 != 0;
+    if (inside_element({y, w_post, w_pre, gate, a.normed}, 2) || inside_element({residual, a.residual_out}, res32 ? 4 : 2))
+        return fail(MOE_B200_ERR_INVALID_ARG, "block_norm: a pointer is not aligned to its elements");
+    a.status = device_status_word();
+    if (!a.status) return fail(MOE_B200_ERR_CUDA, "block_norm: device status word unavailable");
     const int access = access_of(d,
                                  {{y, y_stride, false}, {residual, residual_stride, res32}, {a.residual_out, d, res32},
                                   {a.normed, d, false}, {gate_form == kGateFull ? gate : nullptr, d, false}},

@@ -463,6 +463,11 @@ extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const vo
     if ((w_pre && residual_stride < d) || (y && y_stride < d))
         return fail(MOE_B200_ERR_INVALID_ARG, "block_norm_backward: row strides below d=%d", d);
     const bool res32 = residual_f32 != 0;
+    if (inside_element({y, w_post, w_pre, gate, w_pre ? d_normed : nullptr, y ? d_y : nullptr}, 2) ||
+        inside_element({d_residual_out, w_pre ? residual_out : nullptr, d_residual}, res32 ? 4 : 2) ||
+        inside_element({w_post ? d_w_post : nullptr, w_pre ? d_w_pre : nullptr}, 4) ||
+        inside_element({gate ? d_gate : nullptr}, gate_form == kGateFull ? 2 : 4))
+        return fail(MOE_B200_ERR_INVALID_ARG, "block_norm_backward: a pointer is not aligned to its elements");
     NormGradPlan p = plan_norm_backward(T, d);
     const int vectors = column_vectors(w_pre != nullptr, w_post != nullptr, gate_form);
     if (vectors && (!workspace || workspace_bytes < align256(size_t(vectors) * p.grid * size_t(d) * 4)))

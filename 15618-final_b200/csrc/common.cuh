@@ -6,6 +6,8 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include <initializer_list>
+
 #include "moe_b200.h"
 
 namespace moe_b200 {
@@ -189,6 +191,13 @@ __device__ __forceinline__ void bulk_wait() {
 }
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Host: whether one of the pointers (NULL: absent) begins inside an element of `bytes` bytes.
+inline bool inside_element(std::initializer_list<const void*> pointers, size_t bytes) {
+    for (const void* p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return true;
+    return false;
 }
 
 uint32_t* device_status_word();  // status.cu

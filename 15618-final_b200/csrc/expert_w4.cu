@@ -602,6 +602,7 @@ extern "C" int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const in
                          reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(w_zero) |
                          reinterpret_cast<uintptr_t>(out);
     if (al % 16 != 0) return fail(MOE_B200_ERR_INVALID_ARG, "expert_linear_w4: pointers must be 16-byte aligned");
+    if (inside_element({asgn}, 4)) return fail(MOE_B200_ERR_INVALID_ARG, "expert_linear_w4: asgn must be 4-byte aligned");
     uint32_t* st = device_status_word();
     if (!st) return fail(MOE_B200_ERR_CUDA, "expert_linear_w4: device status word unavailable");
     W4Args a{};

@@ -723,6 +723,8 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
         return fail(MOE_B200_ERR_INVALID_ARG, "%s: null pointer", who);
     const uintptr_t al = reinterpret_cast<uintptr_t>(pa) | reinterpret_cast<uintptr_t>(pb) | reinterpret_cast<uintptr_t>(out);
     if (al % 16 != 0) return fail(MOE_B200_ERR_INVALID_ARG, "%s: pointers must be 16-byte aligned", who);
+    if (inside_element({seg_start, seg_expert}, 4))
+        return fail(MOE_B200_ERR_INVALID_ARG, "%s: the segment tables must be 4-byte aligned", who);
     MmArgs a{};
     a.seg_start = seg_start;
     a.seg_expert = seg_expert;

@@ -245,11 +245,10 @@ int moe_b200_ffn_weights_from_reference(const void* w1, const void* w2, int E, i
  * seg_start [nseg + 1] ascending within [0, rows] (held so otherwise);
  * rows outside every segment are left as they were, and a segment whose
  * expert is outside [0, E) gives zeros, whatever its rows hold.  N and K
- * multiples of 8; nseg <= 1024;
- * pointers 16-byte aligned; no workspace.  Replaces the per-expert
- * cublasHgemm calls of apps/bench_e2e.cu:274-301 as single products; the
- * reference has no gradients.  Device-side conditions:
- * moe_b200_device_status().                                                 */
+ * multiples of 8; nseg <= 1024; x, dy, w and the results 16-byte aligned, the
+ * tables 4-byte; no workspace.  Replaces the per-expert cublasHgemm calls of
+ * apps/bench_e2e.cu:274-301 as single products; the reference has no
+ * gradients.  Device-side conditions: moe_b200_device_status().             */
 int moe_b200_grouped_mm(const void* x, const int32_t* seg_start, const int32_t* seg_expert, int nseg, int rows, int N,
                         int K, int E, const void* w, int dtype, void* y, void* stream);
 int moe_b200_grouped_mm_dgrad(const void* dy, const int32_t* seg_start, const int32_t* seg_expert, int nseg, int rows,
@@ -385,8 +384,8 @@ uint64_t moe_b200_ep_epoch(void* ctx);
  *                        residual itself where that is contiguous
  *   normed       [T, d]  out, contiguous, 16-bit; taken from the unrounded
  *                        residual_out; may be y itself where that is contiguous
- * Sums in fp32; d <= 16384, any alignment (rows whose d, strides and pointers
- * are in 16-byte steps are read in 16-byte pieces).  No counterpart in the
+ * Sums in fp32; d <= 16384, any alignment to whole elements (rows whose d,
+ * strides and pointers are in 16-byte steps are read in 16-byte pieces).  No counterpart in the
  * reference, whose layer has no norms.                                      */
 enum moe_b200_gate_form {
     MOE_B200_GATE_NONE = 0,
@@ -438,7 +437,7 @@ int moe_b200_block_norm_backward(const void* d_residual_out, const void* d_norme
  * fp32 accumulation, out rounded once.  The outputs of a down product are
  * combined by moe_b200_unpermute with slot_pos[s] = s.  group 32, 64 or 128
  * and a divisor of d; N a multiple of 8 (SwiGLU: 16); T*K <= 4096; pointers
- * 16-byte aligned.  An expert outside [0, E) other than -1 gives zeros too
+ * 16-byte aligned (asgn 4-byte).  An expert outside [0, E) other than -1 gives zeros too
  * and MOE_B200_DEV_BAD_ASSIGNMENT in moe_b200_device_status().  No
  * counterpart in the reference, whose expert weights are 16-bit.            */
 enum moe_b200_act { MOE_B200_ACT_NONE = 0, MOE_B200_ACT_SWIGLU = 1 };
