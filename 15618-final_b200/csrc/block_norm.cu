@@ -286,6 +286,19 @@ extern "C" int moe_b200_block_norm(const void* y, int64_t y_stride, const void* 
     const bool res32 = residual_f32 != 0;
     if (inside_element({y, w_post, w_pre, gate, a.normed}, 2) || inside_element({residual, a.residual_out}, res32 ? 4 : 2))
         return fail(MOE_B200_ERR_INVALID_ARG, "block_norm: a pointer is not aligned to its elements");
+    const int64_t w16 = 2 * int64_t(d), w_res = (res32 ? 4 : 2) * int64_t(d);
+    const RowSet ro{a.residual_out, w_res, w_res, T}, no{a.normed, w16, w16, T};
+    const RowSet rows_in[] = {{y, 2 * a.y_stride, w16, T}, {residual, (res32 ? 4 : 2) * residual_stride, w_res, T},
+                              {gate_form == kGateFull ? gate : nullptr, w16, w16, T}};
+    // A row is read in full before it is written, each column by the thread that
+    // writes it: a result may be rows that are read, but not lie on others.
+    bool overlap = rows_overlap(ro, no);
+    for (const RowSet& out : {ro, no}) {
+        for (const RowSet& in : rows_in) overlap = overlap || (!same_rows(out, in) && rows_overlap(out, in));
+        overlap = overlap || overlaps_any(out, {whole(w_post, w16), whole(w_pre, w16),
+                                                whole(gate_form == kGateFull ? nullptr : gate, gate_form == kGateToken ? 2 * int64_t(T) : w16)});
+    }
+    if (overlap) return fail(MOE_B200_ERR_INVALID_ARG, "block_norm: a result overlaps an operand or the other result");
     a.status = device_status_word();
     if (!a.status) return fail(MOE_B200_ERR_CUDA, "block_norm: device status word unavailable");
     const int access = access_of(d,

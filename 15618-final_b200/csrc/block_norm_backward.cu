@@ -487,6 +487,33 @@ extern "C" int moe_b200_block_norm_backward(const void* d_residual_out, const vo
         }
         return MOE_B200_OK;
     }
+    const int64_t w16 = 2 * int64_t(d), w32 = 4 * int64_t(d), w_res = (res32 ? 4 : 2) * int64_t(d);
+    const bool full = gate_form == kGateFull;
+    const RowSet in_ds{d_residual_out, w_res, w_res, T}, in_rr{w_pre ? residual_out : nullptr, (res32 ? 4 : 2) * residual_stride, w_res, T};
+    const RowSet in_dn{w_pre ? d_normed : nullptr, w16, w16, T}, in_y{y, 2 * y_stride, w16, T};
+    const RowSet in_gate = full ? RowSet{gate, w16, w16, T} : whole(gate, gate_form == kGateToken ? 2 * int64_t(T) : w16);
+    const RowSet out_r{d_residual, w_res, w_res, T}, out_y{y ? d_y : nullptr, w16, w16, T};
+    const RowSet out_g = !gate  ? whole(nullptr, 0)
+                         : full ? RowSet{d_gate, w16, w16, T}
+                                : whole(d_gate, gate_form == kGateToken ? 4 * int64_t(T) : w32);
+    const RowSet flat[] = {whole(w_post ? d_w_post : nullptr, w32), whole(w_pre ? d_w_pre : nullptr, w32),
+                           whole(vectors ? workspace : nullptr, int64_t(align256(size_t(vectors) * p.grid * size_t(d) * 4)))};
+    // A thread reads its columns of a row, then writes d_residual, then reads the
+    // row's y and gate, then writes d_gate and d_y: a result may be rows that are
+    // read before it is written, but not lie on others.
+    auto on = [](const RowSet& out, std::initializer_list<RowSet> others) {
+        for (const RowSet& o : others)
+            if (!same_rows(out, o) && rows_overlap(out, o)) return true;
+        return false;
+    };
+    bool overlap = on(out_r, {in_ds, in_rr, in_dn}) || overlaps_any(out_r, {in_y, in_gate, out_y, out_g}) ||
+                   on(out_y, {in_ds, in_rr, in_dn, in_y, in_gate}) || on(out_g, {in_ds, in_rr, in_dn, in_y, in_gate}) ||
+                   rows_overlap(out_y, out_g) || rows_overlap(flat[0], flat[1]) || rows_overlap(flat[0], flat[2]) ||
+                   rows_overlap(flat[1], flat[2]);
+    for (const RowSet& out : {out_r, out_y, out_g}) overlap = overlap || overlaps_any(out, {whole(w_post, w16), whole(w_pre, w16)});
+    for (const RowSet& f : flat)
+        overlap = overlap || overlaps_any(f, {in_ds, in_rr, in_dn, in_y, in_gate, whole(w_post, w16), whole(w_pre, w16), out_r, out_y, out_g});
+    if (overlap) return fail(MOE_B200_ERR_INVALID_ARG, "block_norm_backward: a result overlaps an operand or another result");
     uint32_t* status = device_status_word();
     if (!status) return fail(MOE_B200_ERR_CUDA, "block_norm_backward: device status word unavailable");
     const NormGradArgs a{d_residual_out, d_normed, residual_out, y, w_post, w_pre, gate, y ? y_stride : 0,

@@ -200,6 +200,31 @@ inline bool inside_element(std::initializer_list<const void*> pointers, size_t b
     return false;
 }
 
+// Host: rows of `width` bytes, `stride` bytes apart (p NULL: absent).
+struct RowSet {
+    const void* p;
+    int64_t stride, width, rows;
+};
+// Whether rows share a byte with `out`, whose rows touch one another.
+inline bool rows_overlap(const RowSet& out, const RowSet& in) {
+    if (!out.p || !in.p || out.rows < 1 || in.rows < 1) return false;
+    const int64_t lo = int64_t(reinterpret_cast<uintptr_t>(out.p)), hi = lo + out.width * out.rows;
+    const int64_t base = int64_t(reinterpret_cast<uintptr_t>(in.p)), end0 = base + in.width;
+    const int64_t r = lo < end0 ? 0 : (lo - end0) / in.stride + 1;  // the first row that ends behind `lo`
+    return r < in.rows && base + r * in.stride < hi;
+}
+// The same rows, each in the same place.
+inline bool same_rows(const RowSet& a, const RowSet& b) {
+    return a.p == b.p && a.width == b.width && a.rows == b.rows && (a.rows == 1 || a.stride == b.stride);
+}
+inline RowSet whole(const void* p, int64_t bytes) { return RowSet{p, bytes, bytes, 1}; }
+// Whether `out` shares a byte with one of them.
+inline bool overlaps_any(const RowSet& out, std::initializer_list<RowSet> others) {
+    for (const RowSet& o : others)
+        if (rows_overlap(out, o)) return true;
+    return false;
+}
+
 uint32_t* device_status_word();  // status.cu
 int device_sm_count();                  // status.cu: SMs of the current device (148 if it cannot be asked)
 

@@ -603,6 +603,11 @@ extern "C" int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const in
                          reinterpret_cast<uintptr_t>(out);
     if (al % 16 != 0) return fail(MOE_B200_ERR_INVALID_ARG, "expert_linear_w4: pointers must be 16-byte aligned");
     if (inside_element({asgn}, 4)) return fail(MOE_B200_ERR_INVALID_ARG, "expert_linear_w4: asgn must be 4-byte aligned");
+    const int64_t slots = int64_t(T) * K, weights = int64_t(E) * N * d;
+    if (overlaps_any(whole(out, 2 * slots * (act == MOE_B200_ACT_SWIGLU ? N / 2 : N)),
+                     {whole(x, 2 * int64_t(d) * (x_per_slot ? slots : T)), whole(asgn, 4 * slots), whole(w_q, weights / 2),
+                      whole(w_scale, weights / group * 2), whole(w_zero, weights / group)}))
+        return fail(MOE_B200_ERR_INVALID_ARG, "expert_linear_w4: out overlaps an operand");
     uint32_t* st = device_status_word();
     if (!st) return fail(MOE_B200_ERR_CUDA, "expert_linear_w4: device status word unavailable");
     W4Args a{};

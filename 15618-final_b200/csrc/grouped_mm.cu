@@ -725,6 +725,12 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
     if (al % 16 != 0) return fail(MOE_B200_ERR_INVALID_ARG, "%s: pointers must be 16-byte aligned", who);
     if (inside_element({seg_start, seg_expert}, 4))
         return fail(MOE_B200_ERR_INVALID_ARG, "%s: the segment tables must be 4-byte aligned", who);
+    const int64_t row_n = 2 * int64_t(N), row_k = 2 * int64_t(K), weights = row_k * N;
+    const bool wg = mode == kMmWgrad;
+    if (overlaps_any(whole(out, wg ? nseg * weights : rows * (mode == kMmForward ? row_n : row_k)),
+                     {whole(pa, rows * (mode == kMmForward ? row_k : row_n)), whole(pb, wg ? rows * row_k : E * weights),
+                      whole(seg_start, 4 * (int64_t(nseg) + 1)), whole(seg_expert, 4 * int64_t(nseg))}))
+        return fail(MOE_B200_ERR_INVALID_ARG, "%s: the result overlaps an operand", who);
     MmArgs a{};
     a.seg_start = seg_start;
     a.seg_expert = seg_expert;

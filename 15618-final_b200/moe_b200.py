@@ -605,7 +605,8 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
       normed = rms(residual_out) * w_pre (w_pre None: None)
     residual [T, d] 16-bit or float32, y [T, d] 16-bit (None: residual_out is
     the residual), gate [T, 1], [1, d] / [d] or [T, d].  residual and y may be
-    row-strided.  out: a BlockNormResult of contiguous tensors to write."""
+    row-strided.  out: a BlockNormResult of contiguous tensors to write, each
+    of its own or the rows of residual, y or a [T, d] gate of its width."""
     import torch
     T, d, dtype, code, res32, form, res_stride, y_stride = _check_block_norm("block_norm", residual, y, w_post, w_pre,
                                                                               gate)
@@ -758,7 +759,8 @@ def expert_linear_w4(x, asgn, w_q, w_scale, w_zero=None, act=None, out=None, str
       w_zero  uint8 [E, N, d/group], None: 8
       act     None, or "swiglu": silu(y[:, :N/2]) * y[:, N/2:]
     Returns [T*K, N] (swiglu [T*K, N/2]); combine a down product's rows with
-    unpermute and slot_pos = arange(T*K)."""
+    unpermute and slot_pos = arange(T*K).  At most 4096 slots T*K and 1024
+    experts; N a multiple of 8 (swiglu: 16)."""
     import torch
     what = "expert_linear_w4"
     if act not in (None, "swiglu"):

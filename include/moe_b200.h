@@ -246,9 +246,10 @@ int moe_b200_ffn_weights_from_reference(const void* w1, const void* w2, int E, i
  * rows outside every segment are left as they were, and a segment whose
  * expert is outside [0, E) gives zeros, whatever its rows hold.  N and K
  * multiples of 8; nseg <= 1024; x, dy, w and the results 16-byte aligned, the
- * tables 4-byte; no workspace.  Replaces the per-expert cublasHgemm calls of
- * apps/bench_e2e.cu:274-301 as single products; the reference has no
- * gradients.  Device-side conditions: moe_b200_device_status().             */
+ * tables 4-byte; a result that overlaps an operand is refused; no workspace.
+ * Replaces the per-expert cublasHgemm calls of apps/bench_e2e.cu:274-301 as
+ * single products; the reference has no gradients.  Device-side conditions:
+ * moe_b200_device_status().                                                 */
 int moe_b200_grouped_mm(const void* x, const int32_t* seg_start, const int32_t* seg_expert, int nseg, int rows, int N,
                         int K, int E, const void* w, int dtype, void* y, void* stream);
 int moe_b200_grouped_mm_dgrad(const void* dy, const int32_t* seg_start, const int32_t* seg_expert, int nseg, int rows,
@@ -380,10 +381,11 @@ uint64_t moe_b200_ep_epoch(void* ctx);
  *   w_post, w_pre [d]    16-bit (dtype)
  *   gate                 16-bit (dtype): one value per token [T], per channel
  *                        [d] or per element [T, d] (MOE_B200_GATE_*)
- *   residual_out [T, d]  out, contiguous, the residual's type; may be the
- *                        residual itself where that is contiguous
+ *   residual_out [T, d]  out, contiguous, the residual's type
  *   normed       [T, d]  out, contiguous, 16-bit; taken from the unrounded
- *                        residual_out; may be y itself where that is contiguous
+ *                        residual_out
+ * A result may be the very rows of the residual, y or a [T, d] gate (where
+ * these are contiguous and as wide); any other overlap is refused.
  * Sums in fp32; d <= 16384, any alignment to whole elements (rows whose d,
  * strides and pointers are in 16-byte steps are read in 16-byte pieces).  No counterpart in the
  * reference, whose layer has no norms.                                      */
@@ -407,6 +409,8 @@ int moe_b200_block_norm(const void* y, int64_t y_stride, const void* residual, i
  *   d_residual [T, d] the residual's type    d_y [T, d] 16-bit (with y)
  *   d_w_post, d_w_pre [d] fp32               (with w_post / w_pre)
  *   d_gate  fp32 [T] / fp32 [d] / 16-bit [T, d] by gate_form
+ * A result [T, d] may be the very rows of an operand that it is as wide as
+ * (d_residual not of y or the gate); any other overlap is refused.
  * Sums over tokens are taken in a fixed order.  workspace:
  * moe_b200_block_norm_backward_workspace_bytes(T, d) bytes (on this device),
  * 256-byte aligned, needs no initial value; concurrent calls use distinct
@@ -437,9 +441,10 @@ int moe_b200_block_norm_backward(const void* d_residual_out, const void* d_norme
  * fp32 accumulation, out rounded once.  The outputs of a down product are
  * combined by moe_b200_unpermute with slot_pos[s] = s.  group 32, 64 or 128
  * and a divisor of d; N a multiple of 8 (SwiGLU: 16); T*K <= 4096; pointers
- * 16-byte aligned (asgn 4-byte).  An expert outside [0, E) other than -1 gives zeros too
- * and MOE_B200_DEV_BAD_ASSIGNMENT in moe_b200_device_status().  No
- * counterpart in the reference, whose expert weights are 16-bit.            */
+ * 16-byte aligned (asgn 4-byte); an out that overlaps an operand is refused.
+ * An expert outside [0, E) other than -1 gives zeros too and
+ * MOE_B200_DEV_BAD_ASSIGNMENT in moe_b200_device_status().  No counterpart in
+ * the reference, whose expert weights are 16-bit.                           */
 enum moe_b200_act { MOE_B200_ACT_NONE = 0, MOE_B200_ACT_SWIGLU = 1 };
 int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const int32_t* asgn, int T, int K, int E, int d, int N,
                               const void* w_q, const void* w_scale, const void* w_zero, int group, int act, int dtype,

@@ -221,6 +221,41 @@ def test_in_place(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,d", [(7, 40), (9, 33), (2500, 64), (700, 1024)])
+def test_results_on_rows_that_are_read(cuda, T, d):
+    """Either result on any of the rows that are read: the same bits."""
+    bf = torch.bfloat16
+    p = make(T, d, bf, bf, "full", True, True, seed=d)
+    want = mb.block_norm(p["residual"], p["y"], p["w_post"], p["w_pre"], p["gate"], 0.3)
+    for first, second in (("residual", "y"), ("y", "residual"), ("gate", "y"), ("residual", "gate")):
+        q = {k: v.clone() if v is not None else None for k, v in p.items()}
+        got = mb.block_norm(q["residual"], q["y"], q["w_post"], q["w_pre"], q["gate"], 0.3, out=mb.BlockNormResult(q[first], q[second]))
+        assert torch.equal(got.residual_out, want.residual_out) and torch.equal(got.normed, want.normed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,d", [(7, 40), (9, 33), (2500, 64), (700, 1024), (5, 8200)])
+def test_gradients_on_rows_that_are_read(cuda, T, d):
+    bf = torch.bfloat16
+    p = make(T, d, bf, bf, "full", True, True, seed=d)
+    r = p["residual"]
+    want = mb.block_norm_backward(p["d_res"], p["d_normed"], r, p["y"], p["w_post"], p["w_pre"], p["gate"], 0.3)
+    L = mb.lib()
+    nbytes = L.moe_b200_block_norm_backward_workspace_bytes(T, d)
+    for places in (("d_res", "y", "gate"), ("residual", "d_normed", "y"), ("d_normed", "gate", "d_res"), ("d_res", "residual", "d_normed")):
+        q = {k: v.clone() for k, v in p.items()}
+        sums, ws = torch.empty((2, d), device="cuda"), torch.empty(nbytes, device="cuda", dtype=torch.uint8)
+        out = [q[k] for k in places]
+        status = L.moe_b200_block_norm_backward(
+            q["d_res"].data_ptr(), q["d_normed"].data_ptr(), q["residual"].data_ptr(), d, 0, q["y"].data_ptr(), d, q["w_post"].data_ptr(),
+            q["w_pre"].data_ptr(), q["gate"].data_ptr(), mb.GATE_FULL, 0.3, 1e-6, T, d, mb.BF16, out[0].data_ptr(), out[1].data_ptr(),
+            sums[0].data_ptr(), sums[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream or None)
+        assert status == mb.OK
+        for got, ref in zip((*out, *sums), (want.d_residual, want.d_y, want.d_gate, want.d_w_post, want.d_w_pre)):
+            assert torch.equal(got, ref), places
+
+
+@pytest.mark.gpu
 def test_no_rows(cuda):
     p = make(0, 48, torch.bfloat16, torch.float32, "channel", True, True)
     f, b = run_both(p, 1.0, 1e-6)

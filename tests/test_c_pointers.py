@@ -65,3 +65,66 @@ def test_grouped_tables_inside_an_element(fn):
 
 def test_w4_assignments_inside_an_element():
     assert w4(asgn=P + 0x10002) == mb.ERR_INVALID_ARG
+
+
+# Results that lie on what is read, or on one another.  (T, d = 4, 16: a 16-bit
+# row set of 128 bytes, a 16-bit vector of 32, fp32 twice that.)
+
+ROWS, VEC = 128, 32
+
+
+@pytest.mark.parametrize("out", ["ro", "no"])
+@pytest.mark.parametrize("read", ["y", "r", "ga"])
+def test_norm_results_on_other_rows(out, read):
+    at = P + 0x60000
+    for off in (-ROWS + 2, -32, 32, ROWS - 2):
+        assert norm(**{out: at + off, read: at}) == mb.ERR_INVALID_ARG
+
+
+def test_norm_results_on_vectors_and_on_one_another():
+    at = P + 0x60000
+    for out in ("ro", "no"):
+        for vec in ("wo", "wn"):
+            for off in (-VEC + 2, 0, ROWS - 2):
+                assert norm(**{out: at, vec: at + off}) == mb.ERR_INVALID_ARG
+    assert norm(ro=at, no=at) == norm(ro=at, no=at + ROWS - 2) == norm(ro=at, no=at - ROWS + 2) == mb.ERR_INVALID_ARG
+    # the same start, but rows of another width lie on other rows
+    assert norm(res32=1, r=at, no=at) == norm(res32=1, y=at, ro=at) == mb.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("out,size", [("d_r", ROWS), ("d_y", ROWS), ("d_g", ROWS), ("d_wo", 64), ("d_wn", 64), ("ws", 256)])
+def test_norm_backward_results_on_other_rows(out, size):
+    at = P + 0x200000
+    names = ["dr", "dn", "r", "y", "ga", "wo", "wn", "d_r", "d_y", "d_g", "d_wo", "d_wn", "ws"]
+    for other in names:
+        if other == out:
+            continue
+        step = 256 if "ws" in (out, other) else 4
+        for off in (-step, 0, step):
+            if off == 0 and other in ("dr", "dn", "r", "y", "ga") and out in ("d_r", "d_y", "d_g") and (out, other) not in (
+                    ("d_r", "y"), ("d_r", "ga")):
+                continue  # the same rows: right
+            if off < 0 and off + {"ws": 256, "d_wo": 64, "d_wn": 64, "wo": VEC, "wn": VEC}.get(other, ROWS) <= 0:
+                continue  # ends before
+            if off > 0 and off >= size:
+                continue  # begins behind
+            assert norm_backward(**{out: at, other: at + off}) == mb.ERR_INVALID_ARG, (other, off)
+
+
+@pytest.mark.parametrize("fn", ["forward", "dgrad", "wgrad"])
+def test_grouped_results_on_what_is_read(fn):
+    at = P + 0x60000
+    size = {"wgrad": 2 * 16 * 16 * 2}.get(fn, ROWS)
+    for read, nbytes in (("x", ROWS), ("w", ROWS if fn == "wgrad" else 1024), ("seg", 12)):
+        for off in (-(nbytes // 16 * 16) + 16 if nbytes > 16 else 0, 0, size - 16):
+            assert grouped(fn, **{"y": at, read: at + off}) == mb.ERR_INVALID_ARG
+    if fn != "wgrad":
+        assert grouped(fn, y=at, se=at + 4) == mb.ERR_INVALID_ARG
+
+
+def test_w4_results_on_what_is_read():
+    at = P + 0x60000
+    size = 4 * 32 * 2
+    for read, nbytes in (("x", 2 * 64 * 2), ("asgn", 16), ("q", 4 * 32 * 32), ("s", 4 * 32 * 2 * 2), ("z", 4 * 32 * 2)):
+        for off in (-nbytes + 16, 0, size - 16):
+            assert w4(**{"out": at, read: at + off}) == mb.ERR_INVALID_ARG

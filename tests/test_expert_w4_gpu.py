@@ -181,6 +181,13 @@ def test_same_bits_streams_and_graphs(cuda):
     check(*p, act="swiglu", got=out)
 
 
+@pytest.mark.gpu
+def test_result_on_the_rows_is_refused(cuda):
+    x, a, wq, ws, wz = make(3, 2, 4, 64, 64, 32, torch.bfloat16, per_slot=True)
+    with pytest.raises(mb.MoEB200Error, match="overlaps"):
+        mb.expert_linear_w4(x, a, wq, ws, out=x.view(6, 64))
+
+
 # ------------------------------------------------------------- refusals ----
 
 def test_refusals():

@@ -285,6 +285,16 @@ def test_streams_and_graphs(cuda):
     assert mb.device_status() == 0
 
 
+@pytest.mark.gpu
+def test_result_on_the_rows_is_refused(cuda):
+    """N = K: the shapes would allow it, but other tiles still read the rows."""
+    x, dy, w, seg = make([30, 50], 64, 64, torch.bfloat16)
+    for f in (lambda: mb.grouped_mm(x, seg, w, out=x), lambda: mb.grouped_mm_dgrad(dy, seg, w, out=dy),
+              lambda: mb.grouped_mm_wgrad(w.view(128, 64), w.view(128, 64), seg, out=w)):
+        with pytest.raises(mb.MoEB200Error, match="overlaps"):
+            f()
+
+
 # ------------------------------------------------------------- refusals ----
 
 def test_refusals():
