@@ -27,7 +27,10 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+// The runtime keeps the thread's last error until it is asked for it; reported
+// here, it must not be reported again by the thread's next launch.
 int cuda_fail(cudaError_t err, const char* where) {
+    cudaGetLastError();
     return fail(MOE_B200_ERR_CUDA, "%s: %s", where, cudaGetErrorString(err));
 }
 

@@ -30,7 +30,10 @@ uint32_t* device_status_word() {
     std::lock_guard<std::mutex> lock(g_mutex);
     if (!g_addr[dev]) {
         void* p = nullptr;
-        if (cudaGetSymbolAddress(&p, g_moe_b200_device_status) != cudaSuccess) return nullptr;
+        if (cudaGetSymbolAddress(&p, g_moe_b200_device_status) != cudaSuccess) {
+            cudaGetLastError();  // the caller reports it
+            return nullptr;
+        }
         g_addr[dev] = static_cast<uint32_t*>(p);
     }
     return g_addr[dev];
