@@ -19,16 +19,21 @@
 // A row belongs to a warp or to a CTA, so that its sums are one or two short
 // reductions, and a thread to fixed columns.  Rows come through a ring of
 // shared-memory stages that bulk copies fill: loads in flight cost no registers.
-// The instructions count nearly as much as the bytes (per element 4 to 7 values
-// are unpacked, and 12 to 30 fp32 operations done): conversions are packed, the
+// The instructions count nearly as much as the bytes (25 an element in the
+// forward, 44 in the backward with a channel gate): conversions are packed, the
 // backward works on pairs of fp32, calls of the usual form have kernels
 // without branches.  Barriers are whole-CTA ones: a named barrier with a
 // register for its number reserves 16 of them, which left 25% occupancy.
 // Measured on one B200 (bf16, cases back to back): forward with both norms and
 // a gate per token, 16384 x 2048: 47 us, 5.7 TB/s, 0.87 of the copy bandwidth;
 // backward with a channel gate, 8192 x 4096: 83 us, 4.8 TB/s (77 us for the
-// rows, where 2.3 instructions a cycle of 4 are issued, and the rest for
-// adding up the CTAs' column sums).
+// rows, where 2.3 instructions a cycle of 4 are issued at 1.88 GHz, and the rest
+// for adding up the CTAs' column sums).
+// Wider rows, 33.5 M elements each, gate per token (floor 41 us, backward 61):
+// 4096 x 8192: 55 us, backward 95; rows of 4104 columns and more need 512
+// threads, whose kernel has 64 registers a thread and spills 4 to 200 bytes of
+// them by form.  6553 x 5120: 68 and 120 (those 512 threads hold 8192 columns);
+// 3276 x 10240: 85 and 237, 2048 x 16384: 67 and 201 (no ring in the backward).
 #include "block_norm.cuh"
 
 namespace moe_b200 {

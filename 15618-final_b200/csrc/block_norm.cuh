@@ -77,8 +77,10 @@ __device__ __forceinline__ float sum2(f32x2 v) {
 //            kind (the grid steps by an even number of rows), so its columns
 //            stay its own.
 //   kSingle  other rows: element by element, neighbours on neighbours
-// (fp16, 3475 x 3545, fp32 residual, gate per token: 49 us in pairs, 69
-// one by one; backward 83 against 133.)
+// 3475 rows of 3545, gate per token, in a captured graph: fp16 with fp32
+// residual 50 us in pairs and 68 one by one, backward 110 and 125; bf16 with
+// bf16 residual 41 and 65, backward 99 and 193.  Rows of 3544, in chunks: 29 and
+// 49, 19 and 40.
 enum { kSingle = 0, kPairs = 1, kChunks = 2 };
 enum { kOddRow = 1, kHalfPair = 2 };  // of `odd`: the row begins inside a word; a pair of this thread has one column only
 template <int AL>
@@ -113,9 +115,11 @@ template <bool F32> struct Raw {
 };
 
 // Pairs: BRANCH puts the columns that are alone in their word behind a branch
-// that few threads take (the backward: 74 us against 88 for 3475 x 3545);
-// otherwise they are predicated accesses, and all of a row's loads start at
-// once (the forward: 40 us against 50).
+// that few threads take; otherwise they are predicated accesses, and all of a
+// row's loads start at once.  The backward takes the branch (rows and types as
+// above: 110 us against 118, bf16 99 against 112; even 3546 columns 93 against
+// 116), the forward does not (50 against 54, bf16 41 against 45; only with 3546
+// columns the branch is better, 46 against 49).
 template <int AL, bool F32, bool BRANCH = false>
 __device__ __forceinline__ Raw<F32> load_raw(const void* row, int chunk, int t, int nt, int d, int odd) {
     Raw<F32> r;

@@ -29,18 +29,19 @@
 //    shared memory in warp order: results do not depend on timing.
 // What bounds it: for one token latency (launch, slot list, one trip to memory
 // for x and for the weights); for batches the work between the MMAs, spread
-// over all of it: about half of the issue slots are used, by 4 warps a
-// scheduler (128 registers each), with 4 instructions a weight and lane
-// (unpacking, x and scales from shared memory and by shuffles, the groups' sums)
-// and stalls on all of these.  The tensor pipe is not it: mma.sync m16n8k16 takes
-// 8 cycles a scheduler, a quarter of the time, and a unit with 8 rows of x costs
+// over all of it, done by 4 warps a scheduler (128 registers each), and their
+// stalls: a pass over a weight executes 2.9 instructions a lane with groups of 128 and
+// up to 8 rows of x (63% of the issue slots at 1.81 GHz) and 5.2 with groups of 32,
+// zero points and up to 16 rows (55%): unpacking, x and scales from shared memory
+// and by shuffles, the groups' sums.  The tensor pipe is not it: mma.sync m16n8k16 takes
+// 8 cycles a scheduler, 21 to 23% of the time, and a unit with 8 rows of x costs
 // about as much as one with 16, so that shares weighted by rows are worse (66 to
 // 78 us against 62).  tcgen05.mma with the unpacked weights in tensor memory was
 // built and measured too: the chain from unpacking to reading the groups'
 // accumulators back is longer (64 tokens 75 us, one token 11, in a graph;
 // this form 50 and 7).  Measured on one B200, 60 experts, 4 a token (bf16, groups
 // of 128, gate/up 2816 x 2048 with SwiGLU): 1 token 12.7 us, 64 tokens 52 us;
-// down 2048 x 1408 (fp16, groups of 32, zero points), 147 tokens: 73 to 81 us by
+// down 2048 x 1408 (fp16, groups of 32, zero points), 147 tokens: 64 to 83 us by
 // routing.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -540,7 +541,12 @@ static cudaError_t launch_w4(const CUtensorMap& map, W4Args a, int served, cudaS
     int64_t grid = 16 / W * device_sm_count();
     // Warps that share a tile's k: few, as each joint costs about as much as a
     // step, but so that every CTA gets several units, and none that loses more
-    // than an eighth of its steps to an uneven split.
+    // than an eighth of its steps to an uneven split.  Shared 1 / 2 / 4 / 8 ways,
+    // us in captured graphs: one token, 4 experts of 2816 x 2048 (8 blocks of k;
+    // 8 taken) 13.8 / 8.8 / 8.4 / 7.6; one row of 4096 x 4096 (8) 23 / 13.7 / 8.7 /
+    // 6.2; 64 tokens (4) 51.1 / 51.1 / 51.2 / 54.3; 147 tokens, 2048 x 1408 (6 blocks;
+    // 2) 67 / 63 / 67 / 72.  The bound on uneven splits is for batches: one
+    // token there takes 9.4 in 2 parts and would take 7.0 in 8.
     const int blocks = (a.K + kW4Block - 1) / kW4Block;
     a.wk = 8;
     while (a.wk > 1 && (8 * blocks < 7 * a.wk * ((blocks + a.wk - 1) / a.wk) ||

@@ -683,20 +683,26 @@ static int form_cols(int form) {
                                : MmGeo<kMmSingle>::kBCols;
 }
 
-// The form of forward and dgrad, from what the host knows (measured on one B200,
-// bf16, routing even / Zipf):
-//  few     segments of at most 16 rows on average: 60 experts of 1408 x 2048:
-//          4 rows 58 / 49 us against 66 / 48 as single tiles, 15 rows 59 / 68
-//          against 68 / 67, 20 rows 63 / 69 against 68 / 68, 40 rows 76 / 90
-//          against 70 / 68; 4 experts of 2816 x 1024, 16 rows: 7.1 against 9.9.
-//          (All 900 rows on one of the 60 experts: 30 against 19.)
-//  narrow  at most two narrow tiles an SM: 1024 rows of one expert, 1408 x 2048
-//          (176 tiles): 13.9 against 14.7 as single tiles; 256 rows (44 tiles)
-//          8.6 against 14.5; 2048 rows (352 tiles) 19.1 against 15.1.
-//  pair    segments of 384 rows on average and two rounds of pair tiles: 60 x
-//          384 rows 282 / 287 us against 292 / 300; with 128 rows 140 / 171
-//          against 140 / 169; with one round (16 x 512 rows of 1024 x 1024) 26
-//          against 21.
+// The form of forward and dgrad, from what the host knows.  Measured on one
+// B200, bf16, in captured graphs, us of forward / dgrad:
+//  few     segments of at most 16 rows on average.  60 experts of 1408 x 2048,
+//          15 rows: even 59 / 59 against 65 / 62 as single tiles, Zipf 61 / 61
+//          against 64 / 60; 20 rows: even 61 / 60 against 67 / 64, Zipf 70 / 67
+//          against 64 / 61; 40 rows: even 78 / 81 against 66 / 63.  4 experts of
+//          2816 x 1024, 16 rows: 8.3 / 12.7 against 11.2 / 12.0 as narrow tiles.
+//          (All 900 rows on one of the 60 experts: 23 / 23 against 16 / 13.)
+//  narrow  at most two narrow tiles an SM.  One expert of 1408 x 2048 (22 / 32
+//          tiles for 128 rows), 256 rows: 10.1 / 8.4 against 16.6 / 13.5 as
+//          single tiles; 1024 rows: 15.9 / 13.1 against 16.4 / 13.8; 2048 rows:
+//          21.5 / 21.6 against 16.8 / 14.3.
+//  pair    segments of 384 rows on average and two rounds of pair tiles.  60
+//          experts of 2816 x 2048, 512 rows: even 311 / 305 against 358 / 347 as
+//          single tiles, Zipf 343 / 342 against 367 / 362; 384 rows: even (every
+//          other pair tile half empty) 278 / 272 against 265 / 252, Zipf 287 /
+//          280 against 298 / 296; 128 rows: even 138 / 137 against 125 / 125,
+//          Zipf 163 / 163 against 156 / 151.  (With 256 rows pairs would win: even
+//          152 / 156 against 174 / 172, Zipf 209 / 204 against 220 / 218.)  One
+//          round (16 x 512 rows of 1024 x 1024): equal, 27 / 27.
 static int mm_form(int mode, int rows, int nseg, int wide) {
     if (mode == kMmWgrad) return kMmSingle;
     const int sms = device_sm_count();
