@@ -207,7 +207,7 @@ struct RowSet {
 };
 // Whether rows share a byte with `out`, whose rows touch one another.
 inline bool rows_overlap(const RowSet& out, const RowSet& in) {
-    if (!out.p || !in.p || out.rows < 1 || in.rows < 1) return false;
+    if (!out.p || !in.p || out.rows < 1 || in.rows < 1 || out.width < 1 || in.width < 1) return false;
     const int64_t lo = int64_t(reinterpret_cast<uintptr_t>(out.p)), hi = lo + out.width * out.rows;
     const int64_t base = int64_t(reinterpret_cast<uintptr_t>(in.p)), end0 = base + in.width;
     const int64_t r = lo < end0 ? 0 : (lo - end0) / in.stride + 1;  // the first row that ends behind `lo`

@@ -128,3 +128,11 @@ def test_w4_results_on_what_is_read():
     for read, nbytes in (("x", 2 * 64 * 2), ("asgn", 16), ("q", 4 * 32 * 32), ("s", 4 * 32 * 2 * 2), ("z", 4 * 32 * 2)):
         for off in (-nbytes + 16, 0, size - 16):
             assert w4(**{"out": at, read: at + off}) == mb.ERR_INVALID_ARG
+
+
+def test_no_bytes_overlap_nothing():
+    """A product without rows has operands of no bytes, wherever they point."""
+    L, at = mb.lib(), P + 0x60000
+    for x in (at - 16, at, at + 512, at + 4096):
+        # (the result overlaps its table, which refuses the call before anything is enqueued)
+        assert L.moe_b200_grouped_mm_wgrad(x, x, at + 4, 2, 0, 16, 16, mb.BF16, at, None) == mb.ERR_INVALID_ARG
