@@ -63,6 +63,7 @@ constexpr int kW4Block = 256;       // k per step
 constexpr int kW4TileRows = 32;     // weight rows per warp step: two 16-row operands
 constexpr int kW4StageBytes = kW4TileRows * kW4Block / 2;
 constexpr int kW4MaxSlots = 4096;
+constexpr int kW4MaxSize = 1 << 29;  // d and N: bytes of a staged row of x and row indices stay 32-bit
 // Dynamic shared memory a CTA may ask for.
 constexpr size_t kW4SmemLimit = 227 * 1024 - 1024;
 
@@ -597,6 +598,8 @@ extern "C" int moe_b200_expert_linear_w4(const void* x, int x_per_slot, const in
     if (d % group != 0) return fail(MOE_B200_ERR_UNSUPPORTED, "expert_linear_w4: d=%d is no multiple of group=%d", d, group);
     if (N % (act == MOE_B200_ACT_SWIGLU ? 16 : 8) != 0)
         return fail(MOE_B200_ERR_UNSUPPORTED, "expert_linear_w4: N=%d must be a multiple of 8 (SwiGLU: 16)", N);
+    if (d > kW4MaxSize || N > kW4MaxSize)
+        return fail(MOE_B200_ERR_UNSUPPORTED, "expert_linear_w4: d and N may be at most %d", kW4MaxSize);
     if (E > MOE_B200_MAX_EXPERTS)
         return fail(MOE_B200_ERR_UNSUPPORTED, "expert_linear_w4: %d experts exceed %d", E, MOE_B200_MAX_EXPERTS);
     if (int64_t(T) * K > kW4MaxSlots)

@@ -77,6 +77,7 @@ constexpr uint32_t kMmBoxBytes = 64 * 64 * 2;            // one MN-major box: 64
 constexpr uint32_t kMmTmemCols = 512;
 constexpr int kMmBufCols = 256;                          // TMEM columns of one accumulator
 constexpr int kMmMaxSegments = 1024;
+constexpr int kMmMaxSize = INT32_MAX - 4095;             // rows, N, K: indices that run past a tile's end stay 32-bit
 constexpr int kSchedSlots = 4;
 enum { kMmFew = 0, kMmSingle = 1, kMmPair = 2, kMmNarrow = 3 };
 template <int FORM> struct MmGeo {
@@ -724,6 +725,8 @@ static int grouped_mm_impl(const char* who, int mode, const void* pa, const void
         return fail(MOE_B200_ERR_INVALID_ARG, "%s: dtype %d is neither F16 nor BF16", who, dtype);
     if (N % 8 != 0 || K % 8 != 0)
         return fail(MOE_B200_ERR_UNSUPPORTED, "%s: N and K must be multiples of 8 (N=%d K=%d)", who, N, K);
+    if (rows > kMmMaxSize || N > kMmMaxSize || K > kMmMaxSize)
+        return fail(MOE_B200_ERR_UNSUPPORTED, "%s: rows, N and K may be at most %d", who, kMmMaxSize);
     if (rows == 0 && mode != kMmWgrad) return MOE_B200_OK;
     if (!seg_start || !out || (rows > 0 && (!pa || !pb)) || (mode != kMmWgrad && !pb))
         return fail(MOE_B200_ERR_INVALID_ARG, "%s: null pointer", who);

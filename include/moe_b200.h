@@ -245,8 +245,9 @@ int moe_b200_ffn_weights_from_reference(const void* w1, const void* w2, int E, i
  * seg_start [nseg + 1] ascending within [0, rows] (held so otherwise);
  * rows outside every segment are left as they were, and a segment whose
  * expert is outside [0, E) gives zeros, whatever its rows hold.  N and K
- * multiples of 8; nseg <= 1024; x, dy, w and the results 16-byte aligned, the
- * tables 4-byte; a result that overlaps an operand is refused; no workspace.
+ * multiples of 8; nseg <= 1024; rows, N and K at most 2^31 - 4096; x, dy, w and
+ * the results 16-byte aligned, the tables 4-byte; a result that overlaps an
+ * operand is refused; no workspace.
  * Replaces the per-expert cublasHgemm calls of apps/bench_e2e.cu:274-301 as
  * single products; the reference has no gradients.  Device-side conditions:
  * moe_b200_device_status().                                                 */
@@ -440,8 +441,9 @@ int moe_b200_block_norm_backward(const void* d_residual_out, const void* d_norme
  *                               silu(y[:, :N/2]) * y[:, N/2:]
  * fp32 accumulation, out rounded once.  The outputs of a down product are
  * combined by moe_b200_unpermute with slot_pos[s] = s.  group 32, 64 or 128
- * and a divisor of d; N a multiple of 8 (SwiGLU: 16); T*K <= 4096; pointers
- * 16-byte aligned (asgn 4-byte); an out that overlaps an operand is refused.
+ * and a divisor of d; N a multiple of 8 (SwiGLU: 16); T*K <= 4096; d and N at
+ * most 2^29; pointers 16-byte aligned (asgn 4-byte); an out that overlaps an
+ * operand is refused.
  * An expert outside [0, E) other than -1 gives zeros too and
  * MOE_B200_DEV_BAD_ASSIGNMENT in moe_b200_device_status().  No counterpart in
  * the reference, whose expert weights are 16-bit.                           */
