@@ -45,7 +45,9 @@
 // warp's elected thread (see elect_one): a K step of a small tile takes 300
 // cycles so, 600 under `lane == 0` (one row, 4096 x 4096: 13.5 us against 22.3).
 // Results leave through TMA stores from the swizzled staging tile.  Every wait
-// is bounded, as in the expert FFN.
+// is bounded, as in the expert FFN; those for a whole tile have 64 ns more for each
+// index of the sum (a 64-wide K step takes 350 ns: a segment of 360 M rows passes
+// the 2 s that a wait has otherwise).
 //
 // Measured on one B200, bf16, back to back (the power limit holds the SM clock
 // near 1.2 to 1.4 GHz then, and cuBLAS at 1340 TFLOP/s for one product of this
@@ -228,6 +230,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &ctl->abort_flag;
+    const uint64_t tile_limit = kWaitLimitNs + uint64_t(MODE == kMmWgrad ? a.rows : a.kdim) * 64;
     // Pair coordinates: rank 0 is the leader, which issues the MMAs and finds the tiles.
     const uint32_t crank = CG == 2 ? cluster_rank() : 0u;
     const int tile0 = CG == 2 ? int(cluster_id_x()) : int(blockIdx.x);
@@ -322,7 +325,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             return n < total_tiles && !__any_sync(0xffffffffu, *abort_flag) ? n : -1;
         }
         const int slot = int(sidx % kSchedSlots);
-        const bool ok = wait_or_abort(&ctl->sched_full[slot], (sidx / kSchedSlots) & 1u, abort_flag, a.status);
+        const bool ok = wait_or_abort(&ctl->sched_full[slot], (sidx / kSchedSlots) & 1u, abort_flag, a.status, tile_limit);
         const int n = ok ? *const_cast<volatile int*>(&ctl->next[slot]) : -1;
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->sched_empty[slot]);
@@ -441,7 +444,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const int nfull = nk - (rem > 0 ? 1 : 0);
             const uint32_t d_tmem = tmem + uint32_t(buf) * kMmBufCols;
             if (elect_one(leader)) {
-                ok = wait_or_abort(&ctl->tmem_empty[buf], ((j >> 1) & 1u) ^ 1u, abort_flag, a.status);
+                ok = wait_or_abort(&ctl->tmem_empty[buf], ((j >> 1) & 1u) ^ 1u, abort_flag, a.status, tile_limit);
                 tc_fence_after();
                 for (int kb = 0; ok && kb < nfull; ++kb) {
                     ok = wait_or_abort(&ctl->full[st], phase, abort_flag, a.status);
@@ -498,7 +501,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const bool by_tma = MODE == kMmWgrad || nrows_w >= 32;
             const int buf = int(j & 1u);
             if (nk > 0) {
-                const bool ok = wait_or_abort(&ctl->tmem_full[buf], (j >> 1) & 1u, abort_flag, a.status);
+                const bool ok = wait_or_abort(&ctl->tmem_full[buf], (j >> 1) & 1u, abort_flag, a.status, tile_limit);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 ++j;
                 tc_fence_after();
@@ -559,7 +562,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         uint32_t asked = 0;
         while (tile >= 0) {
             const int slot = int(sidx % kSchedSlots);
-            bool ok = wait_or_abort(&ctl->sched_empty[slot], ((sidx / kSchedSlots) & 1u) ^ 1u, abort_flag, a.status);
+            bool ok = wait_or_abort(&ctl->sched_empty[slot], ((sidx / kSchedSlots) & 1u) ^ 1u, abort_flag, a.status, tile_limit);
             if (!__all_sync(0xffffffffu, ok)) break;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&ctl->clc_full, 16);

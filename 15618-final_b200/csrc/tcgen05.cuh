@@ -165,13 +165,13 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {
 
 // Bounded wait that also gives up as soon as another role raised the abort.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                              uint32_t* dev_status) {
+                                              uint32_t* dev_status, uint64_t limit_ns = kWaitLimitNs) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     while (true) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (globaltimer_ns() - t0 > limit_ns) {
             *abort_flag = 1;
             atomicOr(dev_status, MOE_B200_DEV_WAIT_TIMEOUT);
             return false;

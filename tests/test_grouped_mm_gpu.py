@@ -254,6 +254,23 @@ def test_offsets_past_32_bits(cuda):
 
 
 @pytest.mark.gpu
+def test_sums_that_take_longer_than_a_wait(cuda):
+    """One segment of 450 million rows: a tile takes 2.5 s, longer than a wait
+    without regard to the sum's length.  All rows but the first and last 2000 are
+    zeros, which add nothing, so the tolerance is that of 4000 rows."""
+    rows, n = 450_000_000, 2000
+    dy, x = (torch.zeros((rows, 8), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for t in (dy, x):
+        for at in (slice(0, n), slice(rows - n, rows)):
+            t[at] = torch.randn((n, 8), generator=g, device="cuda").bfloat16()
+    dw = mb.grouped_mm_wgrad(dy, x, torch.tensor([0, rows], dtype=torch.int32, device="cuda"))
+    assert mb.device_status() == 0
+    ends = [torch.cat([t[:n], t[rows - n:]]) for t in (dy, x)]
+    assert_close(dw[0], ends[0].T, ends[1], "dw")
+
+
+@pytest.mark.gpu
 def test_matches_the_two_product_ffn(cuda):
     """Two grouped products are the plain FFN, bit for bit."""
     x, _, w_up, seg = make([100, 0, 300, 17], 128, 96, torch.bfloat16)
