@@ -79,6 +79,7 @@ struct FfnSmem {
     uint64_t empty[kMaxStages];
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
+    uint64_t drained;  // after a wait gave up: the MMAs in flight are through
     uint32_t tmem_base;
     int abort_flag;
     int nseg;
@@ -156,6 +157,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             mbar_init(&ctl->tmem_full[b], 1);
             mbar_init(&ctl->tmem_empty[b], 4 * CG);  // epilogue warps of every CTA of the group
         }
+        mbar_init(&ctl->drained, 1);
         ctl->abort_flag = 0;
         mbar_fence_init();
     }
@@ -441,6 +443,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     __syncthreads();
     // expert parallel: the last CTA to finish raises the senders' back flags
     if (sig.peer && threadIdx.x == 0) ep_signal_done(sig, *abort_flag != 0);
+    // After a wait gave up nobody has waited for the last MMAs, which must not
+    // run into the TMEM and shared memory of the next CTA.
+    if (warp == 1 && lane == 0 && crank == 0 && *abort_flag) {
+        if (CG == 1) umma_commit(&ctl->drained);
+        else umma_commit_pair(map_to_rank(&ctl->drained, 0));
+        mbar_wait(&ctl->drained, 0);
+    }
     if (CG == 2) cluster_sync();  // no CTA leaves while its pair may still signal it
     tc_fence_after();
     if (warp == 1) {

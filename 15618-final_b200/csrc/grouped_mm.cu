@@ -104,6 +104,7 @@ struct MmSmem {
     uint64_t sched_full[kSchedSlots];
     uint64_t sched_empty[kSchedSlots];
     uint64_t clc_full;  // answers of cluster launch control
+    uint64_t drained;   // after a wait gave up: the MMAs in flight are through
     uint4 clc;
     int next[kSchedSlots];  // tiles handed to the warps
     uint32_t tmem_base;
@@ -250,6 +251,7 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             mbar_init(&ctl->sched_empty[b], 7);  // one arrival per warp
         }
         mbar_init(&ctl->clc_full, 1);
+        mbar_init(&ctl->drained, 1);
         ctl->abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tmap_a);
@@ -589,6 +591,17 @@ grouped_mm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
     tc_fence_before();
     __syncthreads();
+    // After a wait gave up nobody has waited for the last MMAs, which must not
+    // run into the TMEM and shared memory of the next CTA.
+    if (warp == 1 && crank == 0 && *abort_flag) {
+        int issuer;
+        if (elect_one(issuer)) {
+            if (CG == 1) umma_commit(&ctl->drained);
+            else umma_commit_both(&ctl->drained);
+            mbar_wait(&ctl->drained, 0);
+        }
+        __syncwarp();
+    }
     if (CG == 2) cluster_sync();  // no CTA leaves while its pair may still signal it
     tc_fence_after();
     if (warp == 1) {
