@@ -512,20 +512,43 @@ def _on_device(dev, fn, *args):
         return fn(*args)
 
 
-def _enqueue(what, fn, dev, stream, fresh, *args):
-    """Calls fn(*args, stream) with `dev` current.  `fresh`: tensors that this
-    call allocated, which the allocator must not hand out again before the
-    work on `stream` is done."""
+def _other_stream(dev, stream):
+    """`stream` (a torch stream or a raw handle) as a torch stream; None where
+    it is the current one of `dev`."""
     import torch
-    index = dev.index
-    handle = torch._C._cuda_getCurrentRawStream(index) or None
-    if stream is not None:
-        current, handle = handle, _stream_handle(stream)
-        if handle != current:
-            s = torch.cuda.ExternalStream(handle or 0, device=dev)
-            for t in fresh:
-                if t is not None:
-                    t.record_stream(s)
+    if stream is None:
+        return None
+    handle = _stream_handle(stream) or 0
+    if handle == torch._C._cuda_getCurrentRawStream(dev.index):
+        return None
+    if not isinstance(stream, int):
+        return stream
+    return torch.cuda.ExternalStream(handle, device=dev) if handle else torch.cuda.default_stream(dev)
+
+
+def _fresh(dev, stream, alloc):
+    """alloc()'s tensors (or Nones), which a call will write on `stream`.
+    Where that is another stream than the current one they are allocated on it,
+    since memory that the current stream's earlier work still uses may be handed
+    out to the current stream alone; and they are kept from reuse until the
+    current stream, on which the caller goes on, is through with them too."""
+    import torch
+    other = _other_stream(dev, stream)
+    if other is None:
+        return alloc()
+    with torch.cuda.stream(other):
+        got = alloc()
+    here = torch.cuda.current_stream(dev)
+    for t in got:
+        if t is not None:
+            t.record_stream(here)
+    return got
+
+
+def _enqueue(what, fn, dev, stream, *args):
+    """Calls fn(*args, stream) with `dev` current."""
+    import torch
+    handle = torch._C._cuda_getCurrentRawStream(dev.index) or None if stream is None else _stream_handle(stream)
     status = _on_device(dev, fn, *args, handle)
     if status != OK:
         _check(status, what)
@@ -611,12 +634,11 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
     T, d, dtype, code, res32, form, res_stride, y_stride = _check_block_norm("block_norm", residual, y, w_post, w_pre,
                                                                               gate)
     dev = _same_device("block_norm", residual, y, w_post, w_pre, gate)
-    fresh = ()
     if out is None:
         like, plain = torch.empty_like, torch.contiguous_format
-        fresh = out = BlockNormResult(
+        out = _fresh(dev, stream, lambda: BlockNormResult(
             like(residual, memory_format=plain) if y is not None else None,
-            like(residual, dtype=dtype, memory_format=plain) if w_pre is not None else None)
+            like(residual, dtype=dtype, memory_format=plain) if w_pre is not None else None))
     else:
         if (out.residual_out is None) != (y is None) or (out.normed is None) != (w_pre is None):
             _refuse("block_norm", "out needs residual_out with y and normed with w_pre, and neither without")
@@ -627,7 +649,7 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
             _rows("block_norm", "out.normed", out.normed, (T, d), dtype)
     if T == 0:
         return out if y is not None else BlockNormResult(residual, out.normed)
-    _enqueue("block_norm", lib().moe_b200_block_norm, dev, stream, fresh,
+    _enqueue("block_norm", lib().moe_b200_block_norm, dev, stream,
              _ptr(y), y_stride, _ptr(residual), res_stride, res32, _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale,
              eps, T, d, code, _ptr(out.residual_out), _ptr(out.normed))
     return out if y is not None else BlockNormResult(residual, out.normed)
@@ -657,20 +679,21 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
 
     like, plain = torch.empty_like, torch.contiguous_format
     f32 = torch.float32
-    got = BlockNormGrads(
+    *got, ws = _fresh(dev, stream, lambda: (
         like(residual_out, memory_format=plain),
         like(y, memory_format=plain) if y is not None else None,
         like(w_post, dtype=f32) if w_post is not None else None,
         like(w_pre, dtype=f32) if w_pre is not None else None,
-        None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32))
+        None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32),
+        residual_out.new_empty((max(nbytes, 256),), dtype=torch.uint8)))
+    got = BlockNormGrads(*got)
     if T == 0:  # sums over no token
-        with torch.cuda.stream(stream if not isinstance(stream, int) else torch.cuda.ExternalStream(stream, device=dev)):
+        with torch.cuda.stream(_other_stream(dev, stream)):
             for t in got[2:]:
                 if t is not None:
                     t.zero_()
         return got
-    ws = residual_out.new_empty((max(nbytes, 256),), dtype=torch.uint8)
-    _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream, (*got, ws),
+    _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream,
              _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), res_stride, res32, _ptr(y), y_stride,
              _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d, code, _ptr(got.d_residual),
              _ptr(got.d_y), _ptr(got.d_w_post), _ptr(got.d_w_pre), _ptr(got.d_gate), _ptr(ws), nbytes)
@@ -695,13 +718,11 @@ def _grouped_mm(what, fn, rows_in, seg_start, w, seg_expert, out, stream, forwar
     elif nseg > E:
         _refuse(what, f"{nseg} segments for {E} experts need seg_expert")
     dev = _same_device(what, rows_in, seg_start, w, seg_expert, out)
-    fresh = ()
     if out is None:
-        out = rows_in.new_empty((rows, width_out))
-        fresh = (out,)
+        out, = _fresh(dev, stream, lambda: (rows_in.new_empty((rows, width_out)),))
     else:
         _rows(what, "out", out, (rows, width_out), dtype)
-    _enqueue(what, fn, dev, stream, fresh, _ptr(rows_in), _ptr(seg_start), _ptr(seg_expert), nseg, rows, N, K, E,
+    _enqueue(what, fn, dev, stream, _ptr(rows_in), _ptr(seg_start), _ptr(seg_expert), nseg, rows, N, K, E,
              _ptr(w), code, _ptr(out))
     return out
 
@@ -739,13 +760,11 @@ def grouped_mm_wgrad(dy, x, seg_start, out=None, stream=None):
     _rows(what, "x", x, (rows, K), dtype)
     _rows(what, "seg_start", seg_start, (nseg + 1,), torch.int32)
     dev = _same_device(what, x, dy, seg_start, out)
-    fresh = ()
     if out is None:
-        out = x.new_empty((nseg, N, K))
-        fresh = (out,)
+        out, = _fresh(dev, stream, lambda: (x.new_empty((nseg, N, K)),))
     else:
         _rows(what, "out", out, (nseg, N, K), dtype)
-    _enqueue(what, lib().moe_b200_grouped_mm_wgrad, dev, stream, fresh, _ptr(dy), _ptr(x), _ptr(seg_start), nseg, rows,
+    _enqueue(what, lib().moe_b200_grouped_mm_wgrad, dev, stream, _ptr(dy), _ptr(x), _ptr(seg_start), nseg, rows,
              N, K, code, _ptr(out))
     return out
 
@@ -783,13 +802,11 @@ def expert_linear_w4(x, asgn, w_q, w_scale, w_zero=None, act=None, out=None, str
         _rows(what, "w_zero", w_zero, (E, N, groups), torch.uint8)
     n_out = N // 2 if act else N
     dev = _same_device(what, x, asgn, w_q, w_scale, w_zero, out)
-    fresh = ()
     if out is None:
-        out = x.new_empty((T * K, n_out))
-        fresh = (out,)
+        out, = _fresh(dev, stream, lambda: (x.new_empty((T * K, n_out)),))
     else:
         _rows(what, "out", out, (T * K, n_out), dtype)
-    _enqueue(what, lib().moe_b200_expert_linear_w4, dev, stream, fresh,
+    _enqueue(what, lib().moe_b200_expert_linear_w4, dev, stream,
              _ptr(x), int(x.dim() == 3), _ptr(asgn), T, K, E, d, N, _ptr(w_q), _ptr(w_scale), _ptr(w_zero), d // groups,
              ACT_SWIGLU if act else ACT_NONE, code, _ptr(out))
     return out
