@@ -172,6 +172,44 @@ def _stream_handle(stream) -> Optional[int]:
     return stream.cuda_stream or None
 
 
+def _other_stream(dev, stream):
+    """`stream` (a torch stream or a raw handle) as a torch stream; None where
+    it is the current one of `dev`."""
+    import torch
+    if stream is None:
+        return None
+    handle = _stream_handle(stream) or 0
+    if handle == torch._C._cuda_getCurrentRawStream(dev.index):
+        return None
+    if not isinstance(stream, int):
+        return stream
+    return torch.cuda.ExternalStream(handle, device=dev) if handle else torch.cuda.default_stream(dev)
+
+
+def _fresh(dev, stream, alloc):
+    """alloc()'s tensors (or Nones), which a call will write on `stream`.
+    Where that is another stream than the current one they are allocated on it,
+    since memory that the current stream's earlier work still uses may be handed
+    out to the current stream alone; and they are kept from reuse until the
+    current stream, on which the caller goes on, is through with them too."""
+    if stream is None:
+        return alloc()
+    import torch
+    dev = torch.device(dev)
+    if dev.index is None:
+        dev = torch.device(dev.type, torch.cuda.current_device())
+    other = _other_stream(dev, stream)
+    if other is None:
+        return alloc()
+    with torch.cuda.stream(other):
+        got = alloc()
+    here = torch.cuda.current_stream(dev)
+    for t in got:
+        if t is not None:
+            t.record_stream(here)
+    return got
+
+
 # --------------------------------------------------------------------------
 # The reference interface
 # --------------------------------------------------------------------------
@@ -284,7 +322,7 @@ class Workspace:
     def __init__(self, T: int, K: int, E: int, device="cuda", stream=None):
         import torch
         self.nbytes = max(pack_workspace_bytes(T, K, E), 256)
-        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+        self.buf, = _fresh(device, stream, lambda: (torch.empty(self.nbytes, dtype=torch.uint8, device=device),))
         self.shape = (T, K, E)
         _check(lib().moe_b200_workspace_init(self.buf.data_ptr(), self.nbytes, _stream_handle(stream)),
                "workspace_init")
@@ -313,14 +351,14 @@ def pack(emb, asgn, wts, E: int, workspace: Optional[Workspace] = None, out: Opt
     if workspace is None:
         workspace = Workspace(T, K, E, device=dev, stream=stream)
     if out is None:
-        out = PackResult(
+        out = _fresh(dev, stream, lambda: PackResult(
             packed=torch.empty((TK, d), dtype=emb.dtype, device=dev) if rows else None,
             packed_weights=torch.empty(TK, dtype=torch.float32, device=dev) if wts is not None else None,
             perm=torch.empty(TK, dtype=torch.int32, device=dev),
             expert_count=torch.empty(E, dtype=torch.int32, device=dev),
             expert_start=torch.empty(E + 1, dtype=torch.int32, device=dev),
             slot_pos=torch.empty(TK, dtype=torch.int32, device=dev),
-        )
+        ))
     _check(lib().moe_b200_pack(
         _ptr(emb), _ptr(asgn), _ptr(wts), T, K, E, d,
         _ptr(out.packed), _ptr(out.packed_weights), _ptr(out.perm),
@@ -351,7 +389,7 @@ def unpermute(y, packed_weights, slot_pos, T: int, K: int, out=None, stream=None
     import torch
     d = y.shape[1]
     if out is None:
-        out = torch.empty((T, d), dtype=y.dtype, device=y.device)
+        out, = _fresh(y.device, stream, lambda: (torch.empty((T, d), dtype=y.dtype, device=y.device),))
     _check(lib().moe_b200_unpermute(_ptr(y), _ptr(packed_weights), _ptr(slot_pos), T, K, d,
                                     dtype_code(y.dtype), _ptr(out), _stream_handle(stream)),
            "unpermute")
@@ -375,9 +413,9 @@ def grouped_swiglu(x, seg_start, w_gate_up, w_down, seg_expert=None, h=None, y=N
     I = two_i // 2
     nseg = seg_start.numel() - 1
     if h is None:
-        h = torch.empty((rows, I), dtype=x.dtype, device=x.device)
+        h, = _fresh(x.device, stream, lambda: (torch.empty((rows, I), dtype=x.dtype, device=x.device),))
     if y is None:
-        y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
+        y, = _fresh(x.device, stream, lambda: (torch.empty((rows, d), dtype=x.dtype, device=x.device),))
     if row_token is not None:
         _check(lib().moe_b200_grouped_swiglu_gather(_ptr(x), T, _ptr(row_token), _ptr(seg_start), _ptr(seg_expert),
                                                     nseg, rows, d, I, E, _ptr(w_gate_up), _ptr(w_down),
@@ -400,9 +438,9 @@ def grouped_ffn(x, seg_start, w_up, w_down, seg_expert=None, mid=None, y=None, s
     E, F, _ = w_up.shape
     nseg = seg_start.numel() - 1
     if mid is None:
-        mid = torch.empty((rows, F), dtype=x.dtype, device=x.device)
+        mid, = _fresh(x.device, stream, lambda: (torch.empty((rows, F), dtype=x.dtype, device=x.device),))
     if y is None:
-        y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
+        y, = _fresh(x.device, stream, lambda: (torch.empty((rows, d), dtype=x.dtype, device=x.device),))
     _check(lib().moe_b200_grouped_ffn(_ptr(x), _ptr(seg_start), _ptr(seg_expert), nseg, rows, d, F, E, _ptr(w_up),
                                       _ptr(w_down), dtype_code(x.dtype), _ptr(mid), _ptr(y), _stream_handle(stream)),
            "grouped_ffn")
@@ -415,9 +453,11 @@ def ffn_weights_from_reference(w1, w2, stream=None):
     (w_up [E, F, d], w_down [E, d, F]), transposed on the device."""
     import torch
     E, d, F = w1.shape
-    w_up = torch.empty((E, F, d), dtype=w1.dtype, device=w1.device)
-    w_down = torch.empty((E, d, F), dtype=w1.dtype, device=w1.device)
-    _check(lib().moe_b200_ffn_weights_from_reference(_ptr(w1.contiguous()), _ptr(w2.contiguous()), E, d, F,
+    # (a copy that contiguous() makes is read on `stream` too: made there)
+    w_up, w_down, w1, w2 = _fresh(w1.device, stream, lambda: (
+        torch.empty((E, F, d), dtype=w1.dtype, device=w1.device),
+        torch.empty((E, d, F), dtype=w1.dtype, device=w1.device), w1.contiguous(), w2.contiguous()))
+    _check(lib().moe_b200_ffn_weights_from_reference(_ptr(w1), _ptr(w2), E, d, F,
                                                      _ptr(w_up), _ptr(w_down), _stream_handle(stream)),
            "ffn_weights_from_reference")
     return w_up, w_down
@@ -437,8 +477,9 @@ class RouterWeights:
         nbytes = lib().moe_b200_router_weights_bytes(self.d, self.E, dtype_code(dtype))
         if nbytes == 0:
             raise MoEB200Error(ERR_INVALID_ARG, f"RouterWeights: bad shape d={self.d} E={self.E}")
-        self.buf = torch.empty(nbytes, dtype=torch.uint8, device=w_gate.device)
-        _check(lib().moe_b200_router_prepare(_ptr(w_gate.contiguous()), self.d, self.E, dtype_code(dtype),
+        self.buf, w_gate = _fresh(w_gate.device, stream, lambda: (
+            torch.empty(nbytes, dtype=torch.uint8, device=w_gate.device), w_gate.contiguous()))
+        _check(lib().moe_b200_router_prepare(_ptr(w_gate), self.d, self.E, dtype_code(dtype),
                                              _ptr(self.buf), _stream_handle(stream)), "router_prepare")
 
 
@@ -450,8 +491,8 @@ def route(x, weights, K, out=None, stream=None):
     import torch
     T, d = x.shape
     if out is None:
-        out = (torch.empty((T, K), dtype=torch.int32, device=x.device),
-               torch.empty((T, K), dtype=torch.float32, device=x.device))
+        out = _fresh(x.device, stream, lambda: (torch.empty((T, K), dtype=torch.int32, device=x.device),
+                                                torch.empty((T, K), dtype=torch.float32, device=x.device)))
     _check(lib().moe_b200_route(_ptr(x), T, d, weights.E, K, dtype_code(x.dtype), _ptr(weights.buf),
                                 _ptr(out[0]), _ptr(out[1]), _stream_handle(stream)), "route")
     return out
@@ -467,10 +508,10 @@ def ep_layout(all_counts, rank, expert_first, out=None, stream=None):
     L = expert_first[rank + 1] - expert_first[rank]
     dev = all_counts.device
     if out is None:
-        out = (torch.empty(N * L + 1, dtype=torch.int32, device=dev),
-               torch.empty(max(N * L, 1), dtype=torch.int32, device=dev),
-               torch.empty(N, dtype=torch.int32, device=dev),
-               torch.empty(N, dtype=torch.int32, device=dev))
+        out = _fresh(dev, stream, lambda: (torch.empty(N * L + 1, dtype=torch.int32, device=dev),
+                                           torch.empty(max(N * L, 1), dtype=torch.int32, device=dev),
+                                           torch.empty(N, dtype=torch.int32, device=dev),
+                                           torch.empty(N, dtype=torch.int32, device=dev)))
     first = (ctypes.c_int32 * (N + 1))(*expert_first)
     _check(lib().moe_b200_ep_layout(_ptr(all_counts), N, E, rank, first, _ptr(out[0]), _ptr(out[1]),
                                     _ptr(out[2]), _ptr(out[3]), _stream_handle(stream)), "ep_layout")
@@ -510,39 +551,6 @@ def _on_device(dev, fn, *args):
         return fn(*args)
     with torch.cuda.device(dev):
         return fn(*args)
-
-
-def _other_stream(dev, stream):
-    """`stream` (a torch stream or a raw handle) as a torch stream; None where
-    it is the current one of `dev`."""
-    import torch
-    if stream is None:
-        return None
-    handle = _stream_handle(stream) or 0
-    if handle == torch._C._cuda_getCurrentRawStream(dev.index):
-        return None
-    if not isinstance(stream, int):
-        return stream
-    return torch.cuda.ExternalStream(handle, device=dev) if handle else torch.cuda.default_stream(dev)
-
-
-def _fresh(dev, stream, alloc):
-    """alloc()'s tensors (or Nones), which a call will write on `stream`.
-    Where that is another stream than the current one they are allocated on it,
-    since memory that the current stream's earlier work still uses may be handed
-    out to the current stream alone; and they are kept from reuse until the
-    current stream, on which the caller goes on, is through with them too."""
-    import torch
-    other = _other_stream(dev, stream)
-    if other is None:
-        return alloc()
-    with torch.cuda.stream(other):
-        got = alloc()
-    here = torch.cuda.current_stream(dev)
-    for t in got:
-        if t is not None:
-            t.record_stream(here)
-    return got
 
 
 def _enqueue(what, fn, dev, stream, *args):

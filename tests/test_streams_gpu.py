@@ -31,10 +31,28 @@ def operators():
             "w4": lambda s: (mb.expert_linear_w4(xq, a, wq, ws, stream=s),)}
 
 
-@pytest.mark.parametrize("op", ["norm", "norm_backward", "grouped_mm", "dgrad", "wgrad", "w4"])
+def layer_operators():
+    x, wts = rand((T, D), 1), torch.rand((T, 1), device="cuda")
+    a = torch.randint(0, 4, (T, 1), device="cuda", dtype=torch.int32)
+    up, down, seg = rand((1, D, D), 4, 0.02), rand((1, D, D), 5, 0.02), torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    gate_up, pos = rand((1, 2 * D, D), 6, 0.02), torch.arange(T, dtype=torch.int32, device="cuda")
+    w_gate = torch.randn((D, 8), device="cuda")
+    return {"pack": lambda s: mb.pack(x, a, wts, 4, stream=s)[:1],
+            "ffn": lambda s: mb.grouped_ffn(x, seg, up, down, stream=s),
+            "swiglu": lambda s: mb.grouped_swiglu(x, seg, gate_up, down, stream=s),
+            "unpermute": lambda s: (mb.unpermute(x, wts, pos, T, 1, stream=s),),
+            "weights": lambda s: mb.ffn_weights_from_reference(up, down, stream=s),
+            "route": lambda s: mb.route(x, mb.RouterWeights(w_gate, torch.bfloat16, stream=s), 8, stream=s)}
+
+
+@pytest.mark.parametrize("op", ["norm", "norm_backward", "grouped_mm", "dgrad", "wgrad", "w4",
+                                "pack", "ffn", "swiglu", "unpermute", "weights", "route"])
 @pytest.mark.parametrize("by_handle", [False, True])
 def test_results_do_not_take_memory_that_the_current_stream_still_reads(cuda, op, by_handle):
-    call = operators()[op]
+    keep_what_is_read((operators() | layer_operators())[op], by_handle)
+
+
+def keep_what_is_read(call, by_handle):
     side = torch.cuda.Stream()
     want = [t.clone() for t in call(None)]
     torch.cuda.synchronize()
