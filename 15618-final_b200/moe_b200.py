@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
@@ -210,6 +211,42 @@ def _fresh(dev, stream, alloc):
     return got
 
 
+def _new(like, shape, dev, stream, dtype=None):
+    """An empty tensor beside `like`, which a call will write on `stream`."""
+    if stream is None:
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
+    return _fresh(dev, stream, lambda: (like.new_empty(shape, dtype=dtype),))[0]
+
+
+def _device_of(t):
+    """The device that a call on this tensor runs on."""
+    return t.device
+
+
+def _on_device(dev, fn, *args):
+    """fn(*args) with `dev` current."""
+    torch = sys.modules["torch"]
+    if torch._C._cuda_getDevice() == dev.index:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
+def _enqueue(what, fn, dev, stream, *args):
+    """Calls fn(*args, stream) with `dev` current (stream None: its current one)."""
+    index = dev.index
+    if index is None:
+        raise MoEB200Error(ERR_INVALID_ARG, f"{what}: tensors must be on a CUDA device, got {dev}")
+    cuda = sys.modules["torch"]._C  # (there are tensors, so it is loaded)
+    handle = (cuda._cuda_getCurrentRawStream(index) or None) if stream is None else _stream_handle(stream)
+    if cuda._cuda_getDevice() == index:
+        status = fn(*args, handle)
+    else:
+        status = _on_device(dev, fn, *args, handle)
+    if status != OK:
+        _check(status, what)
+
+
 # --------------------------------------------------------------------------
 # The reference interface
 # --------------------------------------------------------------------------
@@ -278,17 +315,17 @@ class B200Scatter:
 
     def run(self, d_emb, d_asgn, d_wts, bufs: MoEBuffers, p: MoEParams, stream=None,
             slot_pos=None) -> ScatterTimings:
-        s = _stream_handle(stream)
+        dev = _device_of(d_emb)
         key = (_ptr(bufs.strategy_ws), bufs.strategy_ws_bytes, p.T, p.K, p.E)
         if key != self._ws_key:
-            _check(lib().moe_b200_workspace_init(_ptr(bufs.strategy_ws), bufs.strategy_ws_bytes, s),
-                   "workspace_init")
+            _enqueue("workspace_init", lib().moe_b200_workspace_init, dev, stream, _ptr(bufs.strategy_ws),
+                     bufs.strategy_ws_bytes)
             self._ws_key = key
-        _check(lib().moe_b200_pack(
-            _ptr(d_emb), _ptr(d_asgn), _ptr(d_wts), p.T, p.K, p.E, p.d_model,
-            _ptr(bufs.packed), _ptr(bufs.packed_weights), _ptr(bufs.perm),
-            _ptr(bufs.expert_count), _ptr(bufs.expert_start), _ptr(slot_pos),
-            _ptr(bufs.strategy_ws), bufs.strategy_ws_bytes, s), "pack")
+        _enqueue("pack", lib().moe_b200_pack, dev, stream,
+                 _ptr(d_emb), _ptr(d_asgn), _ptr(d_wts), p.T, p.K, p.E, p.d_model,
+                 _ptr(bufs.packed), _ptr(bufs.packed_weights), _ptr(bufs.perm),
+                 _ptr(bufs.expert_count), _ptr(bufs.expert_start), _ptr(slot_pos),
+                 _ptr(bufs.strategy_ws), bufs.strategy_ws_bytes)
         return ScatterTimings()
 
 
@@ -324,18 +361,19 @@ class Workspace:
         self.nbytes = max(pack_workspace_bytes(T, K, E), 256)
         self.buf, = _fresh(device, stream, lambda: (torch.empty(self.nbytes, dtype=torch.uint8, device=device),))
         self.shape = (T, K, E)
-        _check(lib().moe_b200_workspace_init(self.buf.data_ptr(), self.nbytes, _stream_handle(stream)),
-               "workspace_init")
+        _enqueue("workspace_init", lib().moe_b200_workspace_init, _device_of(self.buf), stream, self.buf.data_ptr(),
+                 self.nbytes)
 
     def fits(self, T, K, E) -> bool:
         return pack_workspace_bytes(T, K, E) <= self.nbytes
 
     def device_status(self, stream=None) -> int:
         """Synchronise and return (and clear) the device condition bits."""
+        import torch
         out = ctypes.c_int(0)
-        _check(lib().moe_b200_workspace_status(self.buf.data_ptr(), self.nbytes,
-                                               _stream_handle(stream), ctypes.byref(out)),
-               "workspace_status")
+        with torch.cuda.device(_device_of(self.buf)):
+            _check(lib().moe_b200_workspace_status(self.buf.data_ptr(), self.nbytes, _stream_handle(stream),
+                                                   ctypes.byref(out)), "workspace_status")
         return out.value
 
 
@@ -359,11 +397,11 @@ def pack(emb, asgn, wts, E: int, workspace: Optional[Workspace] = None, out: Opt
             expert_start=torch.empty(E + 1, dtype=torch.int32, device=dev),
             slot_pos=torch.empty(TK, dtype=torch.int32, device=dev),
         ))
-    _check(lib().moe_b200_pack(
-        _ptr(emb), _ptr(asgn), _ptr(wts), T, K, E, d,
-        _ptr(out.packed), _ptr(out.packed_weights), _ptr(out.perm),
-        _ptr(out.expert_count), _ptr(out.expert_start), _ptr(out.slot_pos),
-        workspace.buf.data_ptr(), workspace.nbytes, _stream_handle(stream)), "pack")
+    _enqueue("pack", lib().moe_b200_pack, _device_of(emb), stream,
+             _ptr(emb), _ptr(asgn), _ptr(wts), T, K, E, d,
+             _ptr(out.packed), _ptr(out.packed_weights), _ptr(out.perm),
+             _ptr(out.expert_count), _ptr(out.expert_start), _ptr(out.slot_pos),
+             workspace.buf.data_ptr(), workspace.nbytes)
     return out
 
 
@@ -390,9 +428,8 @@ def unpermute(y, packed_weights, slot_pos, T: int, K: int, out=None, stream=None
     d = y.shape[1]
     if out is None:
         out, = _fresh(y.device, stream, lambda: (torch.empty((T, d), dtype=y.dtype, device=y.device),))
-    _check(lib().moe_b200_unpermute(_ptr(y), _ptr(packed_weights), _ptr(slot_pos), T, K, d,
-                                    dtype_code(y.dtype), _ptr(out), _stream_handle(stream)),
-           "unpermute")
+    _enqueue("unpermute", lib().moe_b200_unpermute, _device_of(y), stream, _ptr(y), _ptr(packed_weights), _ptr(slot_pos),
+             T, K, d, dtype_code(y.dtype), _ptr(out))
     return out
 
 
@@ -417,14 +454,12 @@ def grouped_swiglu(x, seg_start, w_gate_up, w_down, seg_expert=None, h=None, y=N
     if y is None:
         y, = _fresh(x.device, stream, lambda: (torch.empty((rows, d), dtype=x.dtype, device=x.device),))
     if row_token is not None:
-        _check(lib().moe_b200_grouped_swiglu_gather(_ptr(x), T, _ptr(row_token), _ptr(seg_start), _ptr(seg_expert),
-                                                    nseg, rows, d, I, E, _ptr(w_gate_up), _ptr(w_down),
-                                                    dtype_code(x.dtype), _ptr(h), _ptr(y), _stream_handle(stream)),
-               "grouped_swiglu_gather")
+        _enqueue("grouped_swiglu_gather", lib().moe_b200_grouped_swiglu_gather, _device_of(x), stream, _ptr(x), T,
+                 _ptr(row_token), _ptr(seg_start), _ptr(seg_expert), nseg, rows, d, I, E, _ptr(w_gate_up), _ptr(w_down),
+                 dtype_code(x.dtype), _ptr(h), _ptr(y))
         return h, y
-    _check(lib().moe_b200_grouped_swiglu(_ptr(x), _ptr(seg_start), _ptr(seg_expert), nseg, rows, d, I, E,
-                                         _ptr(w_gate_up), _ptr(w_down), dtype_code(x.dtype), _ptr(h), _ptr(y),
-                                         _stream_handle(stream)), "grouped_swiglu")
+    _enqueue("grouped_swiglu", lib().moe_b200_grouped_swiglu, _device_of(x), stream, _ptr(x), _ptr(seg_start),
+             _ptr(seg_expert), nseg, rows, d, I, E, _ptr(w_gate_up), _ptr(w_down), dtype_code(x.dtype), _ptr(h), _ptr(y))
     return h, y
 
 
@@ -441,9 +476,8 @@ def grouped_ffn(x, seg_start, w_up, w_down, seg_expert=None, mid=None, y=None, s
         mid, = _fresh(x.device, stream, lambda: (torch.empty((rows, F), dtype=x.dtype, device=x.device),))
     if y is None:
         y, = _fresh(x.device, stream, lambda: (torch.empty((rows, d), dtype=x.dtype, device=x.device),))
-    _check(lib().moe_b200_grouped_ffn(_ptr(x), _ptr(seg_start), _ptr(seg_expert), nseg, rows, d, F, E, _ptr(w_up),
-                                      _ptr(w_down), dtype_code(x.dtype), _ptr(mid), _ptr(y), _stream_handle(stream)),
-           "grouped_ffn")
+    _enqueue("grouped_ffn", lib().moe_b200_grouped_ffn, _device_of(x), stream, _ptr(x), _ptr(seg_start), _ptr(seg_expert),
+             nseg, rows, d, F, E, _ptr(w_up), _ptr(w_down), dtype_code(x.dtype), _ptr(mid), _ptr(y))
     return mid, y
 
 
@@ -457,9 +491,8 @@ def ffn_weights_from_reference(w1, w2, stream=None):
     w_up, w_down, w1, w2 = _fresh(w1.device, stream, lambda: (
         torch.empty((E, F, d), dtype=w1.dtype, device=w1.device),
         torch.empty((E, d, F), dtype=w1.dtype, device=w1.device), w1.contiguous(), w2.contiguous()))
-    _check(lib().moe_b200_ffn_weights_from_reference(_ptr(w1), _ptr(w2), E, d, F,
-                                                     _ptr(w_up), _ptr(w_down), _stream_handle(stream)),
-           "ffn_weights_from_reference")
+    _enqueue("ffn_weights_from_reference", lib().moe_b200_ffn_weights_from_reference, _device_of(w1), stream, _ptr(w1),
+             _ptr(w2), E, d, F, _ptr(w_up), _ptr(w_down))
     return w_up, w_down
 
 
@@ -479,8 +512,8 @@ class RouterWeights:
             raise MoEB200Error(ERR_INVALID_ARG, f"RouterWeights: bad shape d={self.d} E={self.E}")
         self.buf, w_gate = _fresh(w_gate.device, stream, lambda: (
             torch.empty(nbytes, dtype=torch.uint8, device=w_gate.device), w_gate.contiguous()))
-        _check(lib().moe_b200_router_prepare(_ptr(w_gate), self.d, self.E, dtype_code(dtype),
-                                             _ptr(self.buf), _stream_handle(stream)), "router_prepare")
+        _enqueue("router_prepare", lib().moe_b200_router_prepare, _device_of(w_gate), stream, _ptr(w_gate), self.d, self.E,
+                 dtype_code(dtype), _ptr(self.buf))
 
 
 def route(x, weights, K, out=None, stream=None):
@@ -493,8 +526,8 @@ def route(x, weights, K, out=None, stream=None):
     if out is None:
         out = _fresh(x.device, stream, lambda: (torch.empty((T, K), dtype=torch.int32, device=x.device),
                                                 torch.empty((T, K), dtype=torch.float32, device=x.device)))
-    _check(lib().moe_b200_route(_ptr(x), T, d, weights.E, K, dtype_code(x.dtype), _ptr(weights.buf),
-                                _ptr(out[0]), _ptr(out[1]), _stream_handle(stream)), "route")
+    _enqueue("route", lib().moe_b200_route, _device_of(x), stream, _ptr(x), T, d, weights.E, K, dtype_code(x.dtype),
+             _ptr(weights.buf), _ptr(out[0]), _ptr(out[1]))
     return out
 
 
@@ -513,8 +546,8 @@ def ep_layout(all_counts, rank, expert_first, out=None, stream=None):
                                            torch.empty(N, dtype=torch.int32, device=dev),
                                            torch.empty(N, dtype=torch.int32, device=dev)))
     first = (ctypes.c_int32 * (N + 1))(*expert_first)
-    _check(lib().moe_b200_ep_layout(_ptr(all_counts), N, E, rank, first, _ptr(out[0]), _ptr(out[1]),
-                                    _ptr(out[2]), _ptr(out[3]), _stream_handle(stream)), "ep_layout")
+    _enqueue("ep_layout", lib().moe_b200_ep_layout, _device_of(all_counts), stream, _ptr(all_counts), N, E, rank, first,
+             _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _ptr(out[3]))
     return out
 
 
@@ -542,24 +575,6 @@ def _same_device(what, *tensors):
         if t is not None and (t.get_device() != index or index < 0):
             _refuse(what, f"tensors must be on one CUDA device, got {tensors[0].device} and {t.device}")
     return tensors[0].device
-
-
-def _on_device(dev, fn, *args):
-    """fn(*args) with `dev` current."""
-    import torch
-    if torch._C._cuda_getDevice() == dev.index:
-        return fn(*args)
-    with torch.cuda.device(dev):
-        return fn(*args)
-
-
-def _enqueue(what, fn, dev, stream, *args):
-    """Calls fn(*args, stream) with `dev` current."""
-    import torch
-    handle = torch._C._cuda_getCurrentRawStream(dev.index) or None if stream is None else _stream_handle(stream)
-    status = _on_device(dev, fn, *args, handle)
-    if status != OK:
-        _check(status, what)
 
 
 def _row_stride(what, name, t, shape, dtype):
@@ -644,9 +659,13 @@ def block_norm(residual, y=None, w_post=None, w_pre=None, gate=None, scale=1.0, 
     dev = _same_device("block_norm", residual, y, w_post, w_pre, gate)
     if out is None:
         like, plain = torch.empty_like, torch.contiguous_format
-        out = _fresh(dev, stream, lambda: BlockNormResult(
-            like(residual, memory_format=plain) if y is not None else None,
-            like(residual, dtype=dtype, memory_format=plain) if w_pre is not None else None))
+
+        def alloc():
+            return BlockNormResult(
+                like(residual, memory_format=plain) if y is not None else None,
+                like(residual, dtype=dtype, memory_format=plain) if w_pre is not None else None)
+
+        out = alloc() if stream is None else _fresh(dev, stream, alloc)
     else:
         if (out.residual_out is None) != (y is None) or (out.normed is None) != (w_pre is None):
             _refuse("block_norm", "out needs residual_out with y and normed with w_pre, and neither without")
@@ -687,20 +706,23 @@ def block_norm_backward(d_residual_out, d_normed, residual_out, y=None, w_post=N
 
     like, plain = torch.empty_like, torch.contiguous_format
     f32 = torch.float32
-    *got, ws = _fresh(dev, stream, lambda: (
-        like(residual_out, memory_format=plain),
-        like(y, memory_format=plain) if y is not None else None,
-        like(w_post, dtype=f32) if w_post is not None else None,
-        like(w_pre, dtype=f32) if w_pre is not None else None,
-        None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32),
-        residual_out.new_empty((max(nbytes, 256),), dtype=torch.uint8)))
-    got = BlockNormGrads(*got)
+
+    def alloc():
+        return BlockNormGrads(
+            like(residual_out, memory_format=plain),
+            like(y, memory_format=plain) if y is not None else None,
+            like(w_post, dtype=f32) if w_post is not None else None,
+            like(w_pre, dtype=f32) if w_pre is not None else None,
+            None if gate is None else like(gate) if form == GATE_FULL else like(gate, dtype=f32))
+
+    got = alloc() if stream is None else _fresh(dev, stream, alloc)
     if T == 0:  # sums over no token
         with torch.cuda.stream(_other_stream(dev, stream)):
             for t in got[2:]:
                 if t is not None:
                     t.zero_()
         return got
+    ws = _new(residual_out, (max(nbytes, 256),), dev, stream, torch.uint8)
     _enqueue(what, lib().moe_b200_block_norm_backward, dev, stream,
              _ptr(d_residual_out), _ptr(d_normed), _ptr(residual_out), res_stride, res32, _ptr(y), y_stride,
              _ptr(w_post), _ptr(w_pre), _ptr(gate), form, scale, eps, T, d, code, _ptr(got.d_residual),
@@ -727,7 +749,7 @@ def _grouped_mm(what, fn, rows_in, seg_start, w, seg_expert, out, stream, forwar
         _refuse(what, f"{nseg} segments for {E} experts need seg_expert")
     dev = _same_device(what, rows_in, seg_start, w, seg_expert, out)
     if out is None:
-        out, = _fresh(dev, stream, lambda: (rows_in.new_empty((rows, width_out)),))
+        out = _new(rows_in, (rows, width_out), dev, stream)
     else:
         _rows(what, "out", out, (rows, width_out), dtype)
     _enqueue(what, fn, dev, stream, _ptr(rows_in), _ptr(seg_start), _ptr(seg_expert), nseg, rows, N, K, E,
@@ -769,7 +791,7 @@ def grouped_mm_wgrad(dy, x, seg_start, out=None, stream=None):
     _rows(what, "seg_start", seg_start, (nseg + 1,), torch.int32)
     dev = _same_device(what, x, dy, seg_start, out)
     if out is None:
-        out, = _fresh(dev, stream, lambda: (x.new_empty((nseg, N, K)),))
+        out = _new(x, (nseg, N, K), dev, stream)
     else:
         _rows(what, "out", out, (nseg, N, K), dtype)
     _enqueue(what, lib().moe_b200_grouped_mm_wgrad, dev, stream, _ptr(dy), _ptr(x), _ptr(seg_start), nseg, rows,
@@ -811,7 +833,7 @@ def expert_linear_w4(x, asgn, w_q, w_scale, w_zero=None, act=None, out=None, str
     n_out = N // 2 if act else N
     dev = _same_device(what, x, asgn, w_q, w_scale, w_zero, out)
     if out is None:
-        out, = _fresh(dev, stream, lambda: (x.new_empty((T * K, n_out)),))
+        out = _new(x, (T * K, n_out), dev, stream)
     else:
         _rows(what, "out", out, (T * K, n_out), dtype)
     _enqueue(what, lib().moe_b200_expert_linear_w4, dev, stream,
